@@ -8,11 +8,14 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = PRODUCT_LIB = os.path.join(HERE, "libasyrp_hip.so")
 BENCH_LIB = os.path.join(HERE, "libasyrp_hip_bench.so")
-SOURCES = ["kernels.hip", "conv_f16x3.hip", "conv_out.hip", "conv_in.hip", "gemm1x1.hip", "attention.hip", "backward.hip", "engine.hip"]
+SOURCES = ["kernels.hip", "conv_f16x3.hip", "conv_out.hip", "conv_in.hip", "gemm1x1.hip", "attention.hip", "backward.hip", "packed_attention.hip", "residual_norm.hip", "adamw.hip",
+           "engine.hip"]
 BENCH_SOURCES = SOURCES + ["bench_hooks.hip"]   # the profiling library only (-DASYRP_BENCH_HOOKS): micro-benchmark / phase-stamp entry points
 DEPS = BENCH_SOURCES + ["kernels.h", os.path.join("..", "..", "include", "asyrp.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared", "-Wno-comment",
-         "-fvisibility=hidden"]   # exports = the extern "C" entry points of include/asyrp.h (visibility pragma there)
+         "-fvisibility=hidden",   # exports = the extern "C" entry points of include/asyrp.h (visibility pragma there)
+         # no packed fp32 instructions: some of their forms have given wrong results on gfx950 (the host pass warns that it does not know the feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():

@@ -22,6 +22,20 @@ inline const char* ab_env(const char* name) {
 // records the calling thread's error string (what asyrp_last_error returns) and hands `code` back; defined in engine.hip
 int set_last_error(int code, const char* msg);
 
+// makes `device` current for the scope of an entry point and the caller's device again behind it
+struct DeviceGuard {
+  int old = -1;
+  hipError_t error;
+  explicit DeviceGuard(int device) {
+    error = hipGetDevice(&old);
+    if (error == hipSuccess && old != device) error = hipSetDevice(device);
+    else old = -1;
+  }
+  ~DeviceGuard() { if (old >= 0) (void)hipSetDevice(old); }
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
 // One implicit-GEMM launch: out[z][m][n] = alpha * sum_k A[z][m][k] * B[(z)][k][n] (+bias +chan_add +resid)
 //   A = activations, NHWC, up to two channel-concatenated sources, optional per-(image,channel)
 //       affine (GroupNorm apply / FiLM) + SiLU prologue, optional nearest-x2 upsample, 3x3 halo via LDS.

@@ -1,0 +1,496 @@
+// residual_norm.hip -- the seam between two residual blocks in one pass: the norm behind a block, its gate, the residual sum with its scale
+// and the norm in front of the next block, forward and backward.
+//
+//   u = N1(y) (or y),   h = a x + gate * u,   n = N2(h),   N(t) = (t - mean) rstd * w + b  (layer)  or  t rstd * w + b  (rms)
+//
+// backward, with that = (t - mean) rstd and c = d that = d out * w:   d t = rstd (c - mean(c) - that mean(c that))   (rms: no mean(c)):
+//   dh' = dh + N2'(dn),  dx = a dh',  dgate = sum over the gate's rows of dh' u,  dy = N1'(gate dh'),  dw = sum over rows of d out * that
+//
+// The work is bound by HBM: forward 2 reads and 2 writes of [rows, C], backward 4 reads and 2 writes (x and y are read again
+// instead of h: h as stored is rounded to the stream's type, and the statistics and that belong to the unrounded one).  A row lives in
+// registers from the first load to the last store.  Statistics, sums and the partial sums of the parameter gradients are fp32;
+// mean and variance are taken in two passes over the registers, so no large sum of squares cancels.  Parameter gradients go
+// through per-workgroup partial sums and a second kernel that adds them in a fixed order: no atomics.
+#include "kernels.h"
+#include "../../include/asyrp.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace asyrp {
+namespace {
+
+struct NormArgs {
+  const void *x, *y, *dh, *dn;
+  void *h, *n, *dx, *dy;
+  const float *gate, *w1, *b1, *w2, *b2;
+  float *stats;              // [rows][4]: mean and rstd of y, mean and rstd of h (null: not kept)
+  float *partial;            // [slots][vectors][C]
+  float *dgate;
+  float a, eps;
+  long long rows, per_gate;  // rows of one gate row
+  int C, after, before, rms; // which norms there are
+  int chunks;                // workgroups per gate row (1 where a workgroup takes whole gate rows)
+  long long gates_per_wg, chunk_rows, gates;
+  int want_w1, want_b1, want_w2, want_b2, want_gate;
+};
+// partial vectors, in this order
+enum { V_W2, V_B2, V_W1, V_B1, V_GATE, VECTORS };
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f(__bf16 v) { return (float)v; }
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// eight values of a row: contiguous and 16-byte aligned (VEC), or `TPR` apart so that neighbouring lanes still read neighbouring values
+template <typename T, bool VEC, int TPR>
+__device__ __forceinline__ void load8(const T* row, int slot, int t, int C, float (&o)[8]) {
+  if (VEC) {
+    const int c = (slot * TPR + t) * 8;
+    if (c < C) {
+      union { u32x4 u[sizeof(T) / 2]; T v[8]; } x;
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.u[i] = reinterpret_cast<const u32x4*>(row + c)[i];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = to_f(x.v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = (slot * 8 + j) * TPR + t;
+      o[j] = c < C ? to_f(row[c]) : 0.f;
+    }
+  }
+}
+template <typename T, bool VEC, int TPR>
+__device__ __forceinline__ void store8(T* row, int slot, int t, int C, const float (&o)[8]) {
+  if (VEC) {
+    const int c = (slot * TPR + t) * 8;
+    if (c < C) {
+      union { u32x4 u[sizeof(T) / 2]; T v[8]; } x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x.v[j] = (T)o[j];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<u32x4*>(row + c)[i] = x.u[i];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = (slot * 8 + j) * TPR + t;
+      if (c < C) row[c] = (T)o[j];
+    }
+  }
+}
+template <bool VEC, int TPR>
+__device__ __forceinline__ bool in8(int slot, int t, int j, int C) {
+  return VEC ? (slot * TPR + t) * 8 < C : (slot * 8 + j) * TPR + t < C;
+}
+
+// sums of K values over the TPR threads of a row.  `buf` holds two sets of one row of K values per wave, used in turn, so that
+// one barrier per reduction is enough.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* buf, int& turn, int sub, int t) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o);
+  if (TPR > 64) {
+    constexpr int W = TPR / 64;
+    float* b = buf + (turn * 16 + sub * W) * 2;
+    turn ^= 1;
+    if ((t & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; ++k) b[(t >> 6) * 2 + k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += b[w * 2 + k];
+      v[k] = s;
+    }
+  }
+}
+
+// mean and rstd of the values (those behind C are zero and do not count)
+template <bool VEC, int TPR, int NV>
+__device__ __forceinline__ void statistics(const float (&v)[NV][8], const NormArgs& p, float* buf, int& turn, int sub, int t, float& mean, float& rstd) {
+  mean = 0.f;
+  float s[1] = {0.f};
+  if (!p.rms) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[0] += v[i][j];
+    row_sum<TPR, 1>(s, buf, turn, sub, t);
+    mean = s[0] / (float)p.C;
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (in8<VEC, TPR>(i, t, j, p.C)) s[0] += (v[i][j] - mean) * (v[i][j] - mean);
+  row_sum<TPR, 1>(s, buf, turn, sub, t);
+  rstd = 1.0f / sqrtf(s[0] / (float)p.C + p.eps);
+}
+
+template <typename X, typename Y, bool VEC, int TPR, int NV>
+__global__ __launch_bounds__(256) void residual_norm_fwd_kernel(const NormArgs p) {
+  __shared__ float buf[64];
+  constexpr int SUB = 256 / TPR;
+  const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
+  long long row = (long long)blockIdx.x * SUB + sub;
+  const bool there = row < p.rows;
+  if (TPR == 64 && !there) return;
+  if (!there) row = p.rows - 1;
+  int turn = 0;
+  float x[NV][8], y[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load8<Y, VEC, TPR>((const Y*)p.y + row * C, i, t, C, y[i]);
+    load8<X, VEC, TPR>((const X*)p.x + row * C, i, t, C, x[i]);
+  }
+  float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
+  if (p.after) {
+    statistics<VEC, TPR, NV>(y, p, buf, turn, sub, t, m1, r1);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float w[8], b[8];
+      if (p.w1) load8<float, VEC, TPR>(p.w1, i, t, C, w);
+      if (p.b1) load8<float, VEC, TPR>(p.b1, i, t, C, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v = (y[i][j] - m1) * r1;
+        if (p.w1) v *= w[j];
+        if (p.b1) v += b[j];
+        y[i][j] = v;
+      }
+    }
+  }
+  const float* gate = p.gate ? p.gate + (row / p.per_gate) * C : nullptr;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float g[8];
+    if (gate) load8<float, VEC, TPR>(gate, i, t, C, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float u = gate ? y[i][j] * g[j] : y[i][j];
+      x[i][j] = in8<VEC, TPR>(i, t, j, C) ? p.a * x[i][j] + u : 0.f;
+    }
+    if (there) store8<X, VEC, TPR>((X*)p.h + row * C, i, t, C, x[i]);
+  }
+  if (p.before) {
+    statistics<VEC, TPR, NV>(x, p, buf, turn, sub, t, m2, r2);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float w[8], b[8];
+      if (p.w2) load8<float, VEC, TPR>(p.w2, i, t, C, w);
+      if (p.b2) load8<float, VEC, TPR>(p.b2, i, t, C, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v = (x[i][j] - m2) * r2;
+        if (p.w2) v *= w[j];
+        if (p.b2) v += b[j];
+        x[i][j] = v;
+      }
+      if (there) store8<Y, VEC, TPR>((Y*)p.n + row * C, i, t, C, x[i]);
+    }
+  }
+  if (p.stats && there && t == 0) reinterpret_cast<float4*>(p.stats)[row] = make_float4(m1, r1, m2, r2);
+}
+
+// One workgroup of max(256, TPR) threads walks over the rows of one part of a gate row, or of several whole gate rows, and keeps the
+// parameter gradients of its columns in registers.
+template <typename X, typename Y, bool VEC, int TPR>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kernel(const NormArgs p) {
+  constexpr int THREADS = TPR > 256 ? TPR : 256, SUB = THREADS / TPR;
+  __shared__ float buf[64];
+  __shared__ float join[SUB > 1 ? SUB * TPR * 8 : 1];
+  const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
+  int turn = 0;
+  float w1[8], w2[8], b1[8];
+  if (p.w1) load8<float, VEC, TPR>(p.w1, 0, t, C, w1);
+  if (p.b1) load8<float, VEC, TPR>(p.b1, 0, t, C, b1);
+  if (p.w2) load8<float, VEC, TPR>(p.w2, 0, t, C, w2);
+  float sw1[8], sb1[8], sw2[8], sb2[8], sg[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sw1[j] = sb1[j] = sw2[j] = sb2[j] = 0.f;
+  const long long g0 = (long long)(blockIdx.x / p.chunks) * p.gates_per_wg, g1 = min(p.gates, g0 + p.gates_per_wg);
+  const int part = blockIdx.x % p.chunks;
+  float* slot = p.partial + (long long)blockIdx.x * VECTORS * C;
+
+  // adds the row groups' sums of one vector and writes it (join is free again behind it)
+  auto put = [&](float (&v)[8], float* to) {
+    if (SUB > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) join[(sub * 8 + j) * TPR + t] = v[j];
+      __syncthreads();
+      if (sub == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          for (int s = 1; s < SUB; ++s) v[j] += join[(s * 8 + j) * TPR + t];
+    }
+    if (sub == 0) store8<float, VEC, TPR>(to, 0, t, C, v);
+  };
+
+  for (long long g = g0; g < g1; ++g) {
+    const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
+    float gate[8];
+    if (p.gate) load8<float, VEC, TPR>(p.gate + g * C, 0, t, C, gate);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sg[j] = 0.f;
+    for (long long r0 = first; r0 < last; r0 += SUB) {
+      const bool there = r0 + sub < last;
+      const long long row = there ? r0 + sub : last - 1;
+      float x[8], y[8], dh[8], dn[8];
+      load8<Y, VEC, TPR>((const Y*)p.y + row * C, 0, t, C, y);
+      load8<X, VEC, TPR>((const X*)p.x + row * C, 0, t, C, x);
+      if (p.dn) load8<Y, VEC, TPR>((const Y*)p.dn + row * C, 0, t, C, dn);
+      if (p.dh) load8<X, VEC, TPR>((const X*)p.dh + row * C, 0, t, C, dh);
+      const float4 st = reinterpret_cast<const float4*>(p.stats)[row];
+      float u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (!p.dh) dh[j] = 0.f;
+        y[j] = p.after ? (y[j] - st.x) * st.y : y[j];
+        u[j] = y[j];
+        if (p.after && p.w1) u[j] *= w1[j];
+        if (p.after && p.b1) u[j] += b1[j];
+      }
+      if (p.before && p.dn) {
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = in8<VEC, TPR>(0, t, j, C);
+          const float hat = (p.a * x[j] + (p.gate ? u[j] * gate[j] : u[j]) - st.z) * st.w;
+          x[j] = in ? hat : 0.f;
+          if (there) {
+            sw2[j] += dn[j] * x[j];
+            sb2[j] += dn[j];
+          }
+          if (p.w2) dn[j] *= w2[j];
+          s[0] += dn[j];
+          s[1] += dn[j] * x[j];
+        }
+        row_sum<TPR, 2>(s, buf, turn, sub, t);
+        const float c1 = p.rms ? 0.f : s[0] / (float)C, c2 = s[1] / (float)C;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dh[j] += st.w * (dn[j] - c1 - x[j] * c2);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = p.a * dh[j];
+      if (there && p.dx) store8<X, VEC, TPR>((X*)p.dx + row * C, 0, t, C, x);
+      if (p.gate) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (there) sg[j] += dh[j] * u[j];
+          dh[j] *= gate[j];
+        }
+      }
+      if (p.after) {
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (!in8<VEC, TPR>(0, t, j, C)) y[j] = dh[j] = 0.f;
+          if (there) {
+            sw1[j] += dh[j] * y[j];
+            sb1[j] += dh[j];
+          }
+          if (p.w1) dh[j] *= w1[j];
+          s[0] += dh[j];
+          s[1] += dh[j] * y[j];
+        }
+        row_sum<TPR, 2>(s, buf, turn, sub, t);
+        const float c1 = p.rms ? 0.f : s[0] / (float)C, c2 = s[1] / (float)C;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dh[j] = st.y * (dh[j] - c1 - y[j] * c2);
+      }
+      if (there && p.dy) store8<Y, VEC, TPR>((Y*)p.dy + row * C, 0, t, C, dh);
+    }
+    if (p.want_gate) put(sg, p.chunks == 1 ? p.dgate + g * C : slot + V_GATE * C);
+  }
+  if (p.want_w2) put(sw2, slot + V_W2 * C);
+  if (p.want_b2) put(sb2, slot + V_B2 * C);
+  if (p.want_w1) put(sw1, slot + V_W1 * C);
+  if (p.want_b1) put(sb1, slot + V_B1 * C);
+}
+
+// column sums of the partial vectors: 64 columns per workgroup, its four waves take every fourth slot
+struct NormSumArgs {
+  const float* partial;
+  float* out[VECTORS];
+  int C, slots;              // slots of the weights' gradients
+  int chunks;                // slots of one gate row
+  long long gates;
+};
+__global__ __launch_bounds__(256) void residual_norm_sum_kernel(const NormSumArgs p) {
+  __shared__ float part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  const bool gate = blockIdx.y >= V_GATE;
+  const int v = gate ? V_GATE : blockIdx.y;
+  const long long g = gate ? blockIdx.y - V_GATE : 0;
+  if (!p.out[v]) return;
+  const long long s0 = gate ? g * p.chunks : 0, n = gate ? p.chunks : p.slots;
+  float s = 0.f;
+  if (c < p.C)
+    for (long long i = wave; i < n; i += 4) s += p.partial[((s0 + i) * VECTORS + v) * p.C + c];
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < p.C) p.out[v][g * p.C + c] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+}
+
+template <typename X, typename Y, bool VEC>
+hipError_t forward(const NormArgs& a, hipStream_t s) {
+  const dim3 b(256), g4((unsigned)((a.rows + 3) / 4)), g1((unsigned)a.rows);
+  if (a.C <= 512) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 64, 1>), g4, b, 0, s, a);
+  else if (a.C <= 1024) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 64, 2>), g4, b, 0, s, a);
+  else if (a.C <= 2048) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 64, 4>), g4, b, 0, s, a);
+  else if (a.C <= 4096) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 256, 2>), g1, b, 0, s, a);
+  else hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 256, 4>), g1, b, 0, s, a);
+  return hipGetLastError();
+}
+template <typename X, typename Y, bool VEC>
+hipError_t backward(const NormArgs& a, unsigned wgs, hipStream_t s) {
+  const dim3 g(wgs);
+  if (a.C <= 512) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 64>), g, dim3(256), 0, s, a);
+  else if (a.C <= 1024) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 128>), g, dim3(256), 0, s, a);
+  else if (a.C <= 2048) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 256>), g, dim3(256), 0, s, a);
+  else if (a.C <= 4096) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 512>), g, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 1024>), g, dim3(1024), 0, s, a);
+  return hipGetLastError();
+}
+template <typename X, typename Y>
+hipError_t launch(const NormArgs& a, bool vec, bool back, unsigned wgs, hipStream_t s) {
+  if (back) return vec ? backward<X, Y, true>(a, wgs, s) : backward<X, Y, false>(a, wgs, s);
+  return vec ? forward<X, Y, true>(a, s) : forward<X, Y, false>(a, s);
+}
+bool types(int x, int y) { return (x == ASYRP_F32 && (y == ASYRP_F32 || y == ASYRP_F16 || y == ASYRP_BF16)) || (x == y && (x == ASYRP_F16 || x == ASYRP_BF16)); }
+hipError_t dispatch(int x, int y, const NormArgs& a, bool vec, bool back, unsigned wgs, hipStream_t s) {
+  if (x == ASYRP_F32 && y == ASYRP_F32) return launch<float, float>(a, vec, back, wgs, s);
+  if (x == ASYRP_F32 && y == ASYRP_F16) return launch<float, _Float16>(a, vec, back, wgs, s);
+  if (x == ASYRP_F32) return launch<float, __bf16>(a, vec, back, wgs, s);
+  return x == ASYRP_F16 ? launch<_Float16, _Float16>(a, vec, back, wgs, s) : launch<__bf16, __bf16>(a, vec, back, wgs, s);
+}
+
+int refuse(const char* m) { return set_last_error(ASYRP_EINVAL, m); }
+
+int check(const asyrp_residual_norm* p) {
+  if (!p) return refuse("residual norm: null argument");
+  if (!types(p->stream_dtype, p->branch_dtype)) return refuse("residual norm: types are f32 with any branch, or f16 / bf16 for both");
+  if (p->rows < 0 || p->rows > 0x7fffffffLL) return refuse("residual norm: bad number of rows");
+  if (p->width < 1 || p->width > 8192) return refuse("residual norm: the width must be 1 .. 8192");
+  if (p->kind != ASYRP_NORM_LAYER && p->kind != ASYRP_NORM_RMS) return refuse("residual norm: unknown kind of norm");
+  if (p->gates < 0 || (p->gates > 0 && p->rows % p->gates)) return refuse("residual norm: the gate's rows must divide the rows");
+  if (!std::isfinite(p->eps) || p->eps < 0 || !std::isfinite(p->residual_scale)) return refuse("residual norm: eps and the residual scale must be finite");
+  return 0;
+}
+// How the backward's rows are dealt out: 1024 workgroups (four per CU) where the rows allow, each with a part of one gate row
+// or with several whole ones; at least 16 rows each, so that the partial sums stay a small part of the traffic.
+void deal(const asyrp_residual_norm* p, NormArgs& a, unsigned& wgs) {
+  a.gates = p->gates > 0 ? p->gates : 1;
+  a.per_gate = std::max<long long>(1, a.rows / a.gates);
+  const long long want = std::max<long long>(1, std::min<long long>(1024, a.rows / 16));
+  a.chunks = (int)std::max<long long>(1, std::min(want / a.gates, a.per_gate));
+  a.chunk_rows = (a.per_gate + a.chunks - 1) / a.chunks;
+  a.chunks = (int)((a.per_gate + a.chunk_rows - 1) / a.chunk_rows);
+  a.gates_per_wg = a.chunks > 1 ? 1 : (a.gates + want - 1) / want;
+  wgs = (unsigned)(((a.gates + a.gates_per_wg - 1) / a.gates_per_wg) * a.chunks);
+}
+void fill(const asyrp_residual_norm* p, NormArgs& a) {
+  a.rows = p->rows;
+  a.C = p->width;
+  a.rms = p->kind == ASYRP_NORM_RMS;
+  a.after = p->after != 0;
+  a.before = p->before != 0;
+  a.a = p->residual_scale;
+  a.eps = p->eps;
+  a.per_gate = p->gates > 0 ? std::max<long long>(1, p->rows / p->gates) : std::max<long long>(1, p->rows);
+}
+bool aligned(std::initializer_list<const void*> ps) {
+  for (const void* q : ps)
+    if ((uintptr_t)q & 15) return false;
+  return true;
+}
+
+}  // namespace
+}  // namespace asyrp
+
+using namespace asyrp;
+
+extern "C" {
+
+int asyrp_residual_norm_forward(int device, const asyrp_residual_norm* p, const void* x, const void* y, const float* gate, const float* after_weight,
+                                const float* after_bias, const float* before_weight, const float* before_bias, void* h, void* n, float* stats, void* stream) {
+  if (int rc = check(p)) return rc;
+  if (p->rows == 0) return 0;
+  if (!x || !y || !h || (p->before && !n) || (p->gates > 0) != (gate != nullptr)) return refuse("residual norm: null argument");
+  NormArgs a{};
+  fill(p, a);
+  a.x = x; a.y = y; a.gate = gate; a.w1 = after_weight; a.b1 = after_bias; a.w2 = before_weight; a.b2 = before_bias; a.h = h; a.n = n; a.stats = stats;
+  if (!aligned({stats})) return refuse("residual norm: the statistics must be 16-byte aligned");
+  const bool vec = a.C % 8 == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, before_bias, h, n});
+  DeviceGuard g(device);
+  if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
+  const hipError_t e = dispatch(p->stream_dtype, p->branch_dtype, a, vec, false, 0, (hipStream_t)stream);
+  return e == hipSuccess ? 0 : set_last_error(ASYRP_EHIP, hipGetErrorString(e));
+}
+
+int64_t asyrp_residual_norm_workspace(const asyrp_residual_norm* p) {
+  if (int rc = check(p)) return rc;
+  NormArgs a{};
+  fill(p, a);
+  unsigned wgs = 0;
+  deal(p, a, wgs);
+  return (int64_t)wgs * VECTORS * a.C;
+}
+
+int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const void* x, const void* y, const float* gate, const float* after_weight,
+                                 const float* after_bias, const float* before_weight, const float* stats, const void* dh, const void* dn, void* dx, void* dy,
+                                 float* dgate, float* d_after_weight, float* d_after_bias, float* d_before_weight, float* d_before_bias, float* workspace,
+                                 void* stream) {
+  if (int rc = check(p)) return rc;
+  float* outs[VECTORS] = {d_before_weight, d_before_bias, d_after_weight, d_after_bias, dgate};
+  if (p->rows > 0 && (!x || !y || !stats || !workspace || (!dh && !dn) || (p->gates > 0) != (gate != nullptr) || (dgate && !gate)))
+    return refuse("residual norm: null argument");
+  if ((dn && !p->before) || ((d_after_weight || d_after_bias) && !p->after) || ((d_before_weight || d_before_bias) && !p->before))
+    return refuse("residual norm: a gradient of a norm that is not there");
+  if (p->rows == 0) return 0;
+  if (!aligned({stats})) return refuse("residual norm: the statistics must be 16-byte aligned");
+  NormArgs a{};
+  fill(p, a);
+  unsigned wgs = 0;
+  deal(p, a, wgs);
+  a.x = x; a.y = y; a.gate = gate; a.w1 = after_weight; a.b1 = after_bias; a.w2 = before_weight; a.stats = const_cast<float*>(stats);
+  a.dh = dh; a.dn = dn; a.dx = dx; a.dy = dy; a.partial = workspace; a.dgate = dgate;
+  a.want_w2 = d_before_weight != nullptr; a.want_b2 = d_before_bias != nullptr; a.want_w1 = d_after_weight != nullptr; a.want_b1 = d_after_bias != nullptr;
+  a.want_gate = dgate != nullptr;
+  const bool vec = a.C % 8 == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, dh, dn, dx, dy, dgate, workspace});
+  DeviceGuard g(device);
+  if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
+  hipError_t e = dispatch(p->stream_dtype, p->branch_dtype, a, vec, true, wgs, (hipStream_t)stream);
+  if (e == hipSuccess) {
+    NormSumArgs sa{};
+    sa.partial = workspace;
+    for (int i = 0; i < VECTORS; ++i) sa.out[i] = outs[i];
+    sa.C = a.C;
+    sa.slots = (int)wgs;
+    sa.chunks = a.chunks;
+    sa.gates = a.gates;
+    if (a.chunks == 1) sa.out[V_GATE] = nullptr;     // whole gate rows were written by the kernel itself
+    bool any = false;
+    for (float* o : sa.out) any = any || o;
+    if (any) {
+      hipLaunchKernelGGL(residual_norm_sum_kernel, dim3((a.C + 63) / 64, V_GATE + (sa.out[V_GATE] ? (unsigned)a.gates : 0)), dim3(256), 0, (hipStream_t)stream, sa);
+      e = hipGetLastError();
+    }
+  }
+  return e == hipSuccess ? 0 : set_last_error(ASYRP_EHIP, hipGetErrorString(e));
+}
+
+}  // extern "C"

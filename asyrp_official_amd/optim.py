@@ -1,0 +1,237 @@
+"""AdamW over many tensors at once on the HIP library (csrc/adamw.hip): the optimiser of the DeltaBlock training step.
+
+The reference steps its DeltaBlock with a torch optimiser (diffusion_latent.py:288-290, 349-350).  `AdamW` takes the same place:
+    opt = AdamW(model.layer_0.parameters(), lr=1e-4, state_bits=8, max_norm=1.0)
+    opt.zero_grad(); loss.backward(); opt.step()
+"""
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .engine import AsyrpDeviceError, _ptr
+
+BLOCK = 256          # values that share one exponent of the 8-bit moments; every parameter's moments start on a multiple of it
+
+
+class _Moments:
+    """The flat moments of one parameter group: parameter i's values lie at offsets[i]."""
+
+    def __init__(self, params, bits, device):
+        self.params, self.bits, self.device = list(params), bits, device
+        self.numels = [p.numel() for p in self.params]
+        self.offsets, n = [], 0
+        for k in self.numels:
+            self.offsets.append(n)
+            n += -(-k // BLOCK) * BLOCK
+        self.n = n
+        if bits == 32:
+            self.m, self.v = (torch.zeros(n, device=device, dtype=torch.float32) for _ in range(2))
+            self.me = self.ve = None
+        else:
+            self.m, self.v = (torch.zeros(n, device=device, dtype=torch.uint8) for _ in range(2))
+            self.me, self.ve = (torch.zeros(n // BLOCK, device=device, dtype=torch.uint8) for _ in range(2))
+        self.steps = torch.zeros(max(1, len(self.params)), device=device, dtype=torch.int32)
+
+    def views(self, i):
+        """What self.state holds of parameter i: views of the flat moments (8 bits: codes and exponent bytes)."""
+        at, k, p = self.offsets[i], self.numels[i], self.params[i]
+        d = {"step": self.steps[i], "exp_avg": self.m[at:at + k].view(p.shape), "exp_avg_sq": self.v[at:at + k].view(p.shape)}
+        if self.bits == 8:
+            e = slice(at // BLOCK, at // BLOCK + -(-k // BLOCK))
+            d["exp_avg_scale"], d["exp_avg_sq_scale"] = self.me[e], self.ve[e]
+        return d
+
+
+class AdamW(torch.optim.Optimizer):
+    """One step: p <- p (1 - lr weight_decay) - lr m^ / (sqrt(v^) + eps) with bias-corrected moments (decoupled weight decay), for every parameter that has a
+    gradient, in a few launches whatever their number.
+
+    params: float32, float16 or bfloat16 parameters on one GPU, contiguous; gradients of the same type.  state_bits: 32, or 8 (blocks of 256
+    values with a power-of-two scale each, rounded at random by the counter hash of csrc/adamw.hip under `seed`; two runs with one seed are alike to the bit).
+    max_norm: clips all gradients by their global norm (factor min(1, max_norm / (norm + 1e-6))); the gradients themselves keep
+    their values, `grad_norm` (device, float32) holds the last norm, and a step whose norm is not finite changes nothing, its step counts included.
+    Without max_norm values that are not finite go their way into the parameters; 8-bit moments keep a block that holds one as NaN.
+
+    Step counts, moments and the norm live on the device, so a step may be captured into a graph once the moments are there (after the first step, or
+    `prepare()`); gradients then have to keep their addresses, and lr, where it changes, has to be a float32 tensor on the device (it is
+    read when the step runs)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if max_norm is not None and not 0.0 < float(max_norm) < float("inf"):
+            raise ValueError(f"max_norm must be positive and finite, got {max_norm}")
+        self.state_bits, self.max_norm, self.seed = int(state_bits), None if max_norm is None else float(max_norm), int(seed) & 0xFFFFFFFF
+        self.grad_norm, self._moments = None, {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_group(g):
+        b1, b2 = g["betas"]
+        if isinstance(g["lr"], torch.Tensor):
+            if g["lr"].numel() != 1:
+                raise ValueError("lr as a tensor holds one value")
+        elif not 0.0 <= g["lr"] < float("inf"):
+            raise ValueError(f"lr must be finite and not negative, got {g['lr']}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"betas must lie in [0, 1), got {g['betas']}")
+        if not 0.0 <= g["eps"] < float("inf") or not 0.0 <= g["weight_decay"] < float("inf"):
+            raise ValueError("eps and weight_decay must be finite and not negative")
+        for p in g["params"]:
+            if p.dtype not in _lib.DTYPES:
+                raise ValueError(f"parameters must be float32, float16 or bfloat16, got {p.dtype}")
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "max_norm": self.max_norm, "seed": self.seed}
+
+    def __setstate__(self, st):
+        super().__setstate__(st)
+        self.grad_norm, self._moments = None, {}          # rebuilt from self.state
+
+    # ---- moments ---------------------------------------------------------------------------------------
+    def _device(self):
+        dev = None
+        for g in self.param_groups:
+            for p in g["params"]:
+                if not p.is_cuda:
+                    raise AsyrpDeviceError("AdamW steps only parameters on an MI355X (device type 'cuda' under ROCm): there is no CPU path")
+                if dev is not None and p.device != dev:
+                    raise AsyrpDeviceError(f"parameters on {dev} and {p.device}: one optimiser steps one device")
+                dev = p.device
+        return dev
+
+    def _group_moments(self, k, device):
+        g, mo = self.param_groups[k], self._moments.get(k)
+        if mo is not None and mo.device == device and len(mo.params) == len(g["params"]) and all(a is b for a, b in zip(mo.params, g["params"])):
+            return mo
+        for p in g["params"]:
+            if not p.is_contiguous():
+                raise ValueError("parameters must be contiguous")
+        mo = _Moments(g["params"], self.state_bits, device)
+        for i, p in enumerate(mo.params):                 # moments that are there already: loaded ones, or those of an unpickled copy
+            views, old = mo.views(i), self.state.get(p) or {}
+            for key, view in views.items():
+                if key in old:
+                    view.copy_(torch.as_tensor(old[key]).reshape(view.shape))
+            self.state[p] = views
+        self._moments[k] = mo
+        return mo
+
+    def prepare(self):
+        """Allocates the moments (the first step does it otherwise)."""
+        device = self._device()
+        if device is not None:
+            with torch.no_grad():
+                for k in range(len(self.param_groups)):
+                    self._group_moments(k, device)
+
+    @torch.no_grad()
+    def moments(self):
+        """[(exp_avg, exp_avg_sq)] of each group as flat float32 tensors, every parameter's values filled up with zeros to a multiple of 256.  32-bit
+        moments are the optimiser's own buffers, 8-bit ones the values that their codes stand for."""
+        device, out = self._device(), []
+        for k in range(len(self.param_groups)):
+            mo = self._group_moments(k, device)
+            if mo.bits == 32:
+                out.append((mo.m, mo.v))
+                continue
+            m, v = (torch.empty(mo.n, device=device, dtype=torch.float32) for _ in range(2))
+            _lib.check(_lib.load().asyrp_adamw_moments(device.index, _ptr(mo.m), _ptr(mo.v), _ptr(mo.me), _ptr(mo.ve), mo.n, _ptr(m), _ptr(v), self._stream(device)))
+            out.append((m, v))
+        return out
+
+    def load_state_dict(self, state_dict):
+        """Takes what state_dict() of an optimiser with the same state_bits gave."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("loaded state dict has other parameter groups")
+        want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
+        pairs = [(i, p) for g, mine in zip(groups, self.param_groups) for i, p in zip(g["params"], mine["params"])]
+        for i, p in pairs:
+            st = saved.get(i)
+            if not st:
+                continue
+            if set(st) != want or tuple(st["exp_avg"].shape) != tuple(p.shape) or tuple(st["exp_avg_sq"].shape) != tuple(p.shape) \
+                    or (st["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
+                raise ValueError(f"loaded state of parameter {i} is not one of AdamW with {self.state_bits}-bit moments and shape {tuple(p.shape)}")
+        super().load_state_dict({"state": {}, "param_groups": groups})
+        self._moments = {}
+        for i, p in pairs:
+            if saved.get(i):
+                self.state[p] = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in saved[i].items()}
+
+    # ---- the step --------------------------------------------------------------------------------------
+    @staticmethod
+    def _stream(device):
+        return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        device = self._device()
+        if device is None:
+            return loss
+        lib, stream, todo = _lib.load(), self._stream(device), []
+        held = []                                          # copies of gradients laid out otherwise live until the launches are queued
+        for k, g in enumerate(self.param_groups):
+            mo = self._group_moments(k, device)
+            by_type = {}
+            for i, p in enumerate(mo.params):
+                grad = p.grad
+                if grad is None:
+                    continue
+                if grad.is_sparse or grad.dtype != p.dtype or grad.device != device or grad.shape != p.shape:
+                    raise ValueError(f"the gradient of a {p.dtype} parameter {tuple(p.shape)} must be dense, of its type, shape and device")
+                if not p.is_contiguous():
+                    raise ValueError("parameters must be contiguous")
+                if not grad.is_contiguous():
+                    grad = grad.contiguous()
+                    held.append(grad)
+                by_type.setdefault(p.dtype, []).append((p, grad, mo.numels[i], mo.offsets[i], i))
+            for dtype, rows in by_type.items():
+                flat = [v for p, grad, n, at, i in rows for v in (p.data_ptr(), grad.data_ptr(), n, at, i)]
+                todo.append((g, mo, _lib.DTYPES[dtype], len(rows), (C.c_int64 * len(flat))(*flat), [r[0] for r in rows]))
+        if not todo:
+            return loss
+        clip = None
+        if self.max_norm is not None:
+            counts = [-(-n // _lib.ADAMW_TABLE) * _lib.ADAMW_PARTIALS for _, _, _, n, _, _ in todo]
+            partial = torch.empty(sum(counts), device=device, dtype=torch.float64)
+            at = 0
+            for (_, _, dtype, n, table, _), c in zip(todo, counts):
+                _lib.check(lib.asyrp_grad_sumsq(device.index, table, n, dtype, C.c_void_p(partial.data_ptr() + 8 * at), stream))
+                at += c
+            both = torch.empty(4, device=device, dtype=torch.float32)
+            clip, self.grad_norm = both[0:2], both[2]
+            _lib.check(lib.asyrp_grad_clip(device.index, _ptr(partial), at, self.max_norm, _ptr(self.grad_norm), _ptr(clip), stream))
+        for g, mo, dtype, n, table, params in todo:
+            c = _lib.AdamWConfig()
+            lr = g["lr"]
+            if isinstance(lr, torch.Tensor) and lr.is_cuda:
+                if lr.dtype != torch.float32 or lr.device != device:
+                    raise ValueError(f"lr as a device tensor must be float32 on {device}")
+                c.lr_device, c.lr = lr.data_ptr(), 0.0
+            else:
+                c.lr = float(lr)
+            (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
+            c.steps, c.clip = mo.steps.data_ptr(), None if clip is None else clip.data_ptr()
+            c.exp_avg, c.exp_avg_sq = mo.m.data_ptr(), mo.v.data_ptr()
+            if mo.bits == 8:
+                c.exp_avg_scale, c.exp_avg_sq_scale = mo.me.data_ptr(), mo.ve.data_ptr()
+            c.state_bits, c.seed = mo.bits, self.seed
+            scratch = torch.empty(32 * n, device=device, dtype=torch.uint8)
+            _lib.check(lib.asyrp_adamw_step(device.index, C.byref(c), table, n, dtype, _ptr(scratch), stream))
+            torch.autograd.graph.increment_version(params)   # the engine re-uploads parameters whose version has moved
+        return loss

@@ -89,6 +89,57 @@ typedef struct asyrp_config {
 
 typedef struct asyrp_engine asyrp_engine;
 
+/* Element types of the stateless operators. */
+enum asyrp_dtype { ASYRP_F32 = 0, ASYRP_F16 = 1, ASYRP_BF16 = 2 };
+
+/* asyrp_packed_attention_*: tensors [tokens][heads][head_dim], the last axis contiguous, strides {token, head} in values and multiples
+ * of 8, addresses multiples of 16 bytes. */
+typedef struct asyrp_packed_attention {
+  int64_t tokens;                 /* rows of every tensor; those behind the last sequence belong to none */
+  int32_t sequences;
+  int32_t heads, kv_heads;        /* query head h reads key / value head h / (heads / kv_heads) */
+  int32_t head_dim;               /* multiple of 8, 8 .. 128 */
+  int32_t causal;
+  int32_t dtype;                  /* ASYRP_F16 or ASYRP_BF16 */
+  float scale;
+  int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2], dout_stride[2];
+} asyrp_packed_attention;
+
+/* asyrp_residual_norm_*: contiguous [rows][width]. */
+enum asyrp_norm_kind { ASYRP_NORM_LAYER = 0, ASYRP_NORM_RMS = 1 };
+typedef struct asyrp_residual_norm {
+  int64_t rows;
+  int64_t gates;                  /* rows of the gate: divides `rows`; 0 = no gate */
+  int32_t width;                  /* 1 .. 8192 */
+  int32_t kind;                   /* enum asyrp_norm_kind, of both norms */
+  int32_t after, before;          /* whether the norm behind the block / in front of the next one is there */
+  int32_t stream_dtype;           /* of x, h and their gradients */
+  int32_t branch_dtype;           /* of y, n and their gradients: any where the stream is f32, else the stream's */
+  float residual_scale, eps;
+} asyrp_residual_norm;
+
+/* asyrp_adamw_step: one tensor of the step, contiguous. */
+typedef struct asyrp_adamw_tensor {
+  void* param;
+  const void* grad;
+  int64_t numel;
+  int64_t offset;                 /* of its first value in the flat state arrays: a multiple of 256, spans of 256 do not overlap */
+  int64_t index;                  /* of its step count in `steps` */
+} asyrp_adamw_tensor;
+#define ASYRP_ADAMW_PARTIALS 1024 /* partial sums per 100 tensors (or part of 100) that asyrp_grad_sumsq writes */
+typedef struct asyrp_adamw {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_device;         /* device, nullable: read in place of lr when the step runs (a captured step whose lr changes) */
+  int32_t* steps;                 /* device: step counts, advanced by the call */
+  const float* clip;              /* device, nullable: {factor, skip} as asyrp_grad_clip writes them */
+  void* exp_avg;                  /* device: flat moments, f32 or (state_bits = 8) one byte each */
+  void* exp_avg_sq;
+  uint8_t* exp_avg_scale;         /* device, state_bits = 8: one exponent byte per 256 values */
+  uint8_t* exp_avg_sq_scale;
+  int32_t state_bits;             /* 32 or 8 */
+  uint32_t seed;                  /* of the 8-bit states' rounding */
+} asyrp_adamw;
+
 /* The library is built with -fvisibility=hidden: the entry points declared in this header are its whole dynamic symbol table
  * (besides the HIP kernel stubs the runtime needs).  (The opaque handle type above stays outside the pragma.) */
 #if defined(__GNUC__) || defined(__clang__)
@@ -96,8 +147,10 @@ typedef struct asyrp_engine asyrp_engine;
 #endif
 /* Version of this ABI (bumped on any signature or semantic change); asyrp_abi_version() returns the library's.
  *   v8 (round 5): asyrp_config.nominal_batch (was reserved[0]) is validated (0, 1, 2, 32), the reserved words must be zero;
- *                 asyrp_run_edit accepts one hs_coeff tuple per image (n_coeff < 0).  The product library reads no environment variable. */
-#define ASYRP_ABI_VERSION 8
+ *                 asyrp_run_edit accepts one hs_coeff tuple per image (n_coeff < 0).  The product library reads no environment variable.
+ *   v9: the operators of a training step outside the UNet (asyrp_packed_attention_*, asyrp_residual_norm_*, asyrp_adamw_* and
+ *                 asyrp_grad_*); nothing that was there has changed. */
+#define ASYRP_ABI_VERSION 9
 int asyrp_abi_version(void);
 
 /* Last error text of the calling thread ("" if none). */
@@ -232,6 +285,40 @@ int asyrp_get_temb(asyrp_engine* e, const float* t, int B, float* temb_out, void
 int asyrp_sampler_update(int device, const float* x, const float* model_out, int out_channels, int B, int C, int HW,
                          const float* coef_host, const float* noise, float* sample, float* pred_xstart, float* log_variance,
                          void* stream);
+
+/* ---- operators of a training step outside the UNet: the transformer encoders of a CLIP-like loss and the optimiser -----------------
+ * (diffusion_latent.py:337-350 leaves both to its libraries.)  Stateless; device pointers; asynchronous on `stream`; every one may be captured into a graph.
+ *
+ * Attention over sequences packed behind each other: sequence i = rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (device, sequences + 1
+ * ascending values from 0; values outside [0, tokens] or falling ones are held inside the tensors but give no defined result).
+ * lse [heads][tokens] (nullable in the forward) = log sum exp of the scaled scores.  Rows behind the last sequence are set to zero in the gradients
+ * and, where fill_tail is not 0, in out.  The gradients are contiguous; delta [heads][tokens] is workspace. */
+int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
+                                   void* out, float* lse, int fill_tail, void* stream);
+int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
+                                    const void* out, const float* lse, const void* d_out, float* delta, void* dq, void* dk, void* dv, void* stream);
+
+/* h = residual_scale * x + gate * N1(y), n = N2(h): the norm behind a block, its gate, the residual sum and the norm in front of the next block.
+ * gate [gates][width], row r takes gate row r / (rows / gates); weights and biases [width] f32, nullable each; n only where `before`.
+ * stats [rows][4] f32 (nullable in the forward: not kept) is what the backward reads again.  Backward: dh / dn nullable (no gradient), every
+ * output nullable; workspace: asyrp_residual_norm_workspace() floats (negative: an error code). */
+int asyrp_residual_norm_forward(int device, const asyrp_residual_norm* p, const void* x, const void* y, const float* gate, const float* after_weight,
+                                const float* after_bias, const float* before_weight, const float* before_bias, void* h, void* n, float* stats, void* stream);
+int64_t asyrp_residual_norm_workspace(const asyrp_residual_norm* p);
+int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const void* x, const void* y, const float* gate, const float* after_weight,
+                                 const float* after_bias, const float* before_weight, const float* stats, const void* dh, const void* dn, void* dx, void* dy,
+                                 float* dgate, float* d_after_weight, float* d_after_bias, float* d_before_weight, float* d_before_bias, float* workspace,
+                                 void* stream);
+
+/* AdamW over many tensors (host table).  asyrp_grad_sumsq writes ASYRP_ADAMW_PARTIALS fp64 sums of squares per 100 tensors; asyrp_grad_clip makes the
+ * norm and {factor, skip} of them (factor = min(1, max_norm / (norm + 1e-6)); skip = 1 where the norm is not finite: the step then changes
+ * nothing); asyrp_adamw_step advances the counts and updates parameters and moments; scratch: 32 bytes per tensor.
+ * asyrp_adamw_moments reads 8-bit moments as f32 (n values, a multiple of 256). */
+int asyrp_grad_sumsq(int device, const asyrp_adamw_tensor* tensors, int n, int dtype, double* partial, void* stream);
+int asyrp_grad_clip(int device, const double* partial, int n_partial, double max_norm, float* norm, float* clip, void* stream);
+int asyrp_adamw_step(int device, const asyrp_adamw* c, const asyrp_adamw_tensor* tensors, int n, int dtype, void* scratch, void* stream);
+int asyrp_adamw_moments(int device, const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_scale, const uint8_t* exp_avg_sq_scale,
+                        int64_t n, float* out_avg, float* out_avg_sq, void* stream);
 
 /* Bytes of device memory held by the engine (weights + workspace). */
 int64_t asyrp_device_bytes(const asyrp_engine* e);
