@@ -6,6 +6,7 @@ entry points raises.  torch is imported first so the process shares torch's HIP 
 """
 import ctypes as C
 import os
+import struct
 
 import torch  # noqa: F401  (must precede CDLL: one HIP runtime per process)
 
@@ -32,21 +33,10 @@ NORM_LAYER, NORM_RMS = 0, 1
 ADAMW_PARTIALS, ADAMW_TABLE = 1024, 100
 
 
-class PackedAttention(C.Structure):
-    _fields_ = [("tokens", C.c_int64), ("sequences", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
-                ("causal", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2),
-                ("v_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("dout_stride", C.c_int64 * 2)]
-
-
-class ResidualNorm(C.Structure):
-    _fields_ = [("rows", C.c_int64), ("gates", C.c_int64), ("width", C.c_int32), ("kind", C.c_int32), ("after", C.c_int32), ("before", C.c_int32),
-                ("stream_dtype", C.c_int32), ("branch_dtype", C.c_int32), ("residual_scale", C.c_float), ("eps", C.c_float)]
-
-
-class AdamWConfig(C.Structure):
-    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
-                ("lr_device", C.c_void_p), ("steps", C.c_void_p), ("clip", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p),
-                ("exp_avg_scale", C.c_void_p), ("exp_avg_sq_scale", C.c_void_p), ("state_bits", C.c_int32), ("seed", C.c_uint32)]
+# include/asyrp.h asyrp_packed_attention / asyrp_residual_norm / asyrp_adamw, field by field in the C compiler's own alignment
+PACKED_ATTENTION = struct.Struct("@qiiiiiif10q")
+RESIDUAL_NORM = struct.Struct("@qqiiiiiiff")
+ADAMW = struct.Struct("@dddddPPPPPPPiI")
 
 
 _P, _F, _I = C.c_void_p, C.c_float, C.c_int
@@ -72,14 +62,15 @@ _SIGS = {
     "asyrp_train_backward": (C.c_int, [_P, C.c_int64, _P, _I, C.POINTER(C.c_char_p), C.POINTER(_P), _P]),
     "asyrp_train_discard": (None, [_P, C.c_int64]),
     "asyrp_sampler_update": (C.c_int, [_I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
-    "asyrp_packed_attention_forward": (C.c_int, [_I, C.POINTER(PackedAttention)] + [_P] * 6 + [_I, _P]),
-    "asyrp_packed_attention_backward": (C.c_int, [_I, C.POINTER(PackedAttention)] + [_P] * 12),
-    "asyrp_residual_norm_forward": (C.c_int, [_I, C.POINTER(ResidualNorm)] + [_P] * 11),
-    "asyrp_residual_norm_workspace": (C.c_int64, [C.POINTER(ResidualNorm)]),
-    "asyrp_residual_norm_backward": (C.c_int, [_I, C.POINTER(ResidualNorm)] + [_P] * 18),
+    "asyrp_packed_attention_forward": (C.c_int, [_I] + [_P] * 8 + [_I, _P]),
+    "asyrp_packed_attention_workspace": (C.c_int64, [_P]),
+    "asyrp_packed_attention_backward": (C.c_int, [_I] + [_P] * 14),
+    "asyrp_residual_norm_forward": (C.c_int, [_I] + [_P] * 12),
+    "asyrp_residual_norm_workspace": (C.c_int64, [_P]),
+    "asyrp_residual_norm_backward": (C.c_int, [_I] + [_P] * 19),
     "asyrp_grad_sumsq": (C.c_int, [_I, _P, _I, _I, _P, _P]),
     "asyrp_grad_clip": (C.c_int, [_I, _P, _I, C.c_double, _P, _P, _P]),
-    "asyrp_adamw_step": (C.c_int, [_I, C.POINTER(AdamWConfig), _P, _I, _I, _P, _P]),
+    "asyrp_adamw_step": (C.c_int, [_I, _P, _P, _I, _I, _P, _P]),
     "asyrp_adamw_moments": (C.c_int, [_I, _P, _P, _P, _P, C.c_int64, _P, _P, _P]),
     "asyrp_device_bytes": (C.c_int64, [_P]),
     "asyrp_profile_table": (C.c_int, [_P, _I, _P, _P, _P, _P, _P]),

@@ -48,11 +48,14 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 struct PackedAttnArgs {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
+  void* rest;                // [T][Hq][D]: what rounding took from o (delta of the unrounded o halves what dq and dk are off); null: not kept
   float* lse;                // [Hq][T]
   float* delta;              // [Hq][T]
   const int* cu;
   long long T;
   int nseq, Hq, Hkv, D, causal, fill_tail;
+  int parts;                 // workgroups that share the queries of one key tile (dk / dv)
+  float* partial;            // [parts][T][Hkv][dk, dv][D] where there are several
   int tiles;                 // row tiles launched per head: T / BM + nseq + 1, at least one more than the sequences have
   float scale;
   long long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h, do_t, do_h, dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
@@ -96,43 +99,69 @@ __device__ __forceinline__ typename Frag<T>::V load_frag(const T* row, int ks, i
   return x.v;
 }
 
-template <int DP, int ROWS>
-struct Stage {              // a tile on its way from global memory to LDS through registers
-  static constexpr int N = ROWS * (DP / 8) / 256;
-  u32x4 r[N];
-  template <typename T>
-  __device__ __forceinline__ void load(const T* base, long long stride, int rows, int D, int tid) {
+// A tile [BN rows][DP] on its way from global memory to LDS, 16 bytes per lane and load, without passing through registers.
+// LDS is written in lane order, so the swizzle is in the addresses that the lanes read.  Rows behind the sequence are read from its last
+// row, columns behind D from the row's own columns: both are multiplied by probabilities or operands that are zero.
+// (Inline assembly, since the compiler waits for all loads in flight before each such load that it can see behind another one;
+// nothing is written but LDS, and the wait stands before the barrier that hands the tile over.)
+template <typename T, int DP>
+struct Tile {
+  static constexpr int N = BN * (DP / 8) / 256;
+  unsigned off[N];
+  int rows;                  // rows that the offsets stand for
+  unsigned stride;
+  __device__ __forceinline__ void offsets(int have, int D, int tid) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = tid + i * 256, row = c / (DP / 8), col = c % (DP / 8);
-      r[i] = u32x4{0, 0, 0, 0};
-      if (row < rows && col * 8 < D) r[i] = *reinterpret_cast<const u32x4*>(base + row * stride + col * 8);
+      const int c = tid + i * 256, row = c / (DP / 8), col = ((c % (DP / 8)) ^ swz<DP>(row)) % (unsigned)(D / 8);
+      off[i] = (unsigned)min(row, have - 1) * stride + col * 16;
     }
+    rows = have;
   }
-  __device__ __forceinline__ void store(char* tile, int tid) const {
+  __device__ __forceinline__ void init(long long st, int have, int D, int tid) {
+    stride = (unsigned)st * sizeof(T);
+    offsets(min(have, BN), D, tid);
+  }
+  // `have` (at least 1) rows from `base` on; both are the same in all lanes
+  __device__ __forceinline__ void load(const T* base, int have, unsigned lds, int D, int tid) {
+    have = min(have, BN);
+    if (have != rows) offsets(have, D, tid);
+    const unsigned w = __builtin_amdgcn_readfirstlane(lds + (tid >> 6) * 1024);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = tid + i * 256, row = c / (DP / 8), col = c % (DP / 8);
-      *reinterpret_cast<u32x4*>(tile + lds_at<DP>(row, col)) = r[i];
+      unsigned keep;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                   : "=&s"(keep)
+                   : "v"(off[i]), "s"(base), "s"(w + i * 4096)
+                   : "memory");
     }
   }
 };
+__device__ __forceinline__ unsigned lds_offset(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p; }
+// this wave's tiles have landed, and everybody's have behind the barrier
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // one instruction; results under 2^-126 are zero
 
 // The sequence and the row tile that tile number `t` of the launch stands for.  Tiles are numbered sequence by sequence; the numbers
 // behind the last one share the rows behind the last sequence.  Every wave finds it by itself: 64 lengths at a time, summed over the wave.
 // Offsets are held inside [0, T] and never fall, so that no value of `cu` leads outside the tensors.
-struct TileAt { long long start; int len, row0; int idle; int idles; long long end; };
+struct TileAt { long long start; int len, row0; int idle; int idles; int low, end; };
+// lane `src`'s value as one that the compiler knows to be the same in all lanes (all lanes active, src < 64)
+__device__ __forceinline__ int uniform(int v, int src) { return __builtin_amdgcn_readlane(v, __builtin_amdgcn_readfirstlane(src)); }
 __device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T, int t, int tiles, int lane) {
-  TileAt f{0, 0, 0, 0, 1, 0};
+  TileAt f{0, 0, 0, 0, 1, 0, 0};
   int before = 0;
   bool found = false;
-  long long high = 0;
+  int high = 0, low = 0;
   for (int b0 = 0; b0 < nseq; b0 += 64) {
     const int b = b0 + lane;
     long long s = 0, e = 0;
     if (b < nseq) { s = cu[b]; e = cu[b + 1]; }
     s = s < 0 ? 0 : s > T ? T : s;
-    e = e < s ? s : e > T ? T : e;
+    e = e < s ? s : e > T ? T : e;                        // T < 2^31
     const int n = (int)((e - s + BM - 1) / BM);
     int sum = n;
 #pragma unroll
@@ -144,47 +173,59 @@ __device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T
     const unsigned long long hit = __ballot(n > 0 && t >= first && t < first + n);
     if (hit) {
       const int src = __ffsll(hit) - 1;
-      f.start = __shfl(s, src);
-      f.len = (int)(__shfl(e, src) - f.start);
-      f.row0 = (t - __shfl(first, src)) * BM;
+      f.start = uniform((int)s, src);
+      f.len = uniform((int)e, src) - (int)f.start;
+      f.row0 = (t - uniform(first, src)) * BM;
       found = true;
       break;
     }
-    before += __shfl(sum, 63);
-    high = __shfl(e, nseq - 1 - b0 < 63 ? nseq - 1 - b0 : 63);
+    before += uniform(sum, 63);
+    high = uniform((int)e, nseq - 1 - b0 < 63 ? nseq - 1 - b0 : 63);
+    if (b0 == 0) low = uniform((int)s, 0);
   }
   if (!found) {
     f.idle = 1 + (t - before);
     f.idles = tiles - before;
+    f.low = low;
     f.end = high;
   }
   return f;
 }
 
-// zeros in the rows behind the last sequence: the idle tiles of each head take them in turn
+// zeros in the rows that belong to no sequence (behind the last one, before the first): the idle tiles of each head take them in turn
 template <typename T>
 __device__ __forceinline__ void zero_tail(T* p, long long st, long long sh, int head, int D, const TileAt& f, long long total, int tid) {
   const int chunks = D / 8;
-  for (long long row = f.end + (f.idle - 1); row < total; row += f.idles)
+  const long long rows = f.low + (total - f.end);
+  for (long long i = f.idle - 1; i < rows; i += f.idles) {
+    const long long row = i < f.low ? i : f.end + (i - f.low);
     for (int c = tid; c < chunks; c += 256) *reinterpret_cast<u32x4*>(p + row * st + head * sh + c * 8) = u32x4{0, 0, 0, 0};
+  }
 }
 
 __device__ __forceinline__ float both_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 __device__ __forceinline__ float both_halves_sum(float v) { return v + __shfl_xor(v, 32); }
 
 // rows d of a transposed result (column = this lane's row of the output tensor) times `m`, as 8-byte stores
+// (`rest`: where given, what the rounding to T took away, rounded itself)
 template <typename T, int DP>
-__device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float m, int h, int D) {
+__device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float m, int h, int D, T* rest = nullptr) {
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const int d = 32 * dt + 8 * r4 + 4 * h;
       if (d >= D) continue;
-      union { T t[4]; u32x2 u; } x;
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      T4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x.t[j] = (T)(acc[dt][4 * r4 + j] * m);
-      *reinterpret_cast<u32x2*>(row + d) = x.u;
+      for (int j = 0; j < 4; ++j) x[j] = (T)(acc[dt][4 * r4 + j] * m);
+      *reinterpret_cast<T4*>(row + d) = x;
+      if (rest) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = (T)(acc[dt][4 * r4 + j] * m - (float)x[j]);
+        *reinterpret_cast<T4*>(rest + d) = x;
+      }
     }
 }
 
@@ -198,9 +239,9 @@ __device__ __forceinline__ typename Frag<T>::V pack8(const f32x16& s, int half) 
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void packed_attn_fwd_kernel(const PackedAttnArgs p) {
-  __shared__ __attribute__((aligned(16))) char kt[BN * DP * 2], vt[BN * DP * 2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+__global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAttnArgs p) {
+  __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int head = blockIdx.x % p.Hq, tile = p.tiles - 1 - blockIdx.x / p.Hq;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
   if (f.idle) {
@@ -213,6 +254,13 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_kernel(const PackedAttnAr
   const int row = f.row0 + wave * 32 + (lane & 31);
   const bool there = row < f.len;
   const T* qrow = (const T*)p.q + (f.start + (there ? row : 0)) * p.q_t + head * p.q_h;
+  const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
+  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
+  Tile<T, DP> ks_, vs_;
+  ks_.init(p.k_t, f.len, p.D, tid);
+  vs_.init(p.v_t, f.len, p.D, tid);
+  ks_.load(k, f.len, lds_offset(kt[0]), p.D, tid);
+  vs_.load(v, f.len, lds_offset(vt[0]), p.D, tid);
   typename Frag<T>::V qf[DP / 16];
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) qf[ks] = load_frag<T>(qrow, ks, h, p.D, there);
@@ -222,21 +270,14 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_kernel(const PackedAttnAr
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f;                         // reference and sum, in the scores' own units and of this lane's rows
   const float sc = p.scale * LOG2E;
-  const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
-  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
-  Stage<DP, BN> ks_, vs_;
-  ks_.load(k, p.k_t, f.len, p.D, tid);
-  vs_.load(v, p.v_t, f.len, p.D, tid);
-  for (int k0 = 0; k0 < kend; k0 += BN) {
-    __syncthreads();
-    ks_.store(kt, tid);
-    vs_.store(vt, tid);
-    __syncthreads();
+  int buf = 0;
+  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
+    tile_barrier();
     if (k0 + BN < kend) {
-      ks_.load(k + (long long)(k0 + BN) * p.k_t, p.k_t, f.len - k0 - BN, p.D, tid);
-      vs_.load(v + (long long)(k0 + BN) * p.v_t, p.v_t, f.len - k0 - BN, p.D, tid);
+      ks_.load(k + (long long)(k0 + BN) * p.k_t, f.len - k0 - BN, lds_offset(kt[buf ^ 1]), p.D, tid);
+      vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(vt[buf ^ 1]), p.D, tid);
     }
     if (k0 >= wend) continue;
     f32x16 s[2];
@@ -245,58 +286,61 @@ __global__ __launch_bounds__(256) void packed_attn_fwd_kernel(const PackedAttnAr
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) s[n] = Frag<T>::mma(read_rows<T, DP>(kt, 32 * n, ks, lane), qf[ks], s[n]);
+      for (int ks = 0; ks < DP / 16; ++ks) s[n] = Frag<T>::mma(read_rows<T, DP>(kt[buf], 32 * n, ks, lane), qf[ks], s[n]);
     }
-    const int last = p.causal ? min(row, f.len - 1) : f.len - 1;    // the last key this column sees
-    const bool edge = k0 + BN > f.len || (p.causal && k0 + BN - 1 > f.row0 + wave * 32);
-    float mx = -INFINITY;
+    if (k0 + BN > f.len || (p.causal && k0 + BN - 1 > f.row0 + wave * 32)) {
+      const int last = (p.causal ? min(row, f.len - 1) : f.len - 1) - k0 - 4 * h;    // the last key this column sees
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * n + 8 * (r >> 2) + (r & 3) > last) s[n][r] = -INFINITY;
+    }
+    float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float x = s[n][r] * sc;
-        if (edge && k0 + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3) > last) x = -INFINITY;
-        s[n][r] = x;
-        mx = fmaxf(mx, x);
-      }
-    const float mn = fmaxf(m, both_halves_max(mx));
-    const float keep = exp2f(m - mn);
-    float sum = 0.f;
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = both_halves_max(mx);
+    // The reference moves only where a column's maximum has outgrown it by 8 powers of two (and in the first tile): the exponentials stay under
+    // 2^8, well inside f16, and most tiles leave the sums as they are.
+    if (__any(!((mx - m) * sc <= 8.f))) {
+      const float mn = fmaxf(m, mx), keep = exp2_fast((m - mn) * sc);
+      m = mn;
+      l *= keep;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float e = exp2f(s[n][r] - mn);
-        s[n][r] = e;
-        sum += e;
-      }
-    l = l * keep + sum;
-    m = mn;
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
+    }
+    const float ms = m * sc;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int r = 8 * b; r < 8 * b + 8; ++r) {
+          s[n][r] = exp2_fast(__builtin_fmaf(s[n][r], sc, -ms));
+          l += s[n][r];
+        }
         const typename Frag<T>::V pf = pack8<T>(s[n], b);
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(vt, 32 * n + 16 * b, dt, lane), pf, acc[dt]);
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(vt[buf], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
       }
   }
   l = both_halves_sum(l);
   if (there) {
-    store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, acc, 1.0f / l, h, p.D);
-    if (p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (m + log2f(l)) * LN2;
+    store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, acc, 1.0f / l, h, p.D,
+                      p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
+    if (p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (m * sc + log2f(l)) * LN2;
   }
 }
 
 // dq, and delta = rowsum(do * o) for the other kernel
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void packed_attn_dq_kernel(const PackedAttnArgs p) {
-  __shared__ __attribute__((aligned(16))) char kt[BN * DP * 2], vt[BN * DP * 2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+__global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttnArgs p) {
+  __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int head = blockIdx.x % p.Hq, tile = p.tiles - 1 - blockIdx.x / p.Hq;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
   if (f.idle) {
@@ -312,6 +356,7 @@ __global__ __launch_bounds__(256) void packed_attn_dq_kernel(const PackedAttnArg
   const T* qrow = (const T*)p.q + at * p.q_t + head * p.q_h;
   const T* grow = (const T*)p.dout + at * p.do_t + head * p.do_h;
   const T* orow = (const T*)p.o + at * p.o_t + head * p.o_h;
+  const T* rrow = p.rest ? (const T*)p.rest + (at * p.Hq + head) * p.D : nullptr;
   typename Frag<T>::V qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
 #pragma unroll
@@ -321,6 +366,11 @@ __global__ __launch_bounds__(256) void packed_attn_dq_kernel(const PackedAttnArg
     const typename Frag<T>::V of = load_frag<T>(orow, ks, h, p.D, there);
 #pragma unroll
     for (int j = 0; j < 8; ++j) delta += (float)gf[ks][j] * (float)of[j];
+    if (rrow) {
+      const typename Frag<T>::V rf = load_frag<T>(rrow, ks, h, p.D, there);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += (float)gf[ks][j] * (float)rf[j];
+    }
   }
   delta = both_halves_sum(delta);
   const float lse2 = there ? p.lse[(long long)head * p.T + at] * LOG2E : 0.f;
@@ -334,20 +384,20 @@ __global__ __launch_bounds__(256) void packed_attn_dq_kernel(const PackedAttnArg
   const float sc = p.scale * LOG2E;
   const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
   const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;
-  Stage<DP, BN> ks_, vs_;
-  ks_.load(k, p.k_t, f.len, p.D, tid);
-  vs_.load(v, p.v_t, f.len, p.D, tid);
-  for (int k0 = 0; k0 < kend; k0 += BN) {
-    __syncthreads();
-    ks_.store(kt, tid);
-    vs_.store(vt, tid);
-    __syncthreads();
+  Tile<T, DP> ks_, vs_;
+  ks_.init(p.k_t, f.len, p.D, tid);
+  vs_.init(p.v_t, f.len, p.D, tid);
+  ks_.load(k, f.len, lds_offset(kt[0]), p.D, tid);
+  vs_.load(v, f.len, lds_offset(vt[0]), p.D, tid);
+  int buf = 0;
+  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
+    tile_barrier();
     if (k0 + BN < kend) {
-      ks_.load(k + (long long)(k0 + BN) * p.k_t, p.k_t, f.len - k0 - BN, p.D, tid);
-      vs_.load(v + (long long)(k0 + BN) * p.v_t, p.v_t, f.len - k0 - BN, p.D, tid);
+      ks_.load(k + (long long)(k0 + BN) * p.k_t, f.len - k0 - BN, lds_offset(kt[buf ^ 1]), p.D, tid);
+      vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(vt[buf ^ 1]), p.D, tid);
     }
     if (k0 >= wend) continue;
-    const int last = there ? (p.causal ? row : f.len - 1) : -1;
+    const int last = (there ? (p.causal ? row : f.len - 1) : -1) - k0 - 4 * h;
     const bool edge = k0 + BN > f.len || f.row0 + wave * 32 + 32 > f.len || (p.causal && k0 + BN - 1 > f.row0 + wave * 32);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -356,20 +406,20 @@ __global__ __launch_bounds__(256) void packed_attn_dq_kernel(const PackedAttnArg
       for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        s = Frag<T>::mma(read_rows<T, DP>(kt, 32 * n, ks, lane), qf[ks], s);
-        g = Frag<T>::mma(read_rows<T, DP>(vt, 32 * n, ks, lane), gf[ks], g);
+        s = Frag<T>::mma(read_rows<T, DP>(kt[buf], 32 * n, ks, lane), qf[ks], s);
+        g = Frag<T>::mma(read_rows<T, DP>(vt[buf], 32 * n, ks, lane), gf[ks], g);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float e = exp2f(s[r] * sc - lse2) * (g[r] - delta);
-        if (edge && k0 + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3) > last) e = 0.f;
-        s[r] = e;
-      }
+      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], sc, -lse2)) * (g[r] - delta);
+      if (edge)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * n + 8 * (r >> 2) + (r & 3) > last) s[r] = 0.f;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const typename Frag<T>::V pf = pack8<T>(s, b);
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(kt, 32 * n + 16 * b, dt, lane), pf, acc[dt]);
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(kt[buf], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
       }
     }
   }
@@ -378,13 +428,14 @@ __global__ __launch_bounds__(256) void packed_attn_dq_kernel(const PackedAttnArg
 
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void packed_attn_dkv_kernel(const PackedAttnArgs p) {
-  __shared__ __attribute__((aligned(16))) char qt[BN * DP * 2], gt[BN * DP * 2];
-  __shared__ __attribute__((aligned(16))) float ls[BN], ds[BN];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-  const int hk = blockIdx.x % p.Hkv, tile = blockIdx.x / p.Hkv, G = p.Hq / p.Hkv;
+__global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAttnArgs p) {
+  __shared__ __attribute__((aligned(16))) char qt[2][BN * DP * 2], gt[2][BN * DP * 2];
+  __shared__ __attribute__((aligned(16))) float ls[2][BN], ds[2][BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
   if (f.idle) {
+    if (part) return;
     zero_tail((T*)p.dk, p.dk_t, p.dk_h, hk, p.D, f, p.T, tid);
     zero_tail((T*)p.dv, p.dv_t, p.dv_h, hk, p.D, f, p.T, tid);
     return;
@@ -408,26 +459,31 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_kernel(const PackedAttnAr
   const float sc = p.scale * LOG2E;
   const int qbeg = p.causal ? f.row0 : 0;               // a multiple of BN
   const int per = (f.len - qbeg + BN - 1) / BN, total = per * G;
-  Stage<DP, BN> qs, gs;
-  auto fetch = [&](int i) {
+  const int i0 = (int)((long long)total * part / p.parts), i1 = (int)((long long)total * (part + 1) / p.parts);   // this part of the heads' query tiles
+  Tile<T, DP> qs, gs;
+  qs.init(p.q_t, f.len - qbeg, p.D, tid);
+  gs.init(p.do_t, f.len - qbeg, p.D, tid);
+  float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
+  auto fetch = [&](int i, int buf) {
     const int head = hk * G + i / per, q0 = qbeg + (i % per) * BN;
-    qs.load((const T*)p.q + (f.start + q0) * p.q_t + head * p.q_h, p.q_t, f.len - q0, p.D, tid);
-    gs.load((const T*)p.dout + (f.start + q0) * p.do_t + head * p.do_h, p.do_t, f.len - q0, p.D, tid);
-  };
-  fetch(0);
-  for (int i = 0; i < total; ++i) {
-    const int head = hk * G + i / per, q0 = qbeg + (i % per) * BN;
-    __syncthreads();
-    qs.store(qt, tid);
-    gs.store(gt, tid);
+    qs.load((const T*)p.q + (f.start + q0) * p.q_t + head * p.q_h, f.len - q0, lds_offset(qt[buf]), p.D, tid);
+    gs.load((const T*)p.dout + (f.start + q0) * p.do_t + head * p.do_h, f.len - q0, lds_offset(gt[buf]), p.D, tid);
     if (tid < BN) {
-      const bool in = q0 + tid < f.len;
-      const long long a = (long long)head * p.T + f.start + q0 + tid;
-      ls[tid] = in ? p.lse[a] * LOG2E : 0.f;
-      ds[tid] = in ? p.delta[a] : 0.f;
+      const long long a = (long long)head * p.T + f.start + min(q0 + tid, f.len - 1);
+      lv_ = p.lse[a] * LOG2E;
+      dl_ = p.delta[a];
     }
-    __syncthreads();
-    if (i + 1 < total) fetch(i + 1);
+  };
+  if (i0 < i1) fetch(i0, 0);
+  int buf = 0;
+  for (int i = i0; i < i1; ++i, buf ^= 1) {
+    const int q0 = qbeg + (i % per) * BN;
+    if (tid < BN) {
+      ls[buf][tid] = lv_;
+      ds[buf][tid] = dl_;
+    }
+    tile_barrier();
+    if (i + 1 < i1) fetch(i + 1, buf ^ 1);
     if (p.causal && q0 + BN <= f.row0 + wave * 32) continue;      // every query lies before this wave's keys
     const bool edge = q0 + BN > f.len || (p.causal && q0 < f.row0 + wave * 32 + 31);
 #pragma unroll
@@ -437,17 +493,17 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_kernel(const PackedAttnAr
       for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
-        s = Frag<T>::mma(read_rows<T, DP>(qt, 32 * n, ks, lane), kf[ks], s);
-        g = Frag<T>::mma(read_rows<T, DP>(gt, 32 * n, ks, lane), vf[ks], g);
+        s = Frag<T>::mma(read_rows<T, DP>(qt[buf], 32 * n, ks, lane), kf[ks], s);
+        g = Frag<T>::mma(read_rows<T, DP>(gt[buf], 32 * n, ks, lane), vf[ks], g);
       }
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[32 * n + 8 * r4 + 4 * h]);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[32 * n + 8 * r4 + 4 * h]);
+        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * n + 8 * r4 + 4 * h]);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[buf][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * r4 + j, q = q0 + 32 * n + 8 * r4 + 4 * h + j;
-          float e = exp2f(s[r] * sc - lv[j]);
+          float e = exp2_fast(__builtin_fmaf(s[r], sc, -lv[j]));
           if (edge && (q >= f.len || (p.causal && q < row))) e = 0.f;
           s[r] = e;
           g[r] = e * (g[r] - dl[j]);
@@ -458,16 +514,151 @@ __global__ __launch_bounds__(256) void packed_attn_dkv_kernel(const PackedAttnAr
         const typename Frag<T>::V pf = pack8<T>(s, b), zf = pack8<T>(g, b);
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) {
-          dv[dt] = Frag<T>::mma(read_cols<T, DP>(gt, 32 * n + 16 * b, dt, lane), pf, dv[dt]);
-          dk[dt] = Frag<T>::mma(read_cols<T, DP>(qt, 32 * n + 16 * b, dt, lane), zf, dk[dt]);
+          dv[dt] = Frag<T>::mma(read_cols<T, DP>(gt[buf], 32 * n + 16 * b, dt, lane), pf, dv[dt]);
+          dk[dt] = Frag<T>::mma(read_cols<T, DP>(qt[buf], 32 * n + 16 * b, dt, lane), zf, dk[dt]);
         }
       }
     }
   }
-  if (there) {
+  if (there && p.parts > 1) {
+    float* to = p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D;
+    store_cols<float, DP>(to, dk, p.scale, h, p.D);
+    store_cols<float, DP>(to + p.D, dv, 1.0f, h, p.D);
+  } else if (there) {
     store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, p.scale, h, p.D);
     store_cols<T, DP>((T*)p.dv + at * p.dv_t + hk * p.dv_h, dv, 1.0f, h, p.D);
   }
+}
+
+// The same for heads wider than 64, where one wave cannot hold both sums, its keys' and values' fragments and the scores in half a SIMD's registers, and a
+// wave alone on its SIMD waits out every exponential: eight waves, of which the first four form dk and the others dv of the same 128 keys
+// from the same tiles.  S is formed by both (5 products instead of 4), and in return two waves share each SIMD, one in its products
+// while the other is in its exponentials: 435 us with one wave per SIMD, XXX so (16 query heads on 4, 128 wide, 8192 rows, causal).
+template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const PackedAttnArgs p) {
+  __shared__ __attribute__((aligned(16))) char qt[2][BN * DP * 2], gt[2][BN * DP * 2];
+  __shared__ __attribute__((aligned(16))) float ls[2][BN], ds[2][BN];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, h = lane >> 5;
+  const bool values = __builtin_amdgcn_readfirstlane(tid >> 8);          // this wave forms dv
+  const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
+  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
+  if (f.idle) {
+    if (part) return;
+    if (values) zero_tail((T*)p.dv, p.dv_t, p.dv_h, hk, p.D, f, p.T, tid & 255);
+    else zero_tail((T*)p.dk, p.dk_t, p.dk_h, hk, p.D, f, p.T, tid);
+    return;
+  }
+  const int row = f.row0 + wave * 32 + (lane & 31);     // this lane's key
+  const bool there = row < f.len;
+  const long long at = f.start + (there ? row : 0);
+  const T* krow = (const T*)p.k + at * p.k_t + hk * p.k_h;
+  const T* vrow = (const T*)p.v + at * p.v_t + hk * p.v_h;
+  typename Frag<T>::V kf[DP / 16], vf[DP / 16];
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    kf[ks] = load_frag<T>(krow, ks, h, p.D, there);
+    vf[ks] = load_frag<T>(vrow, ks, h, p.D, there);
+  }
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+  const float sc = p.scale * LOG2E;
+  const int qbeg = p.causal ? f.row0 : 0;               // a multiple of BN
+  const int per = (f.len - qbeg + BN - 1) / BN, total = per * G;
+  const int i0 = (int)((long long)total * part / p.parts), i1 = (int)((long long)total * (part + 1) / p.parts);   // this part of the heads' query tiles
+  Tile<T, DP> ts;                                       // four waves load the queries, four the output's gradients
+  ts.init(values ? p.do_t : p.q_t, f.len - qbeg, p.D, tid & 255);
+  const T* base = values ? (const T*)p.dout + f.start * p.do_t : (const T*)p.q + f.start * p.q_t;
+  const long long st = values ? p.do_t : p.q_t, sh = values ? p.do_h : p.q_h;
+  float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
+  auto fetch = [&](int i, int buf) {
+    const int head = hk * G + i / per, q0 = qbeg + (i % per) * BN;
+    ts.load(base + q0 * st + head * sh, f.len - q0, values ? lds_offset(gt[buf]) : lds_offset(qt[buf]), p.D, tid & 255);
+    if (tid < BN) {
+      const long long a = (long long)head * p.T + f.start + min(q0 + tid, f.len - 1);
+      lv_ = p.lse[a] * LOG2E;
+      dl_ = p.delta[a];
+    }
+  };
+  if (i0 < i1) fetch(i0, 0);
+  int buf = 0;
+  for (int i = i0; i < i1; ++i, buf ^= 1) {
+    const int q0 = qbeg + (i % per) * BN;
+    if (tid < BN) {
+      ls[buf][tid] = lv_;
+      ds[buf][tid] = dl_;
+    }
+    tile_barrier();
+    if (i + 1 < i1) fetch(i + 1, buf ^ 1);
+    if (p.causal && q0 + BN <= f.row0 + wave * 32) continue;      // every query lies before this wave's keys
+    const bool edge = q0 + BN > f.len || (p.causal && q0 < f.row0 + wave * 32 + 31);
+#pragma unroll
+    for (int n = 0; n < BN / 32; ++n) {
+      f32x16 s, g;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(qt[buf], 32 * n, ks, lane), kf[ks], s);
+      if (!values)
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[buf], 32 * n, ks, lane), vf[ks], g);
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * n + 8 * r4 + 4 * h]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
+      }
+      if (!values)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[buf][32 * n + 8 * r4 + 4 * h]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[4 * r4 + j] *= g[4 * r4 + j] - dl[j];
+        }
+      if (edge)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int q = q0 + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+          if (q >= f.len || (p.causal && q < row)) s[r] = 0.f;
+        }
+      const char* from = values ? gt[buf] : qt[buf];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const typename Frag<T>::V pf = pack8<T>(s, b);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(from, 32 * n + 16 * b, dt, lane), pf, acc[dt]);
+      }
+    }
+  }
+  if (there && p.parts > 1) {
+    store_cols<float, DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
+  } else if (there) {
+    store_cols<T, DP>(values ? (T*)p.dv + at * p.dv_t + hk * p.dv_h : (T*)p.dk + at * p.dk_t + hk * p.dk_h, acc, values ? 1.0f : p.scale, h, p.D);
+  }
+}
+
+// dk and dv from the parts' sums, in the parts' order; 8 values per thread
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_join_kernel(const PackedAttnArgs p) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;
+  const long long row = i / (2 * p.D * p.Hkv), begin = p.cu[0] < 0 ? 0 : p.cu[0], end = min(p.T, (long long)p.cu[p.nseq]);
+  if (row >= end || row < begin) return;                // rows of no sequence are zero already
+  const int c = (int)(i % (2 * p.D)), hk = (int)(i / (2 * p.D) % p.Hkv);
+  const float* from = p.partial + i;
+  const long long step = p.T * p.Hkv * 2 * p.D;
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = from[j];
+  for (int k = 1; k < p.parts; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += from[k * step + j];
+  typename Frag<T>::V x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = (T)s[j];
+  T* to = c < p.D ? (T*)p.dk + row * p.dk_t + hk * p.dk_h + c : (T*)p.dv + row * p.dv_t + hk * p.dv_h + c - p.D;
+  *reinterpret_cast<typename Frag<T>::V*>(to) = x;
 }
 
 template <typename T, int DP>
@@ -478,7 +669,11 @@ hipError_t launch_forward(const PackedAttnArgs& a, hipStream_t s) {
 template <typename T, int DP>
 hipError_t launch_backward(const PackedAttnArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq), dim3(256), 0, s, a);
-  hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hkv), dim3(256), 0, s, a);
+  const dim3 g((unsigned)a.tiles * a.Hkv * a.parts);
+  if constexpr (DP > 64) hipLaunchKernelGGL((packed_attn_dkv_pair_kernel<T, DP>), g, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP>), g, dim3(256), 0, s, a);
+  if (a.parts > 1)
+    hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)((a.T * a.Hkv * 2 * a.D / 8 + 255) / 256)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 template <typename T>
@@ -492,6 +687,15 @@ hipError_t launch(const PackedAttnArgs& a, bool backward, hipStream_t s) {
   }
 }
 
+// Into how many parts the queries of a key tile are dealt: a kernel of few tiles (few rows, or few key / value heads with many query heads each) leaves CUs idle
+// and ends with its longest workgroup; the parts' fp32 sums cost a write and a read of 8 bytes per value and part.
+int dkv_parts(long long T, int nseq, int Hq, int Hkv) {
+  const long long wgs = std::max<long long>(1, T / BM) * Hkv;       // full tiles; the ragged ones are light
+  int parts = 1;
+  while (parts < 8 && wgs * parts < 1024 && T / nseq * (Hq / Hkv) >= 1024LL * parts) parts *= 2;
+  return parts;
+}
+
 int refuse(const std::string& m) { return set_last_error(ASYRP_EINVAL, m.c_str()); }
 
 // the checks that both directions share; 0 or the error
@@ -500,11 +704,12 @@ int check(const PackedAttnArgs& a, int dtype, const long long* strides, int n) {
   if (a.D < 8 || a.D > 128 || a.D % 8) return refuse("packed attention: the head width must be a multiple of 8 from 8 to 128");
   if (a.Hq < 1 || a.Hkv < 1 || a.Hq % a.Hkv) return refuse("packed attention: query heads must be a multiple of key/value heads");
   if (a.nseq < 1 || a.T < 0 || a.T > 0x7fffffffLL) return refuse("packed attention: bad number of sequences or rows");
-  if (!(a.scale == a.scale) || std::isinf(a.scale)) return refuse("packed attention: the scale must be finite");
+  if (!(a.scale > 0) || std::isinf(a.scale)) return refuse("packed attention: the scale must be positive and finite");
   for (int i = 0; i < n; ++i)
-    if (strides[i] < 0 || strides[i] % 8 || strides[i] > (1LL << 40)) return refuse("packed attention: strides must be multiples of 8 values, not negative");
+    if (strides[i] < 0 || strides[i] % 8 || strides[i] > (i % 2 ? 1LL << 40 : 1LL << 23))
+      return refuse("packed attention: strides must be multiples of 8 values, not negative, rows at most 2^23 values apart");
   const long long tiles = a.T / BM + a.nseq + 1;
-  if (tiles * a.Hq > 0x7fffffffLL) return refuse("packed attention: too many rows x heads for one launch");
+  if (tiles * a.Hq * 8 > 0x7fffffffLL) return refuse("packed attention: too many rows x heads for one launch");
   return 0;
 }
 bool unaligned(std::initializer_list<const void*> ps) {
@@ -521,18 +726,18 @@ using namespace asyrp;
 extern "C" {
 
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
-                                   float* lse, int fill_tail, void* stream) {
+                                   float* lse, void* out_rest, int fill_tail, void* stream) {
   if (!p || !cu_seqlens) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.cu = cu_seqlens;
   a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.causal = p->causal != 0; a.scale = p->scale;
   a.q_t = p->q_stride[0]; a.q_h = p->q_stride[1]; a.k_t = p->k_stride[0]; a.k_h = p->k_stride[1]; a.v_t = p->v_stride[0]; a.v_h = p->v_stride[1];
   a.o_t = p->out_stride[0]; a.o_h = p->out_stride[1];
-  a.fill_tail = fill_tail;
+  a.fill_tail = fill_tail; a.rest = out_rest;
   const long long st[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.o_t, a.o_h};
   if (int rc = check(a, p->dtype, st, 8)) return rc;
   if (a.T == 0) return 0;
-  if (unaligned({q, k, v, out})) return refuse("packed attention: tensors must be given and 16-byte aligned");
+  if (unaligned({q, k, v, out}) || ((uintptr_t)out_rest & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");
   a.tiles = (int)(a.T / BM + a.nseq + 1);
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
@@ -540,11 +745,20 @@ int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, 
   return e == hipSuccess ? 0 : set_last_error(ASYRP_EHIP, hipGetErrorString(e));
 }
 
+int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p) {
+  if (!p) return refuse("packed attention: null argument");
+  PackedAttnArgs a{};
+  a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.scale = p->scale;
+  if (int rc = check(a, p->dtype, nullptr, 0)) return rc;
+  const int parts = dkv_parts(a.T, a.nseq, a.Hq, a.Hkv);
+  return (a.T * a.Hq + 3) / 4 * 4 + (parts > 1 ? parts * a.T * a.Hkv * 2 * a.D : 0);
+}
+
 int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                    const void* out, const float* lse, const void* d_out, float* delta, void* dq, void* dk, void* dv, void* stream) {
+                                    const void* out, const float* lse, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream) {
   if (!p || !cu_seqlens) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
-  a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<float*>(lse); a.dout = d_out; a.delta = delta; a.dq = dq; a.dk = dk; a.dv = dv; a.cu = cu_seqlens;
+  a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<float*>(lse); a.rest = const_cast<void*>(out_rest); a.dout = d_out; a.delta = workspace; a.dq = dq; a.dk = dk; a.dv = dv; a.cu = cu_seqlens;
   a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.causal = p->causal != 0; a.scale = p->scale;
   a.q_t = p->q_stride[0]; a.q_h = p->q_stride[1]; a.k_t = p->k_stride[0]; a.k_h = p->k_stride[1]; a.v_t = p->v_stride[0]; a.v_h = p->v_stride[1];
   a.o_t = p->out_stride[0]; a.o_h = p->out_stride[1]; a.do_t = p->dout_stride[0]; a.do_h = p->dout_stride[1];
@@ -553,7 +767,9 @@ int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p,
   const long long st[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.o_t, a.o_h, a.do_t, a.do_h};
   if (int rc = check(a, p->dtype, st, 10)) return rc;
   if (a.T == 0) return 0;
-  if (unaligned({q, k, v, out, d_out, dq, dk, dv}) || !lse || !delta) return refuse("packed attention: tensors must be given and 16-byte aligned");
+  a.parts = dkv_parts(a.T, a.nseq, a.Hq, a.Hkv);
+  a.partial = workspace + (a.T * a.Hq + 3) / 4 * 4;
+  if (unaligned({q, k, v, out, d_out, dq, dk, dv}) || ((uintptr_t)out_rest & 15) || !lse || !workspace || ((uintptr_t)workspace & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");
   a.tiles = (int)(a.T / BM + a.nseq + 1);
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));

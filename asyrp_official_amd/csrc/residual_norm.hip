@@ -37,58 +37,53 @@ struct NormArgs {
 // partial vectors, in this order
 enum { V_W2, V_B2, V_W1, V_B1, V_GATE, VECTORS };
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(_Float16 v) { return (float)v; }
-__device__ __forceinline__ float to_f(__bf16 v) { return (float)v; }
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-
-// eight values of a row: contiguous and 16-byte aligned (VEC), or `TPR` apart so that neighbouring lanes still read neighbouring values
-template <typename T, bool VEC, int TPR>
-__device__ __forceinline__ void load8(const T* row, int slot, int t, int C, float (&o)[8]) {
+// A thread's VPT values of a row: contiguous (VEC: whole 16-byte groups of the row), or TPR apart, so that neighbouring lanes still read
+// neighbouring values of a row of any width and address.
+template <typename T, int VPT>
+struct Raw {
+  typedef T V __attribute__((ext_vector_type(VPT), aligned(sizeof(T) * VPT < 16 ? sizeof(T) * VPT : 16)));
+  V v;
+};
+template <typename T, bool VEC, int TPR, int VPT>
+__device__ __forceinline__ void load(const T* row, int t, int C, Raw<T, VPT>& o) {
   if (VEC) {
-    const int c = (slot * TPR + t) * 8;
-    if (c < C) {
-      union { u32x4 u[sizeof(T) / 2]; T v[8]; } x;
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.u[i] = reinterpret_cast<const u32x4*>(row + c)[i];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = to_f(x.v[j]);
+    if (t * VPT < C) {
+      o.v = *reinterpret_cast<const typename Raw<T, VPT>::V*>(row + t * VPT);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) o[j] = 0.f;
+      for (int j = 0; j < VPT; ++j) o.v[j] = (T)0.f;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = (slot * 8 + j) * TPR + t;
-      o[j] = c < C ? to_f(row[c]) : 0.f;
-    }
+    for (int j = 0; j < VPT; ++j) o.v[j] = j * TPR + t < C ? row[j * TPR + t] : (T)0.f;
   }
 }
-template <typename T, bool VEC, int TPR>
-__device__ __forceinline__ void store8(T* row, int slot, int t, int C, const float (&o)[8]) {
+template <typename T, int VPT>
+__device__ __forceinline__ void floats(const Raw<T, VPT>& r, float (&o)[VPT]) {
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) o[j] = (float)r.v[j];
+}
+template <bool VEC, int TPR, int VPT>
+__device__ __forceinline__ void loadf(const float* row, int t, int C, float (&o)[VPT]) {
+  Raw<float, VPT> r;
+  load<float, VEC, TPR, VPT>(row, t, C, r);
+  floats(r, o);
+}
+template <typename T, bool VEC, int TPR, int VPT>
+__device__ __forceinline__ void store(T* row, int t, int C, const float (&o)[VPT]) {
+  Raw<T, VPT> x;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) x.v[j] = (T)o[j];
   if (VEC) {
-    const int c = (slot * TPR + t) * 8;
-    if (c < C) {
-      union { u32x4 u[sizeof(T) / 2]; T v[8]; } x;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x.v[j] = (T)o[j];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<u32x4*>(row + c)[i] = x.u[i];
-    }
+    if (t * VPT < C) *reinterpret_cast<typename Raw<T, VPT>::V*>(row + t * VPT) = x.v;
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = (slot * 8 + j) * TPR + t;
-      if (c < C) row[c] = (T)o[j];
-    }
+    for (int j = 0; j < VPT; ++j)
+      if (j * TPR + t < C) row[j * TPR + t] = x.v[j];
   }
 }
-template <bool VEC, int TPR>
-__device__ __forceinline__ bool in8(int slot, int t, int j, int C) {
-  return VEC ? (slot * TPR + t) * 8 < C : (slot * 8 + j) * TPR + t < C;
-}
+template <bool VEC, int TPR, int VPT>
+__device__ __forceinline__ bool inside(int t, int j, int C) { return VEC ? t * VPT < C : j * TPR + t < C; }
 
 // sums of K values over the TPR threads of a row.  `buf` holds two sets of one row of K values per wave, used in turn, so that
 // one barrier per reduction is enough.
@@ -117,146 +112,155 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* buf, int& turn, in
 }
 
 // mean and rstd of the values (those behind C are zero and do not count)
-template <bool VEC, int TPR, int NV>
-__device__ __forceinline__ void statistics(const float (&v)[NV][8], const NormArgs& p, float* buf, int& turn, int sub, int t, float& mean, float& rstd) {
+template <bool VEC, int TPR, int VPT>
+__device__ __forceinline__ void statistics(const float (&v)[VPT], const NormArgs& p, float* buf, int& turn, int sub, int t, float& mean, float& rstd) {
   mean = 0.f;
   float s[1] = {0.f};
   if (!p.rms) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[0] += v[i][j];
+    for (int j = 0; j < VPT; ++j) s[0] += v[j];
     row_sum<TPR, 1>(s, buf, turn, sub, t);
     mean = s[0] / (float)p.C;
   }
   s[0] = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (in8<VEC, TPR>(i, t, j, p.C)) s[0] += (v[i][j] - mean) * (v[i][j] - mean);
+  for (int j = 0; j < VPT; ++j)
+    if (inside<VEC, TPR, VPT>(t, j, p.C)) s[0] += (v[j] - mean) * (v[j] - mean);
   row_sum<TPR, 1>(s, buf, turn, sub, t);
   rstd = 1.0f / sqrtf(s[0] / (float)p.C + p.eps);
 }
 
-template <typename X, typename Y, bool VEC, int TPR, int NV>
-__global__ __launch_bounds__(256) void residual_norm_fwd_kernel(const NormArgs p) {
+// Both directions: a workgroup of max(256, TPR) threads, TPR to a row, walks over the rows of one part of a gate row, or of several whole
+// gate rows, with the weights (and, backward, the parameter gradients) of its columns in registers.  The next row's loads are issued before
+// the current one is worked on, so that the reductions' barriers stand in the shadow of memory.
+template <int TPR> constexpr int threads() { return TPR > 256 ? TPR : 256; }
+
+template <typename X, typename Y, bool VEC, int TPR, int VPT>
+__global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const NormArgs p) {
   __shared__ float buf[64];
-  constexpr int SUB = 256 / TPR;
+  constexpr int SUB = threads<TPR>() / TPR;
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
-  long long row = (long long)blockIdx.x * SUB + sub;
-  const bool there = row < p.rows;
-  if (TPR == 64 && !there) return;
-  if (!there) row = p.rows - 1;
   int turn = 0;
-  float x[NV][8], y[NV][8];
+  float w1[VPT], w2[VPT], b1[VPT], b2[VPT];
+  if (p.w1) loadf<VEC, TPR, VPT>(p.w1, t, C, w1);
+  if (p.b1) loadf<VEC, TPR, VPT>(p.b1, t, C, b1);
+  if (p.w2) loadf<VEC, TPR, VPT>(p.w2, t, C, w2);
+  if (p.b2) loadf<VEC, TPR, VPT>(p.b2, t, C, b2);
+  const long long g0 = (long long)(blockIdx.x / p.chunks) * p.gates_per_wg, g1 = min(p.gates, g0 + p.gates_per_wg);
+  const int part = blockIdx.x % p.chunks;
+  for (long long g = g0; g < g1; ++g) {
+    const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
+    float gate[VPT];
+    if (p.gate) loadf<VEC, TPR, VPT>(p.gate + g * C, t, C, gate);
+    Raw<X, VPT> xn;
+    Raw<Y, VPT> yn;
+    auto fetch = [&](long long r) {
+      const long long row = min(r + sub, last - 1);
+      load<Y, VEC, TPR, VPT>((const Y*)p.y + row * C, t, C, yn);
+      load<X, VEC, TPR, VPT>((const X*)p.x + row * C, t, C, xn);
+    };
+    if (first < last) fetch(first);
+    for (long long r0 = first; r0 < last; r0 += SUB) {
+      const bool there = r0 + sub < last;
+      const long long row = there ? r0 + sub : last - 1;
+      float x[VPT], y[VPT];
+      floats(xn, x);
+      floats(yn, y);
+      if (r0 + SUB < last) fetch(r0 + SUB);
+      float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
+      if (p.after) {
+        statistics<VEC, TPR, VPT>(y, p, buf, turn, sub, t, m1, r1);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    load8<Y, VEC, TPR>((const Y*)p.y + row * C, i, t, C, y[i]);
-    load8<X, VEC, TPR>((const X*)p.x + row * C, i, t, C, x[i]);
-  }
-  float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
-  if (p.after) {
-    statistics<VEC, TPR, NV>(y, p, buf, turn, sub, t, m1, r1);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float w[8], b[8];
-      if (p.w1) load8<float, VEC, TPR>(p.w1, i, t, C, w);
-      if (p.b1) load8<float, VEC, TPR>(p.b1, i, t, C, b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float v = (y[i][j] - m1) * r1;
-        if (p.w1) v *= w[j];
-        if (p.b1) v += b[j];
-        y[i][j] = v;
+        for (int j = 0; j < VPT; ++j) {
+          y[j] = (y[j] - m1) * r1;
+          if (p.w1) y[j] *= w1[j];
+          if (p.b1) y[j] += b1[j];
+        }
       }
-    }
-  }
-  const float* gate = p.gate ? p.gate + (row / p.per_gate) * C : nullptr;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float g[8];
-    if (gate) load8<float, VEC, TPR>(gate, i, t, C, g);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float u = gate ? y[i][j] * g[j] : y[i][j];
-      x[i][j] = in8<VEC, TPR>(i, t, j, C) ? p.a * x[i][j] + u : 0.f;
-    }
-    if (there) store8<X, VEC, TPR>((X*)p.h + row * C, i, t, C, x[i]);
-  }
-  if (p.before) {
-    statistics<VEC, TPR, NV>(x, p, buf, turn, sub, t, m2, r2);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float w[8], b[8];
-      if (p.w2) load8<float, VEC, TPR>(p.w2, i, t, C, w);
-      if (p.b2) load8<float, VEC, TPR>(p.b2, i, t, C, b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float v = (x[i][j] - m2) * r2;
-        if (p.w2) v *= w[j];
-        if (p.b2) v += b[j];
-        x[i][j] = v;
+      for (int j = 0; j < VPT; ++j) {
+        if (p.gate) y[j] *= gate[j];
+        x[j] = inside<VEC, TPR, VPT>(t, j, C) ? p.a * x[j] + y[j] : 0.f;
       }
-      if (there) store8<Y, VEC, TPR>((Y*)p.n + row * C, i, t, C, x[i]);
+      if (there) store<X, VEC, TPR, VPT>((X*)p.h + row * C, t, C, x);
+      if (p.before) {
+        statistics<VEC, TPR, VPT>(x, p, buf, turn, sub, t, m2, r2);
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+          x[j] = (x[j] - m2) * r2;
+          if (p.w2) x[j] *= w2[j];
+          if (p.b2) x[j] += b2[j];
+        }
+        if (there) store<Y, VEC, TPR, VPT>((Y*)p.n + row * C, t, C, x);
+      }
+      if (p.stats && there && t == 0) reinterpret_cast<float4*>(p.stats)[row] = make_float4(m1, r1, m2, r2);
     }
   }
-  if (p.stats && there && t == 0) reinterpret_cast<float4*>(p.stats)[row] = make_float4(m1, r1, m2, r2);
 }
 
-// One workgroup of max(256, TPR) threads walks over the rows of one part of a gate row, or of several whole gate rows, and keeps the
-// parameter gradients of its columns in registers.
-template <typename X, typename Y, bool VEC, int TPR>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kernel(const NormArgs p) {
-  constexpr int THREADS = TPR > 256 ? TPR : 256, SUB = THREADS / TPR;
+template <typename X, typename Y, bool VEC, int TPR, int VPT>
+__global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const NormArgs p) {
+  constexpr int SUB = threads<TPR>() / TPR;
   __shared__ float buf[64];
-  __shared__ float join[SUB > 1 ? SUB * TPR * 8 : 1];
+  __shared__ float join[SUB > 1 ? SUB * TPR * VPT : 1];
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
   int turn = 0;
-  float w1[8], w2[8], b1[8];
-  if (p.w1) load8<float, VEC, TPR>(p.w1, 0, t, C, w1);
-  if (p.b1) load8<float, VEC, TPR>(p.b1, 0, t, C, b1);
-  if (p.w2) load8<float, VEC, TPR>(p.w2, 0, t, C, w2);
-  float sw1[8], sb1[8], sw2[8], sb2[8], sg[8];
+  float w1[VPT], w2[VPT], b1[VPT];
+  if (p.w1) loadf<VEC, TPR, VPT>(p.w1, t, C, w1);
+  if (p.b1) loadf<VEC, TPR, VPT>(p.b1, t, C, b1);
+  if (p.w2) loadf<VEC, TPR, VPT>(p.w2, t, C, w2);
+  float sw1[VPT], sb1[VPT], sw2[VPT], sb2[VPT], sg[VPT];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sw1[j] = sb1[j] = sw2[j] = sb2[j] = 0.f;
+  for (int j = 0; j < VPT; ++j) sw1[j] = sb1[j] = sw2[j] = sb2[j] = 0.f;
   const long long g0 = (long long)(blockIdx.x / p.chunks) * p.gates_per_wg, g1 = min(p.gates, g0 + p.gates_per_wg);
   const int part = blockIdx.x % p.chunks;
   float* slot = p.partial + (long long)blockIdx.x * VECTORS * C;
 
   // adds the row groups' sums of one vector and writes it (join is free again behind it)
-  auto put = [&](float (&v)[8], float* to) {
+  auto put = [&](float (&v)[VPT], float* to) {
     if (SUB > 1) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) join[(sub * 8 + j) * TPR + t] = v[j];
+      for (int j = 0; j < VPT; ++j) join[(sub * VPT + j) * TPR + t] = v[j];
       __syncthreads();
       if (sub == 0)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          for (int s = 1; s < SUB; ++s) v[j] += join[(s * 8 + j) * TPR + t];
+        for (int j = 0; j < VPT; ++j)
+          for (int s = 1; s < SUB; ++s) v[j] += join[(s * VPT + j) * TPR + t];
     }
-    if (sub == 0) store8<float, VEC, TPR>(to, 0, t, C, v);
+    if (sub == 0) store<float, VEC, TPR, VPT>(to, t, C, v);
   };
 
   for (long long g = g0; g < g1; ++g) {
     const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
-    float gate[8];
-    if (p.gate) load8<float, VEC, TPR>(p.gate + g * C, 0, t, C, gate);
+    float gate[VPT];
+    if (p.gate) loadf<VEC, TPR, VPT>(p.gate + g * C, t, C, gate);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sg[j] = 0.f;
+    for (int j = 0; j < VPT; ++j) sg[j] = 0.f;
+    Raw<X, VPT> xn, dhn;
+    Raw<Y, VPT> yn, dnn;
+    float4 stn;
+    auto fetch = [&](long long r) {
+      const long long row = min(r + sub, last - 1);
+      load<Y, VEC, TPR, VPT>((const Y*)p.y + row * C, t, C, yn);
+      load<X, VEC, TPR, VPT>((const X*)p.x + row * C, t, C, xn);
+      if (p.dn) load<Y, VEC, TPR, VPT>((const Y*)p.dn + row * C, t, C, dnn);
+      if (p.dh) load<X, VEC, TPR, VPT>((const X*)p.dh + row * C, t, C, dhn);
+      stn = reinterpret_cast<const float4*>(p.stats)[row];
+    };
+    if (first < last) fetch(first);
     for (long long r0 = first; r0 < last; r0 += SUB) {
       const bool there = r0 + sub < last;
       const long long row = there ? r0 + sub : last - 1;
-      float x[8], y[8], dh[8], dn[8];
-      load8<Y, VEC, TPR>((const Y*)p.y + row * C, 0, t, C, y);
-      load8<X, VEC, TPR>((const X*)p.x + row * C, 0, t, C, x);
-      if (p.dn) load8<Y, VEC, TPR>((const Y*)p.dn + row * C, 0, t, C, dn);
-      if (p.dh) load8<X, VEC, TPR>((const X*)p.dh + row * C, 0, t, C, dh);
-      const float4 st = reinterpret_cast<const float4*>(p.stats)[row];
-      float u[8];
+      float x[VPT], y[VPT], dh[VPT], dn[VPT], u[VPT];
+      floats(xn, x);
+      floats(yn, y);
+      floats(dhn, dh);
+      floats(dnn, dn);
+      const float4 st = stn;
+      if (r0 + SUB < last) fetch(r0 + SUB);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < VPT; ++j) {
         if (!p.dh) dh[j] = 0.f;
         y[j] = p.after ? (y[j] - st.x) * st.y : y[j];
         u[j] = y[j];
@@ -266,10 +270,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
       if (p.before && p.dn) {
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool in = in8<VEC, TPR>(0, t, j, C);
+        for (int j = 0; j < VPT; ++j) {
           const float hat = (p.a * x[j] + (p.gate ? u[j] * gate[j] : u[j]) - st.z) * st.w;
-          x[j] = in ? hat : 0.f;
+          x[j] = inside<VEC, TPR, VPT>(t, j, C) ? hat : 0.f;
           if (there) {
             sw2[j] += dn[j] * x[j];
             sb2[j] += dn[j];
@@ -281,14 +284,14 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
         row_sum<TPR, 2>(s, buf, turn, sub, t);
         const float c1 = p.rms ? 0.f : s[0] / (float)C, c2 = s[1] / (float)C;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dh[j] += st.w * (dn[j] - c1 - x[j] * c2);
+        for (int j = 0; j < VPT; ++j) dh[j] += st.w * (dn[j] - c1 - x[j] * c2);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = p.a * dh[j];
-      if (there && p.dx) store8<X, VEC, TPR>((X*)p.dx + row * C, 0, t, C, x);
+      for (int j = 0; j < VPT; ++j) x[j] = p.a * dh[j];
+      if (there && p.dx) store<X, VEC, TPR, VPT>((X*)p.dx + row * C, t, C, x);
       if (p.gate) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < VPT; ++j) {
           if (there) sg[j] += dh[j] * u[j];
           dh[j] *= gate[j];
         }
@@ -296,8 +299,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
       if (p.after) {
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (!in8<VEC, TPR>(0, t, j, C)) y[j] = dh[j] = 0.f;
+        for (int j = 0; j < VPT; ++j) {
+          if (!inside<VEC, TPR, VPT>(t, j, C)) y[j] = dh[j] = 0.f;
           if (there) {
             sw1[j] += dh[j] * y[j];
             sb1[j] += dh[j];
@@ -309,9 +312,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
         row_sum<TPR, 2>(s, buf, turn, sub, t);
         const float c1 = p.rms ? 0.f : s[0] / (float)C, c2 = s[1] / (float)C;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dh[j] = st.y * (dh[j] - c1 - y[j] * c2);
+        for (int j = 0; j < VPT; ++j) dh[j] = st.y * (dh[j] - c1 - y[j] * c2);
       }
-      if (there && p.dy) store8<Y, VEC, TPR>((Y*)p.dy + row * C, 0, t, C, dh);
+      if (there && p.dy) store<Y, VEC, TPR, VPT>((Y*)p.dy + row * C, t, C, dh);
     }
     if (p.want_gate) put(sg, p.chunks == 1 ? p.dgate + g * C : slot + V_GATE * C);
   }
@@ -321,7 +324,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void residual_norm_bwd_kerne
   if (p.want_b1) put(sb1, slot + V_B1 * C);
 }
 
-// column sums of the partial vectors: 64 columns per workgroup, its four waves take every fourth slot
+// column sums of the partial vectors: 64 columns per workgroup, its sixteen waves take every sixteenth slot
 struct NormSumArgs {
   const float* partial;
   float* out[VECTORS];
@@ -329,46 +332,59 @@ struct NormSumArgs {
   int chunks;                // slots of one gate row
   long long gates;
 };
-__global__ __launch_bounds__(256) void residual_norm_sum_kernel(const NormSumArgs p) {
-  __shared__ float part[4][64];
+__global__ __launch_bounds__(1024) void residual_norm_sum_kernel(const NormSumArgs p) {
+  __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
   const bool gate = blockIdx.y >= V_GATE;
   const int v = gate ? V_GATE : blockIdx.y;
   const long long g = gate ? blockIdx.y - V_GATE : 0;
   if (!p.out[v]) return;
-  const long long s0 = gate ? g * p.chunks : 0, n = gate ? p.chunks : p.slots;
-  float s = 0.f;
-  if (c < p.C)
-    for (long long i = wave; i < n; i += 4) s += p.partial[((s0 + i) * VECTORS + v) * p.C + c];
-  part[wave][lane] = s;
+  const long long s0 = gate ? g * p.chunks : 0, n = gate ? p.chunks : p.slots, step = (long long)VECTORS * p.C;
+  const float* from = p.partial + (s0 * VECTORS + v) * p.C + c;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < p.C) {
+    long long i = wave;
+    for (; i + 48 < n; i += 64)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += from[(i + 16 * k) * step];
+    for (; i < n; i += 16) s[0] += from[i * step];
+  }
+  part[wave][lane] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
-  if (wave == 0 && c < p.C) p.out[v][g * p.C + c] = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+  if (wave == 0 && c < p.C) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += part[k][lane];
+    p.out[v][g * p.C + c] = t;
+  }
 }
 
+// four values per thread keep the backward's registers (five sums, four weights, two rows) under 128; widths over 4096 take eight
+#define ASYRP_NORM(KERNEL) \
+  if (a.C <= 256) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 64, 4>), g, dim3(256), 0, s, a); \
+  else if (a.C <= 512) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 128, 4>), g, dim3(256), 0, s, a); \
+  else if (a.C <= 1024) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 256, 4>), g, dim3(256), 0, s, a); \
+  else if (a.C <= 2048) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 512, 4>), g, dim3(512), 0, s, a); \
+  else if (a.C <= 4096) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 1024, 4>), g, dim3(1024), 0, s, a); \
+  else hipLaunchKernelGGL((KERNEL<X, Y, VEC, 1024, 8>), g, dim3(1024), 0, s, a)
+
 template <typename X, typename Y, bool VEC>
-hipError_t forward(const NormArgs& a, hipStream_t s) {
-  const dim3 b(256), g4((unsigned)((a.rows + 3) / 4)), g1((unsigned)a.rows);
-  if (a.C <= 512) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 64, 1>), g4, b, 0, s, a);
-  else if (a.C <= 1024) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 64, 2>), g4, b, 0, s, a);
-  else if (a.C <= 2048) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 64, 4>), g4, b, 0, s, a);
-  else if (a.C <= 4096) hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 256, 2>), g1, b, 0, s, a);
-  else hipLaunchKernelGGL((residual_norm_fwd_kernel<X, Y, VEC, 256, 4>), g1, b, 0, s, a);
+hipError_t forward(const NormArgs& a, unsigned wgs, hipStream_t s) {
+  const dim3 g(wgs);
+  ASYRP_NORM(residual_norm_fwd_kernel);
   return hipGetLastError();
 }
 template <typename X, typename Y, bool VEC>
 hipError_t backward(const NormArgs& a, unsigned wgs, hipStream_t s) {
   const dim3 g(wgs);
-  if (a.C <= 512) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 64>), g, dim3(256), 0, s, a);
-  else if (a.C <= 1024) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 128>), g, dim3(256), 0, s, a);
-  else if (a.C <= 2048) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 256>), g, dim3(256), 0, s, a);
-  else if (a.C <= 4096) hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 512>), g, dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((residual_norm_bwd_kernel<X, Y, VEC, 1024>), g, dim3(1024), 0, s, a);
+  ASYRP_NORM(residual_norm_bwd_kernel);
   return hipGetLastError();
 }
+#undef ASYRP_NORM
 template <typename X, typename Y>
 hipError_t launch(const NormArgs& a, bool vec, bool back, unsigned wgs, hipStream_t s) {
   if (back) return vec ? backward<X, Y, true>(a, wgs, s) : backward<X, Y, false>(a, wgs, s);
-  return vec ? forward<X, Y, true>(a, s) : forward<X, Y, false>(a, s);
+  return vec ? forward<X, Y, true>(a, wgs, s) : forward<X, Y, false>(a, wgs, s);
 }
 bool types(int x, int y) { return (x == ASYRP_F32 && (y == ASYRP_F32 || y == ASYRP_F16 || y == ASYRP_BF16)) || (x == y && (x == ASYRP_F16 || x == ASYRP_BF16)); }
 hipError_t dispatch(int x, int y, const NormArgs& a, bool vec, bool back, unsigned wgs, hipStream_t s) {
@@ -390,18 +406,19 @@ int check(const asyrp_residual_norm* p) {
   if (!std::isfinite(p->eps) || p->eps < 0 || !std::isfinite(p->residual_scale)) return refuse("residual norm: eps and the residual scale must be finite");
   return 0;
 }
-// How the backward's rows are dealt out: 1024 workgroups (four per CU) where the rows allow, each with a part of one gate row
-// or with several whole ones; at least 16 rows each, so that the partial sums stay a small part of the traffic.
-void deal(const asyrp_residual_norm* p, NormArgs& a, unsigned& wgs) {
+// How the rows are dealt out: `want` workgroups where the rows allow, each with a part of one gate row or with several whole ones
+void deal(const asyrp_residual_norm* p, NormArgs& a, long long want, unsigned& wgs) {
   a.gates = p->gates > 0 ? p->gates : 1;
   a.per_gate = std::max<long long>(1, a.rows / a.gates);
-  const long long want = std::max<long long>(1, std::min<long long>(1024, a.rows / 16));
+  want = std::max<long long>(1, want);
   a.chunks = (int)std::max<long long>(1, std::min(want / a.gates, a.per_gate));
   a.chunk_rows = (a.per_gate + a.chunks - 1) / a.chunks;
   a.chunks = (int)((a.per_gate + a.chunk_rows - 1) / a.chunk_rows);
   a.gates_per_wg = a.chunks > 1 ? 1 : (a.gates + want - 1) / want;
   wgs = (unsigned)(((a.gates + a.gates_per_wg - 1) / a.gates_per_wg) * a.chunks);
 }
+// backward: at least four rows each, so that the partial sums stay a small part of the traffic
+long long bwd_want(long long rows) { return std::min<long long>(1024, rows / 4); }
 void fill(const asyrp_residual_norm* p, NormArgs& a) {
   a.rows = p->rows;
   a.C = p->width;
@@ -435,9 +452,11 @@ int asyrp_residual_norm_forward(int device, const asyrp_residual_norm* p, const 
   a.x = x; a.y = y; a.gate = gate; a.w1 = after_weight; a.b1 = after_bias; a.w2 = before_weight; a.b2 = before_bias; a.h = h; a.n = n; a.stats = stats;
   if (!aligned({stats})) return refuse("residual norm: the statistics must be 16-byte aligned");
   const bool vec = a.C % 8 == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, before_bias, h, n});
+  unsigned wgs = 0;
+  deal(p, a, std::min<long long>(2048, a.rows), wgs);
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
-  const hipError_t e = dispatch(p->stream_dtype, p->branch_dtype, a, vec, false, 0, (hipStream_t)stream);
+  const hipError_t e = dispatch(p->stream_dtype, p->branch_dtype, a, vec, false, wgs, (hipStream_t)stream);
   return e == hipSuccess ? 0 : set_last_error(ASYRP_EHIP, hipGetErrorString(e));
 }
 
@@ -446,7 +465,7 @@ int64_t asyrp_residual_norm_workspace(const asyrp_residual_norm* p) {
   NormArgs a{};
   fill(p, a);
   unsigned wgs = 0;
-  deal(p, a, wgs);
+  deal(p, a, bwd_want(a.rows), wgs);
   return (int64_t)wgs * VECTORS * a.C;
 }
 
@@ -465,7 +484,7 @@ int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const
   NormArgs a{};
   fill(p, a);
   unsigned wgs = 0;
-  deal(p, a, wgs);
+  deal(p, a, bwd_want(a.rows), wgs);
   a.x = x; a.y = y; a.gate = gate; a.w1 = after_weight; a.b1 = after_bias; a.w2 = before_weight; a.stats = const_cast<float*>(stats);
   a.dh = dh; a.dn = dn; a.dx = dx; a.dy = dy; a.partial = workspace; a.dgate = dgate;
   a.want_w2 = d_before_weight != nullptr; a.want_b2 = d_before_bias != nullptr; a.want_w1 = d_after_weight != nullptr; a.want_b1 = d_after_bias != nullptr;
@@ -486,7 +505,7 @@ int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const
     bool any = false;
     for (float* o : sa.out) any = any || o;
     if (any) {
-      hipLaunchKernelGGL(residual_norm_sum_kernel, dim3((a.C + 63) / 64, V_GATE + (sa.out[V_GATE] ? (unsigned)a.gates : 0)), dim3(256), 0, (hipStream_t)stream, sa);
+      hipLaunchKernelGGL(residual_norm_sum_kernel, dim3((a.C + 63) / 64, V_GATE + (sa.out[V_GATE] ? (unsigned)a.gates : 0)), dim3(1024), 0, (hipStream_t)stream, sa);
       e = hipGetLastError();
     }
   }

@@ -6,23 +6,23 @@ attention and the seams between their residual blocks are the work there that is
   gated_residual_norm   norm behind a block, gate, residual sum with its scale, norm in front of the next block
 Both run on the current stream of their tensors' device, keep nothing between calls, and may be captured into a graph.
 """
-import ctypes as C
 import math
 
 import torch
 
 from . import _lib
-from .engine import AsyrpDeviceError, _ptr
+from .engine import AsyrpDeviceError
+
+_HALF = (torch.float16, torch.bfloat16)
+_TYPES = tuple(_lib.DTYPES)
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle (torch.cuda.current_stream() without its object)
 
 
-def _tensor(t, name, dtypes, dim=None):
+def _tensor(t, name, dtypes):
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise AsyrpDeviceError(f"{name} must be a CUDA(HIP) tensor — the operator has no CPU path")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
-    if dim is not None and t.dim() != dim:
-        raise ValueError(f"{name} must have {dim} dimensions, got shape {tuple(t.shape)}")
-    return t
 
 
 def _same_device(first, *named):
@@ -31,62 +31,71 @@ def _same_device(first, *named):
             raise AsyrpDeviceError(f"{name} lives on {t.device}, the other arguments on {first.device}")
 
 
-def _stream(t):
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------------------
-def _heads_layout(t):
-    """`t` [tokens, heads, head_dim] as the kernels read it: last axis contiguous, other strides multiples of 8 values, 16-byte address.
-    Views of a fused q|k|v projection are; anything else is copied.  A dimension of one has no stride of its own."""
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[d] <= 1 or (t.stride(d) % 8 == 0 and t.stride(d) > 0) for d in (0, 1))
-    return t if ok else t.contiguous().clone() if t.is_contiguous() else t.contiguous()
-
-
 def _strides(t):
-    return tuple(t.stride(d) if t.shape[d] > 1 else t.shape[2] for d in (0, 1))
+    """(token, head) strides of `t` [tokens, heads, head_dim] where the kernels can read it in place: last axis contiguous, the others
+    multiples of 8 values and rows at most 2^23 apart, 16-byte address; None elsewhere.  An axis of one has no stride of its own."""
+    (n, h, d), (a, b, c) = t.shape, t.stride()
+    if n <= 1:
+        a = d
+    if h <= 1:
+        b = d
+    return (a, b) if c == 1 and a > 0 and b > 0 and not (a | b) & 7 and a <= 1 << 23 and not t.data_ptr() & 15 else None
 
 
-def _attention_struct(q, k, v, out, cu, causal, scale, dout=None):
-    p = _lib.PackedAttention()
-    p.tokens, p.sequences, p.heads, p.kv_heads, p.head_dim = q.shape[0], cu.shape[0] - 1, q.shape[1], k.shape[1], q.shape[2]
-    p.causal, p.dtype, p.scale = int(causal), _lib.DTYPES[q.dtype], scale
-    p.q_stride[:], p.k_stride[:], p.v_stride[:], p.out_stride[:] = _strides(q), _strides(k), _strides(v), _strides(out)
-    if dout is not None:
-        p.dout_stride[:] = _strides(dout)
-    return p
+def _readable(t):
+    st = _strides(t)
+    if st is not None:
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _strides(t)
 
 
-def _attention_forward(q, k, v, cu, causal, scale, out, want_lse):
-    q, k, v = _heads_layout(q), _heads_layout(k), _heads_layout(v)
-    fresh = out is None
-    if fresh:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) if want_lse else None
-    p = _attention_struct(q, k, v, out, cu, causal, scale)
-    _lib.check(_lib.load().asyrp_packed_attention_forward(q.device.index, C.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(cu), _ptr(out), _ptr(lse),
-                                                          int(fresh), _stream(q)))
-    return q, k, v, out, lse
+def _attention_forward(q, k, v, cu, causal, scale, out, train):
+    q, sq = _readable(q)
+    k, sk = _readable(k)
+    v, sv = _readable(v)
+    fill = out is None
+    if fill:
+        out = q.new_empty(q.shape)
+    T, H, D = q.shape
+    lse = q.new_empty((H, T), dtype=torch.float32) if train else None
+    rest = q.new_empty(q.shape) if train else None
+    spec = (T, cu.shape[0] - 1, H, k.shape[1], D, causal, _lib.DTYPES[q.dtype], scale, *sq, *sk, *sv, *_strides(out))
+    device = q.device.index
+    rc = _lib.load().asyrp_packed_attention_forward(device, _lib.PACKED_ATTENTION.pack(*spec, 0, 0), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(),
+                                                    out.data_ptr(), _ptr(lse), _ptr(rest), fill, _raw_stream(device))
+    if rc:
+        _lib.check(rc)
+    return q, k, v, out, lse, rest, spec
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, causal, scale):
-        q, k, v, out, lse = _attention_forward(q, k, v, cu, causal, scale, None, True)
-        ctx.save_for_backward(q, k, v, cu, out, lse)
-        ctx.causal, ctx.scale = causal, scale
+        q, k, v, out, lse, rest, ctx.spec = _attention_forward(q, k, v, cu, causal, scale, None, True)
+        ctx.save_for_backward(q, k, v, cu, out, lse, rest)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, cu, out, lse = ctx.saved_tensors
-        d_out = _heads_layout(d_out)
-        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
-        delta = torch.empty_like(lse)
-        p = _attention_struct(q, k, v, out, cu, ctx.causal, ctx.scale, d_out)
-        _lib.check(_lib.load().asyrp_packed_attention_backward(q.device.index, C.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(cu), _ptr(out), _ptr(lse),
-                                                               _ptr(d_out), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv), _stream(q)))
+        q, k, v, cu, out, lse, rest = ctx.saved_tensors
+        d_out, sd = _readable(d_out)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        lib, device, spec = _lib.load(), q.device.index, _lib.PACKED_ATTENTION.pack(*ctx.spec, *sd)
+        words = lib.asyrp_packed_attention_workspace(spec)
+        if words < 0:
+            _lib.check(words)
+        ws = q.new_empty((max(4, words),), dtype=torch.float32)
+        rc = lib.asyrp_packed_attention_backward(device, spec, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                                 rest.data_ptr(), d_out.data_ptr(), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _raw_stream(device))
+        if rc:
+            _lib.check(rc)
         return dq, dk, dv, None, None, None
 
 
@@ -103,11 +112,14 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
     the result's type and shape, laid out as q may be) takes the result and keeps what it holds in those rows.  Sums and softmax statistics are float32;
     probabilities are rounded to the inputs' type before they multiply v.  A value that is not finite may reach every row of its own sequence, the
     rows before it included, and no other sequence.  Results do not depend on the order in which the card works."""
-    _tensor(q, "q", (torch.float16, torch.bfloat16), 3)
-    _tensor(k, "k", (q.dtype,), 3)
-    _tensor(v, "v", (q.dtype,), 3)
-    _tensor(cu_seqlens, "cu_seqlens", (torch.int32,), 1)
+    _tensor(q, "q", _HALF)
+    same = (q.dtype,)
+    _tensor(k, "k", same)
+    _tensor(v, "v", same)
+    _tensor(cu_seqlens, "cu_seqlens", (torch.int32,))
     _same_device(q, ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("out", out))
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"q and k must be [tokens, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
     T, H, D = q.shape
     if k.shape != v.shape or k.shape[0] != T or k.shape[2] != D:
         raise ValueError(f"k and v must be [{T}, kv_heads, {D}] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -115,22 +127,22 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
         raise ValueError(f"{H} query heads are no multiple of {k.shape[1]} key / value heads")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"head_dim must be a multiple of 8 from 8 to 128, got {D}")
-    if cu_seqlens.shape[0] < 2:
-        raise ValueError("cu_seqlens needs at least two offsets")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        raise ValueError(f"cu_seqlens must be a vector of at least two offsets, got shape {tuple(cu_seqlens.shape)}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
-    cu = cu_seqlens.detach().contiguous()
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    cu, causal = cu_seqlens.contiguous(), bool(causal)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:
-        _tensor(out, "out", (q.dtype,), 3)
+        _tensor(out, "out", same)
         if grad:
             raise ValueError("out= takes part in no graph: call without it, or under torch.no_grad()")
-        if out.shape != q.shape or _heads_layout(out) is not out:
+        if out.shape != q.shape or _strides(out) is None:
             raise ValueError(f"out must be {tuple(q.shape)} with its last axis contiguous, other strides multiples of 8 values and a 16-byte address")
     if grad:
-        return _PackedAttention.apply(q, k, v, cu, bool(causal), scale)
-    return _attention_forward(q, k, v, cu, bool(causal), scale, out, False)[3]
+        return _PackedAttention.apply(q, k, v, cu, causal, scale)
+    return _attention_forward(q, k, v, cu, causal, scale, out, False)[3]
 
 
 # ---- the seam between two residual blocks ------------------------------------------------------------------------------------------------
@@ -139,19 +151,18 @@ _KINDS = {"layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
 
 class _GatedResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, gate, w1, b1, w2, b2, kind, after, before, scale, eps, keep):
-        p = _lib.ResidualNorm()
-        p.rows, p.width, p.gates = x.shape[0], x.shape[1], 0 if gate is None else gate.shape[0]
-        p.kind, p.after, p.before = _KINDS[kind], int(after), int(before)
-        p.stream_dtype, p.branch_dtype, p.residual_scale, p.eps = _lib.DTYPES[x.dtype], _lib.DTYPES[y.dtype], scale, eps
-        h = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        n = torch.empty(y.shape, device=x.device, dtype=y.dtype) if before else None
-        stats = torch.empty((x.shape[0], 4), device=x.device, dtype=torch.float32) if keep else None
-        _lib.check(_lib.load().asyrp_residual_norm_forward(x.device.index, C.byref(p), _ptr(x), _ptr(y), _ptr(gate), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2),
-                                                           _ptr(h), _ptr(n), _ptr(stats), _stream(x)))
+    def forward(ctx, x, y, gate, w1, b1, w2, b2, spec, before, keep):
+        h = x.new_empty(x.shape)
+        n = y.new_empty(y.shape) if before else None
+        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32) if keep else None
+        device = x.device.index
+        rc = _lib.load().asyrp_residual_norm_forward(device, spec, x.data_ptr(), y.data_ptr(), _ptr(gate), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), h.data_ptr(),
+                                                     _ptr(n), _ptr(stats), _raw_stream(device))
+        if rc:
+            _lib.check(rc)
         if keep:
             ctx.save_for_backward(x, y, gate, w1, b1, w2, b2, stats)
-            ctx.p = p
+            ctx.spec = spec
             ctx.set_materialize_grads(False)
         return h, n
 
@@ -159,34 +170,34 @@ class _GatedResidualNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dn):
         if dh is None and dn is None:
-            return (None,) * 13
+            return (None,) * 10
         x, y, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
-        p, need = ctx.p, ctx.needs_input_grad
-        dh, dn = (None if t is None else _rows_layout(t) for t in (dh, dn))
-        dx, dy = (torch.empty(t.shape, device=t.device, dtype=t.dtype) if n else None for t, n in ((x, need[0]), (y, need[1])))
-        # without a gradient of n, the norm in front of the next block takes no part: its parameters' gradients are zero
-        zero = dn is None or x.shape[0] == 0
-        outs = [None if t is None or not n else torch.zeros_like(t) if z else torch.empty_like(t)
-                for t, n, z in ((gate, need[2], x.shape[0] == 0), (w1, need[3], x.shape[0] == 0), (b1, need[4], x.shape[0] == 0), (w2, need[5], zero), (b2, need[6], zero))]
-        lib = _lib.load()
-        words = lib.asyrp_residual_norm_workspace(C.byref(p))
+        need = ctx.needs_input_grad
+        dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
+        dx, dy = (t.new_empty(t.shape) if n else None for t, n in ((x, need[0]), (y, need[1])))
+        # without rows every sum is empty; without a gradient of n, the norm in front of the next block takes no part
+        empty = x.shape[0] == 0
+        outs = [None if t is None or not n else t.new_zeros(t.shape) if empty or (k > 2 and dn is None) else t.new_empty(t.shape)
+                for k, (t, n) in enumerate(zip((gate, w1, b1, w2, b2), need[2:7]))]
+        late = outs[3:] if dn is not None else (None, None)
+        lib, device = _lib.load(), x.device.index
+        words = lib.asyrp_residual_norm_workspace(ctx.spec)
         if words < 0:
-            _lib.check(int(words))
-        ws = torch.empty(max(4, words), device=x.device, dtype=torch.float32)
-        _lib.check(lib.asyrp_residual_norm_backward(x.device.index, C.byref(p), _ptr(x), _ptr(y), _ptr(gate), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(stats), _ptr(dh),
-                                                    _ptr(dn), _ptr(dx), _ptr(dy), _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]), None if zero else _ptr(outs[3]),
-                                                    None if zero else _ptr(outs[4]), _ptr(ws), _stream(x)))
-        return (dx, dy, *outs, None, None, None, None, None, None)
-
-
-def _rows_layout(t):
-    """Contiguous rows; a copy also where the address is odd for the type's 16-byte loads is not needed: such rows are read value by value."""
-    return t.contiguous()
+            _lib.check(words)
+        ws = x.new_empty((max(4, words),), dtype=torch.float32)
+        rc = lib.asyrp_residual_norm_backward(device, ctx.spec, x.data_ptr(), y.data_ptr(), _ptr(gate), _ptr(w1), _ptr(b1), _ptr(w2), stats.data_ptr(), _ptr(dh),
+                                              _ptr(dn), _ptr(dx), _ptr(dy), _ptr(outs[0]), _ptr(outs[1]), _ptr(outs[2]), _ptr(late[0]), _ptr(late[1]), ws.data_ptr(),
+                                              _raw_stream(device))
+        if rc:
+            _lib.check(rc)
+        return (dx, dy, *outs, None, None, None)
 
 
 def _vector(t, name, width):
-    _tensor(t, name, tuple(_lib.DTYPES))
-    if tuple(t.shape) != (width,):
+    if t is None:
+        return None
+    _tensor(t, name, _TYPES)
+    if t.dim() != 1 or t.shape[0] != width:
         raise ValueError(f"{name} must be [{width}], got {tuple(t.shape)}")
     return t.float().contiguous()
 
@@ -200,36 +211,39 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, kind="layer", af
     x's other dimensions) and row r takes gate row r // (rows / gates): one gate per image of a batch, or one per row.
     h has x's type, n has y's.  Statistics, the sum h that the second norm sees and the sums of the parameters' gradients are float32; h and n are rounded once.
     Gates, weights and biases of any of the three types; their gradients come back in it."""
-    types = tuple(_lib.DTYPES)
-    _tensor(x, "x", types)
-    _tensor(y, "y", types)
-    if x.dim() < 1 or x.shape != y.shape:
-        raise ValueError(f"x and y must have one shape of at least one dimension, got {tuple(x.shape)} and {tuple(y.shape)}")
+    _tensor(x, "x", _TYPES)
+    _tensor(y, "y", _TYPES)
+    shape = x.shape
+    if not shape or shape != y.shape:
+        raise ValueError(f"x and y must have one shape of at least one dimension, got {tuple(shape)} and {tuple(y.shape)}")
     if x.dtype != y.dtype and x.dtype != torch.float32:
         raise ValueError(f"a stream in {x.dtype} takes a branch of the same type, got {y.dtype}")
     if kind not in _KINDS:
         raise ValueError(f"kind must be 'layer' or 'rms', got {kind!r}")
-    width, shape = x.shape[-1], x.shape
+    width, rows = shape[-1], math.prod(shape[:-1])
     if not 1 <= width <= 8192:
         raise ValueError(f"the width must be 1 to 8192, got {width}")
     residual_scale, eps = float(residual_scale), float(eps)
     if not math.isfinite(residual_scale) or not math.isfinite(eps) or eps < 0:
         raise ValueError("residual_scale and eps must be finite, eps not negative")
-    rows = math.prod(shape[:-1])
     if gate is not None:
-        _tensor(gate, "gate", types)
+        _tensor(gate, "gate", _TYPES)
         if gate.dim() == 1:
             gate = gate[None]
         if gate.dim() != 2 or gate.shape[1] != width or gate.shape[0] < 1 or rows % gate.shape[0]:
             raise ValueError(f"gate must be [{width}] or [gates, {width}] with gates dividing {rows} rows, got {tuple(gate.shape)}")
         gate = gate.float().contiguous()
-    pairs = []
-    for name, wb in (("after", after), ("before", before)):
-        if wb is not None and (not isinstance(wb, (tuple, list)) or len(wb) != 2):
+    for name, pair in (("after", after), ("before", before)):
+        if pair is not None and (not isinstance(pair, (tuple, list)) or len(pair) != 2):
             raise ValueError(f"{name} must be None or (weight, bias)")
-        pairs += [None if t is None else _vector(t, f"{name}[{i}]", width) for i, t in enumerate(wb or (None, None))]
-    _same_device(x, ("y", y), ("gate", gate), *((n, t) for n, t in zip(("after weight", "after bias", "before weight", "before bias"), pairs)))
-    x2, y2 = _rows_layout(x.reshape(rows, width)), _rows_layout(y.reshape(rows, width))
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, y2, gate, *pairs))
-    h, n = _GatedResidualNorm.apply(x2, y2, gate, *pairs, kind, after is not None, before is not None, residual_scale, eps, keep)
+    w1, b1 = (None, None) if after is None else (_vector(after[0], "after[0]", width), _vector(after[1], "after[1]", width))
+    w2, b2 = (None, None) if before is None else (_vector(before[0], "before[0]", width), _vector(before[1], "before[1]", width))
+    _same_device(x, ("y", y), ("gate", gate), ("after[0]", w1), ("after[1]", b1), ("before[0]", w2), ("before[1]", b2))
+    x2, y2 = x.reshape(rows, width).contiguous(), y.reshape(rows, width).contiguous()
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, y2, gate, w1, b1, w2, b2))
+    spec = _lib.RESIDUAL_NORM.pack(rows, 0 if gate is None else gate.shape[0], width, _KINDS[kind], after is not None, before is not None, _lib.DTYPES[x.dtype],
+                                   _lib.DTYPES[y.dtype], residual_scale, eps)
+    h, n = _GatedResidualNorm.apply(x2, y2, gate, w1, b1, w2, b2, spec, before is not None, keep)
+    if len(shape) == 2:
+        return h, n
     return h.view(shape), None if n is None else n.view(shape)

@@ -217,21 +217,14 @@ class AdamW(torch.optim.Optimizer):
             clip, self.grad_norm = both[0:2], both[2]
             _lib.check(lib.asyrp_grad_clip(device.index, _ptr(partial), at, self.max_norm, _ptr(self.grad_norm), _ptr(clip), stream))
         for g, mo, dtype, n, table, params in todo:
-            c = _lib.AdamWConfig()
-            lr = g["lr"]
+            lr, lr_device = g["lr"], 0
             if isinstance(lr, torch.Tensor) and lr.is_cuda:
                 if lr.dtype != torch.float32 or lr.device != device:
                     raise ValueError(f"lr as a device tensor must be float32 on {device}")
-                c.lr_device, c.lr = lr.data_ptr(), 0.0
-            else:
-                c.lr = float(lr)
-            (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
-            c.steps, c.clip = mo.steps.data_ptr(), None if clip is None else clip.data_ptr()
-            c.exp_avg, c.exp_avg_sq = mo.m.data_ptr(), mo.v.data_ptr()
-            if mo.bits == 8:
-                c.exp_avg_scale, c.exp_avg_sq_scale = mo.me.data_ptr(), mo.ve.data_ptr()
-            c.state_bits, c.seed = mo.bits, self.seed
+                lr, lr_device = 0.0, lr.data_ptr()
+            spec = _lib.ADAMW.pack(float(lr), *g["betas"], g["eps"], g["weight_decay"], lr_device, mo.steps.data_ptr(), 0 if clip is None else clip.data_ptr(),
+                                   mo.m.data_ptr(), mo.v.data_ptr(), *(p.data_ptr() if p is not None else 0 for p in (mo.me, mo.ve)), mo.bits, self.seed)
             scratch = torch.empty(32 * n, device=device, dtype=torch.uint8)
-            _lib.check(lib.asyrp_adamw_step(device.index, C.byref(c), table, n, dtype, _ptr(scratch), stream))
+            _lib.check(lib.asyrp_adamw_step(device.index, spec, table, n, dtype, _ptr(scratch), stream))
             torch.autograd.graph.increment_version(params)   # the engine re-uploads parameters whose version has moved
         return loss

@@ -101,7 +101,7 @@ typedef struct asyrp_packed_attention {
   int32_t head_dim;               /* multiple of 8, 8 .. 128 */
   int32_t causal;
   int32_t dtype;                  /* ASYRP_F16 or ASYRP_BF16 */
-  float scale;
+  float scale;                    /* > 0 */
   int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2], dout_stride[2];
 } asyrp_packed_attention;
 
@@ -291,12 +291,15 @@ int asyrp_sampler_update(int device, const float* x, const float* model_out, int
  *
  * Attention over sequences packed behind each other: sequence i = rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (device, sequences + 1
  * ascending values from 0; values outside [0, tokens] or falling ones are held inside the tensors but give no defined result).
- * lse [heads][tokens] (nullable in the forward) = log sum exp of the scaled scores.  Rows behind the last sequence are set to zero in the gradients
- * and, where fill_tail is not 0, in out.  The gradients are contiguous; delta [heads][tokens] is workspace. */
+ * lse [heads][tokens] (nullable in the forward) = log sum exp of the scaled scores.  out_rest [tokens][heads][head_dim] contiguous (nullable in both) = what the
+ * rounding of out took away, so that the backward's rowsum(d_out * out) is that of the unrounded output.  Rows behind the last sequence are set to zero in the gradients
+ * and, where fill_tail is not 0, in out.  The gradients are contiguous; workspace: asyrp_packed_attention_workspace() floats (negative: an
+ * error code). */
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                   void* out, float* lse, int fill_tail, void* stream);
+                                   void* out, float* lse, void* out_rest, int fill_tail, void* stream);
+int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p);
 int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                    const void* out, const float* lse, const void* d_out, float* delta, void* dq, void* dk, void* dv, void* stream);
+                                    const void* out, const float* lse, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream);
 
 /* h = residual_scale * x + gate * N1(y), n = N2(h): the norm behind a block, its gate, the residual sum and the norm in front of the next block.
  * gate [gates][width], row r takes gate row r / (rows / gates); weights and biases [width] f32, nullable each; n only where `before`.
