@@ -36,7 +36,7 @@ ADAMW_PARTIALS, ADAMW_TABLE = 1024, 100
 # include/asyrp.h asyrp_packed_attention / asyrp_residual_norm / asyrp_adamw, field by field in the C compiler's own alignment
 PACKED_ATTENTION = struct.Struct("@qiiiiiif10q")
 RESIDUAL_NORM = struct.Struct("@qqiiiiiiff")
-ADAMW = struct.Struct("@dddddPPPPPPPiI")
+ADAMW = struct.Struct("@dddddPPPdPPPPPiiI4x")
 
 
 _P, _F, _I = C.c_void_p, C.c_float, C.c_int
@@ -69,7 +69,6 @@ _SIGS = {
     "asyrp_residual_norm_workspace": (C.c_int64, [_P]),
     "asyrp_residual_norm_backward": (C.c_int, [_I] + [_P] * 19),
     "asyrp_grad_sumsq": (C.c_int, [_I, _P, _I, _I, _P, _P]),
-    "asyrp_grad_clip": (C.c_int, [_I, _P, _I, C.c_double, _P, _P, _P]),
     "asyrp_adamw_step": (C.c_int, [_I, _P, _P, _I, _I, _P, _P]),
     "asyrp_adamw_moments": (C.c_int, [_I, _P, _P, _P, _P, C.c_int64, _P, _P, _P]),
     "asyrp_device_bytes": (C.c_int64, [_P]),

@@ -61,10 +61,10 @@ __device__ __forceinline__ int tensor_of(const Table& tb, int chunk) {
 
 template <typename T> struct Four { typedef T V __attribute__((ext_vector_type(4))); };
 
-// four values, as one load where the tensor's address allows it
+// four values, as one load where all are there and the tensor's address allows it
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, long long i, long long n, bool wide, float (&o)[4]) {
-  if (wide && i + 4 <= n) {
+__device__ __forceinline__ void load4(const T* p, long long i, long long n, bool whole, float (&o)[4]) {
+  if (whole) {
     const typename Four<T>::V v = *reinterpret_cast<const typename Four<T>::V*>(p + i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = (float)v[j];
@@ -74,8 +74,8 @@ __device__ __forceinline__ void load4(const T* p, long long i, long long n, bool
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, long long i, long long n, bool wide, const float (&o)[4]) {
-  if (wide && i + 4 <= n) {
+__device__ __forceinline__ void store4(T* p, long long i, long long n, bool whole, const float (&o)[4]) {
+  if (whole) {
     typename Four<T>::V v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = (T)o[j];
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(const Table tb, double*
     const bool wide = ((uintptr_t)g & (4 * sizeof(T) - 1)) == 0;
     float v[CHUNK / 1024][4];
 #pragma unroll
-    for (int it = 0; it < CHUNK / 1024; ++it) load4(g, base + it * 1024 + threadIdx.x * 4, n, wide, v[it]);
+    for (int it = 0; it < CHUNK / 1024; ++it) load4(g, base + it * 1024 + threadIdx.x * 4, n, wide && base + CHUNK <= n, v[it]);
 #pragma unroll
     for (int it = 0; it < CHUNK / 1024; ++it)
 #pragma unroll
@@ -111,38 +111,40 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(const Table tb, double*
   if (threadIdx.x == 0) partial[blockIdx.x] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
 }
 
-// the norm and the factor that clips it; clip = {factor, skip}
-__global__ __launch_bounds__(256) void grad_clip_kernel(const double* partial, int n, double max_norm, float* norm, float* clip) {
-  __shared__ double sm[4];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) s += partial[i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const double total = sqrt((sm[0] + sm[1]) + (sm[2] + sm[3])), f = max_norm / (total + 1e-6);
-    *norm = (float)total;
-    const bool fine = total <= 1.7976931348623157e308;        // false for NaN too
-    clip[0] = fine ? (float)(f < 1.0 ? f : 1.0) : 0.f;
-    clip[1] = fine ? 0.f : 1.f;
-  }
-}
-
 struct CountArgs {
   int* steps;                      // all counts of the caller's group
   int* now;                        // out: the counts of this launch's tensors
-  Scalars* sc;
-  const float* clip;
+  Scalars* sc;                     // out
+  float* clip;                     // out: {factor, skip}
+  float* norm;                     // out, nullable
+  const double* sumsq;             // partial sums of squares, or null: nothing is clipped
   const float* lr_dev;
-  double lr, b1, b2, decay;
-  int index[MAXT], count;
+  double lr, b1, b2, decay, max_norm;
+  int index[MAXT], count, n_sumsq;
 };
-__global__ __launch_bounds__(128) void adamw_count_kernel(const CountArgs a) {
+// one workgroup in front of each step: the norm and the factor that clips it, the step counts and what hangs on them
+__global__ __launch_bounds__(256) void adamw_count_kernel(const CountArgs a) {
+  __shared__ double sm[4];
+  bool skip = false;
+  if (a.sumsq) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < a.n_sumsq; i += 256) s += a.sumsq[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
+    __syncthreads();
+    const double total = sqrt((sm[0] + sm[1]) + (sm[2] + sm[3])), f = a.max_norm / (total + 1e-6);
+    skip = !(total <= 1.7976931348623157e308);                // infinite or NaN
+    if (threadIdx.x == 0) {
+      if (a.norm) *a.norm = (float)total;
+      a.clip[0] = skip ? 0.f : (float)(f < 1.0 ? f : 1.0);
+      a.clip[1] = skip ? 1.f : 0.f;
+    }
+  }
   const int i = threadIdx.x;
   if (i >= a.count) return;
   int t = a.steps[a.index[i]];
-  if (!(a.clip && a.clip[1] != 0.f)) a.steps[a.index[i]] = ++t;
+  if (!skip) a.steps[a.index[i]] = ++t;
   const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
   a.now[i] = t;
   a.sc[i] = Scalars{(float)(lr / (1.0 - pow(a.b1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(a.b2, (double)t))), (float)(1.0 - lr * a.decay), 0.f};
@@ -157,105 +159,135 @@ __device__ __forceinline__ int block_exponent(unsigned top, int lowest) {
   const int e = (int)((top + 0xFFFFFu) >> 23);
   return e < lowest ? lowest : e > 255 ? 255 : e;
 }
-// code of a magnitude: 3 bits of mantissa; `low` = biased exponent of the smallest value with a whole mantissa
-__device__ __forceinline__ unsigned encode(float t, unsigned coin, int low) {
-  const unsigned b = float_bits(t);
-  if ((int)(b >> 23) >= low) return ((b + coin) >> 20) - ((unsigned)(low - 1) << 3);
-  return (unsigned)(t * __uint_as_float((unsigned)(257 - low) << 23) + (float)coin * 0x1p-20f);
-}
-__device__ __forceinline__ float decode(unsigned c, int low) {
-  return c < 8 ? (float)c * __uint_as_float((unsigned)(low - 3) << 23) : __uint_as_float((c + ((unsigned)(low - 1) << 3)) << 20);
-}
+// What a block's exponent byte says, worked out once per wave.  A block of zeros (0) holds only codes 0; one that was not finite (255) too, and
+// reads as NaN through its unit.
+template <int EXP>
+struct Block {
+  unsigned low;                    // biased exponent of the smallest value with a whole mantissa
+  float unit;                      // the step under it
+  __device__ __forceinline__ explicit Block(int e) {
+    low = (unsigned)max(e, EXP + 2) - (EXP - 2);
+    unit = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((low - 3) << 23);
+  }
+  __device__ __forceinline__ float decode(unsigned c) const {
+    const float small = (float)c * unit, whole = __uint_as_float((c + ((low - 1) << 3)) << 20);
+    return c < 8 ? small : whole;
+  }
+  // (the product with a power of two is exact: one rounding, as if it stood alone)
+  __device__ __forceinline__ unsigned encode(float t, unsigned coin) const {
+    const unsigned b = float_bits(t), whole = ((b + coin) >> 20) - ((low - 1) << 3);
+    const unsigned small = (unsigned)__builtin_fmaf(t, __uint_as_float((257 - low) << 23), (float)coin * 0x1p-20f);
+    return b >= low << 23 ? whole : small;
+  }
+};
 constexpr int M_EXP = 16, V_EXP = 32;
-// `e`: a block's exponent byte
-__device__ __forceinline__ float decode_m(unsigned c, int e) {
-  if (e == 255) return __uint_as_float(0x7fc00000u);
-  if (e == 0) return 0.f;
-  const float a = decode(c & 127u, e - (M_EXP - 2));
-  return c & 128u ? -a : a;
+__device__ __forceinline__ float decode_m(unsigned c, const Block<M_EXP>& k) { return __uint_as_float(float_bits(k.decode(c & 127u)) | (c & 128u) << 24); }
+
+// largest value of the wave's lanes, as a scalar: rows of 16 by shifts, then row to row
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#define ASYRP_DPP(CTRL, ROWS) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false))
+  ASYRP_DPP(0x111, 0xf);
+  ASYRP_DPP(0x112, 0xf);
+  ASYRP_DPP(0x114, 0xf);
+  ASYRP_DPP(0x118, 0xf);
+  ASYRP_DPP(0x142, 0xa);
+  ASYRP_DPP(0x143, 0xc);
+#undef ASYRP_DPP
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ float decode_v(unsigned c, int e) {
-  if (e == 255) return __uint_as_float(0x7fc00000u);
-  return e == 0 ? 0.f : decode(c, e - (V_EXP - 2));
+
+// One wave's 256 values from `i0` of a tensor on.  WHOLE: all of them are there and may be loaded four at a time.
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ void step_block(T* p, const T* g, long long n, long long off, long long i0, int lane, const StepArgs& a, const Scalars& sc, float clip,
+                                           unsigned key) {
+  const long long i = i0 + lane * 4, si = off + i;
+  float pv[4], gv[4], m[4], v[4];
+  load4(p, i, n, WHOLE, pv);
+  load4(g, i, n, WHOLE, gv);
+  if (BITS == 32) {
+    const float4 mv = *reinterpret_cast<const float4*>(a.m + si), vv = *reinterpret_cast<const float4*>(a.v + si);
+    m[0] = mv.x; m[1] = mv.y; m[2] = mv.z; m[3] = mv.w;
+    v[0] = vv.x; v[1] = vv.y; v[2] = vv.z; v[3] = vv.w;
+  } else {
+    const unsigned mc = *reinterpret_cast<const unsigned*>(a.m8 + si), vc = *reinterpret_cast<const unsigned*>(a.v8 + si);
+    const Block<M_EXP> mb(__builtin_amdgcn_readfirstlane(a.me[(off + i0) >> 8]));
+    const Block<V_EXP> vb(__builtin_amdgcn_readfirstlane(a.ve[(off + i0) >> 8]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = decode_m((mc >> (8 * j)) & 255u, mb);
+      v[j] = vb.decode((vc >> (8 * j)) & 255u);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float gg = gv[j] * clip;
+    m[j] = m[j] * a.b1 + gg * a.nb1;
+    v[j] = v[j] * a.b2 + (gg * gg) * a.nb2;
+    pv[j] = pv[j] * sc.keep;
+    // with 8-bit moments the kernel is as near to its arithmetic as to HBM, and the quotient is taken from the hardware's square root and
+    // reciprocal (one unit in the last place each, of a quotient whose moments are 6 to 12 % wide)
+    if (BITS == 32) pv[j] = pv[j] - (m[j] / (sqrtf(v[j]) * sc.inv_sqrt_bc2 + a.eps)) * sc.step_size;
+    else pv[j] = pv[j] - (m[j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[j]) * sc.inv_sqrt_bc2 + a.eps)) * sc.step_size;
+  }
+  store4(p, i, n, WHOLE, pv);
+  if (BITS == 32) {
+    *reinterpret_cast<float4*>(a.m + si) = make_float4(m[0], m[1], m[2], m[3]);
+    *reinterpret_cast<float4*>(a.v + si) = make_float4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+  unsigned tm = 0, tv = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (!WHOLE && i + j >= n) m[j] = v[j] = 0.f;
+    tm = max(tm, float_bits(m[j]) & 0x7fffffffu);
+    tv = max(tv, float_bits(v[j]) & 0x7fffffffu);
+  }
+  const int me = block_exponent(wave_max(tm), M_EXP + 2), ve = block_exponent(wave_max(tv), V_EXP + 2);
+  const Block<M_EXP> mb(me);
+  const Block<V_EXP> vb(ve);
+  const bool some_m = me != 0 && me != 255, some_v = ve != 0 && ve != 255;
+  const unsigned at = (unsigned)si, k = key ^ ((unsigned)((off + i0) >> 32) * 0xC2B2AE3Du);
+  unsigned mc = 0, vc = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unsigned x = (at + j) ^ k;                       // `at` is a multiple of four: no carry
+    x = (x ^ (x >> 16)) * 0x7FEB352Du;
+    x = (x ^ (x >> 15)) * 0x846CA68Bu;
+    x ^= x >> 16;
+    const unsigned cm = mb.encode(fabsf(m[j]), x & 0xFFFFFu) | (float_bits(m[j]) >> 24 & 128u);
+    unsigned cv = max(vb.encode(v[j], (x * 0x9E3779B1u) >> 12), 1u);
+    if (!WHOLE && i + j >= n) cv = 0;
+    mc |= cm << (8 * j);
+    vc |= cv << (8 * j);
+  }
+  *reinterpret_cast<unsigned*>(a.m8 + si) = some_m ? mc : 0u;
+  *reinterpret_cast<unsigned*>(a.v8 + si) = some_v ? vc : 0u;
+  if (lane == 0) {
+    a.me[(off + i0) >> 8] = (unsigned char)me;
+    a.ve[(off + i0) >> 8] = (unsigned char)ve;
+  }
 }
 
 template <typename T, int BITS>
 __global__ __launch_bounds__(256) void adamw_step_kernel(const Table tb, const StepArgs a) {
   if (a.clip && a.clip[1] != 0.f) return;                     // the norm is not finite: nothing changes
-  const int k = tensor_of(tb, blockIdx.x);
+  const int chunk = tb.chunks - 1 - blockIdx.x;               // from the end: what the norm's pass read last is still in the caches
+  const int k = tensor_of(tb, chunk);
   const float clip = a.clip ? a.clip[0] : 1.f;
   const Scalars sc = a.sc[k];
   T* p = (T*)tb.t[k].p;
   const T* g = (const T*)tb.t[k].g;
-  const long long n = tb.t[k].n, off = tb.t[k].off, base = (long long)(blockIdx.x - tb.first[k]) * CHUNK;
+  const long long n = tb.t[k].n, off = tb.t[k].off;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long base = (long long)(chunk - tb.first[k]) * CHUNK + wave * 256;
   const bool wide = (((uintptr_t)p | (uintptr_t)g) & (4 * sizeof(T) - 1)) == 0;
   const unsigned key = (a.seed * 0x9E3779B1u) ^ ((unsigned)(BITS == 8 ? a.steps[k] : 0) * 0x85EBCA77u);
+  if (wide && base + (CHUNK - 1024) + 256 <= n) {
 #pragma unroll
-  for (int it = 0; it < CHUNK / 1024; ++it) {
-    const long long i = base + it * 1024 + threadIdx.x * 4;
-    if (base + it * 1024 + (threadIdx.x & ~63) * 4 >= n) break;       // the wave's whole block lies behind the end
-    const long long si = off + i;
-    float pv[4], gv[4], m[4], v[4];
-    load4(p, i, n, wide, pv);
-    load4(g, i, n, wide, gv);
-    if (BITS == 32) {
-      const float4 mv = *reinterpret_cast<const float4*>(a.m + si), vv = *reinterpret_cast<const float4*>(a.v + si);
-      m[0] = mv.x; m[1] = mv.y; m[2] = mv.z; m[3] = mv.w;
-      v[0] = vv.x; v[1] = vv.y; v[2] = vv.z; v[3] = vv.w;
-    } else {
-      const unsigned mc = *reinterpret_cast<const unsigned*>(a.m8 + si), vc = *reinterpret_cast<const unsigned*>(a.v8 + si);
-      const int me = a.me[si >> 8], ve = a.ve[si >> 8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = decode_m((mc >> (8 * j)) & 255u, me);
-        v[j] = decode_v((vc >> (8 * j)) & 255u, ve);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float gg = a.clip ? gv[j] * clip : gv[j];
-      m[j] = m[j] * a.b1 + gg * a.nb1;
-      v[j] = v[j] * a.b2 + (gg * gg) * a.nb2;
-      pv[j] = pv[j] * sc.keep;
-      pv[j] = pv[j] - (m[j] / (sqrtf(v[j]) * sc.inv_sqrt_bc2 + a.eps)) * sc.step_size;
-    }
-    store4(p, i, n, wide, pv);
-    if (BITS == 32) {
-      *reinterpret_cast<float4*>(a.m + si) = make_float4(m[0], m[1], m[2], m[3]);
-      *reinterpret_cast<float4*>(a.v + si) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      unsigned tm = 0, tv = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i + j >= n) m[j] = v[j] = 0.f;
-        tm = max(tm, float_bits(m[j]) & 0x7fffffffu);
-        tv = max(tv, float_bits(v[j]) & 0x7fffffffu);
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        tm = max(tm, (unsigned)__shfl_xor((int)tm, o));
-        tv = max(tv, (unsigned)__shfl_xor((int)tv, o));
-      }
-      const int me = block_exponent(tm, M_EXP + 2), ve = block_exponent(tv, V_EXP + 2);
-      const int ml = me - (M_EXP - 2), vl = ve - (V_EXP - 2);
-      unsigned mc = 0, vc = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned long long at = (unsigned long long)(si + j);
-        unsigned x = (unsigned)at ^ (key ^ ((unsigned)(at >> 32) * 0xC2B2AE3Du));
-        x = (x ^ (x >> 16)) * 0x7FEB352Du;
-        x = (x ^ (x >> 15)) * 0x846CA68Bu;
-        x ^= x >> 16;
-        if (me != 0 && me != 255) mc |= (encode(fabsf(m[j]), x & 0xFFFFFu, ml) | (m[j] < 0.f ? 128u : 0u)) << (8 * j);
-        if (ve != 0 && ve != 255 && i + j < n) vc |= max(encode(v[j], (x * 0x9E3779B1u) >> 12, vl), 1u) << (8 * j);
-      }
-      *reinterpret_cast<unsigned*>(a.m8 + si) = mc;
-      *reinterpret_cast<unsigned*>(a.v8 + si) = vc;
-      if ((threadIdx.x & 63) == 0) {
-        a.me[si >> 8] = (unsigned char)me;
-        a.ve[si >> 8] = (unsigned char)ve;
-      }
-    }
+    for (int it = 0; it < CHUNK / 1024; ++it) step_block<T, BITS, true>(p, g, n, off, base + it * 1024, lane, a, sc, clip, key);
+  } else {
+#pragma unroll 1
+    for (long long i0 = base; i0 < base + CHUNK && i0 < n; i0 += 1024) step_block<T, BITS, false>(p, g, n, off, i0, lane, a, sc, clip, key);
   }
 }
 
@@ -264,10 +296,11 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const unsigned char*
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
   const unsigned mc = *reinterpret_cast<const unsigned*>(m8 + i), vc = *reinterpret_cast<const unsigned*>(v8 + i);
-  const int a = me[i >> 8], b = ve[i >> 8];
+  const Block<M_EXP> a(me[i >> 8]);
+  const Block<V_EXP> b(ve[i >> 8]);
   float4 mo, vo;
   mo.x = decode_m(mc & 255u, a); mo.y = decode_m((mc >> 8) & 255u, a); mo.z = decode_m((mc >> 16) & 255u, a); mo.w = decode_m(mc >> 24, a);
-  vo.x = decode_v(vc & 255u, b); vo.y = decode_v((vc >> 8) & 255u, b); vo.z = decode_v((vc >> 16) & 255u, b); vo.w = decode_v(vc >> 24, b);
+  vo.x = b.decode(vc & 255u); vo.y = b.decode((vc >> 8) & 255u); vo.z = b.decode((vc >> 16) & 255u); vo.w = b.decode(vc >> 24);
   *reinterpret_cast<float4*>(m + i) = mo;
   *reinterpret_cast<float4*>(v + i) = vo;
 }
@@ -329,15 +362,6 @@ int asyrp_grad_sumsq(int device, const asyrp_adamw_tensor* tensors, int n, int d
   return 0;
 }
 
-int asyrp_grad_clip(int device, const double* partial, int n_partial, double max_norm, float* norm, float* clip, void* stream) {
-  if (!partial || !norm || !clip || n_partial < 0) return refuse("AdamW: null argument");
-  if (!(max_norm > 0) || !std::isfinite(max_norm)) return refuse("AdamW: max_norm must be positive and finite");
-  DeviceGuard dg(device);
-  if (dg.error != hipSuccess) return failed(dg.error);
-  hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, partial, n_partial, max_norm, norm, clip);
-  return failed(hipGetLastError());
-}
-
 int asyrp_adamw_step(int device, const asyrp_adamw* c, const asyrp_adamw_tensor* tensors, int n, int dtype, void* scratch, void* stream) {
   if (int rc = check(tensors, n, dtype)) return rc;
   if (!c || (n > 0 && (!scratch || !c->steps))) return refuse("AdamW: null argument");
@@ -348,26 +372,30 @@ int asyrp_adamw_step(int device, const asyrp_adamw* c, const asyrp_adamw_tensor*
     return refuse("AdamW: betas must lie in [0, 1), eps, lr and weight decay must be finite");
   for (int i = 0; i < n; ++i)
     if ((tensors[i].numel > 0 && !tensors[i].param) || tensors[i].index < 0 || tensors[i].index > 0x7fffffffLL) return refuse("AdamW: null tensor or bad index");
+  if (c->sumsq && (c->sumsq_count < 0 || !(c->max_norm > 0) || !std::isfinite(c->max_norm))) return refuse("AdamW: max_norm must be positive and finite");
   DeviceGuard dg(device);
   if (dg.error != hipSuccess) return failed(dg.error);
   hipStream_t s = (hipStream_t)stream;
   Table tb;
+  float* clip = c->sumsq ? (float*)scratch : nullptr;
+  Scalars* scalars = (Scalars*)scratch + 1;
   for (int from = 0; from < n;) {
     const int took = table(tensors, n, from, tb);
     CountArgs ca;
     ca.steps = c->steps;
-    ca.sc = reinterpret_cast<Scalars*>(scratch) + from;
-    ca.now = reinterpret_cast<int*>(reinterpret_cast<Scalars*>(scratch) + n) + from;
-    ca.clip = c->clip; ca.lr_dev = c->lr_device; ca.lr = c->lr; ca.b1 = c->beta1; ca.b2 = c->beta2; ca.decay = c->weight_decay;
+    ca.sc = scalars + from;
+    ca.now = reinterpret_cast<int*>(scalars + n) + from;
+    ca.clip = clip; ca.norm = c->grad_norm; ca.sumsq = c->sumsq; ca.n_sumsq = c->sumsq_count; ca.max_norm = c->max_norm;
+    ca.lr_dev = c->lr_device; ca.lr = c->lr; ca.b1 = c->beta1; ca.b2 = c->beta2; ca.decay = c->weight_decay;
     ca.count = tb.count;
     for (int i = 0; i < tb.count; ++i) ca.index[i] = (int)tensors[from + i].index;
-    hipLaunchKernelGGL(adamw_count_kernel, dim3(1), dim3(128), 0, s, ca);
+    hipLaunchKernelGGL(adamw_count_kernel, dim3(1), dim3(256), 0, s, ca);
     if (hipError_t e = hipGetLastError()) return failed(e);
     if (tb.chunks > 0) {
       StepArgs a{};
       a.m = (float*)c->exp_avg; a.v = (float*)c->exp_avg_sq; a.m8 = (unsigned char*)c->exp_avg; a.v8 = (unsigned char*)c->exp_avg_sq;
       a.me = c->exp_avg_scale; a.ve = c->exp_avg_sq_scale;
-      a.sc = ca.sc; a.steps = ca.now; a.clip = c->clip; a.seed = c->seed;
+      a.sc = ca.sc; a.steps = ca.now; a.clip = clip; a.seed = c->seed;
       a.b1 = (float)c->beta1; a.nb1 = (float)(1 - c->beta1); a.b2 = (float)c->beta2; a.nb2 = (float)(1 - c->beta2);
       a.eps = (float)c->eps;
       const dim3 g(tb.chunks), b(256);

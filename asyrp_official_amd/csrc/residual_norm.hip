@@ -27,7 +27,7 @@ struct NormArgs {
   float *stats;              // [rows][4]: mean and rstd of y, mean and rstd of h (null: not kept)
   float *partial;            // [slots][vectors][C]
   float *dgate;
-  float a, eps;
+  float a, eps, inv_c;
   long long rows, per_gate;  // rows of one gate row
   int C, after, before, rms; // which norms there are
   int chunks;                // workgroups per gate row (1 where a workgroup takes whole gate rows)
@@ -58,6 +58,15 @@ __device__ __forceinline__ void load(const T* row, int t, int C, Raw<T, VPT>& o)
     for (int j = 0; j < VPT; ++j) o.v[j] = j * TPR + t < C ? row[j * TPR + t] : (T)0.f;
   }
 }
+// The values are there behind this.  It stands before the current row's stores: loads and stores are counted together, and a wait behind
+// stores that may or may not have been issued would wait for them too.
+template <typename T, int VPT>
+__device__ __forceinline__ void landed(Raw<T, VPT>& r) {
+  typedef unsigned U __attribute__((ext_vector_type(sizeof(T) * VPT / 4)));
+  U u = __builtin_bit_cast(U, r.v);
+  asm volatile("" : "+v"(u));
+  r.v = __builtin_bit_cast(typename Raw<T, VPT>::V, u);
+}
 template <typename T, int VPT>
 __device__ __forceinline__ void floats(const Raw<T, VPT>& r, float (&o)[VPT]) {
 #pragma unroll
@@ -85,14 +94,24 @@ __device__ __forceinline__ void store(T* row, int t, int C, const float (&o)[VPT
 template <bool VEC, int TPR, int VPT>
 __device__ __forceinline__ bool inside(int t, int j, int C) { return VEC ? t * VPT < C : j * TPR + t < C; }
 
+// a wave's sum, in all lanes: within rows of 16 by shifts, then from row to row
+__device__ __forceinline__ float wave_sum(float v) {
+#define ASYRP_DPP(CTRL, ROWS) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false))
+  ASYRP_DPP(0x111, 0xf);
+  ASYRP_DPP(0x112, 0xf);
+  ASYRP_DPP(0x114, 0xf);
+  ASYRP_DPP(0x118, 0xf);
+  ASYRP_DPP(0x142, 0xa);
+  ASYRP_DPP(0x143, 0xc);
+#undef ASYRP_DPP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 // sums of K values over the TPR threads of a row.  `buf` holds two sets of one row of K values per wave, used in turn, so that
 // one barrier per reduction is enough.
 template <int TPR, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float* buf, int& turn, int sub, int t) {
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o);
+  for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
   if (TPR > 64) {
     constexpr int W = TPR / 64;
     float* b = buf + (turn * 16 + sub * W) * 2;
@@ -111,7 +130,8 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* buf, int& turn, in
   }
 }
 
-// mean and rstd of the values (those behind C are zero and do not count)
+// mean and rstd of the values (those behind C are zero and do not count).  The reciprocal root is the hardware's (one unit in the last place), except for
+// values near the smallest ones, which eps = 0 alone leaves.
 template <bool VEC, int TPR, int VPT>
 __device__ __forceinline__ void statistics(const float (&v)[VPT], const NormArgs& p, float* buf, int& turn, int sub, int t, float& mean, float& rstd) {
   mean = 0.f;
@@ -120,16 +140,33 @@ __device__ __forceinline__ void statistics(const float (&v)[VPT], const NormArgs
 #pragma unroll
     for (int j = 0; j < VPT; ++j) s[0] += v[j];
     row_sum<TPR, 1>(s, buf, turn, sub, t);
-    mean = s[0] / (float)p.C;
+    mean = s[0] * p.inv_c;
   }
   s[0] = 0.f;
 #pragma unroll
-  for (int j = 0; j < VPT; ++j)
-    if (inside<VEC, TPR, VPT>(t, j, p.C)) s[0] += (v[j] - mean) * (v[j] - mean);
+  for (int j = 0; j < VPT; ++j) {
+    const float d = inside<VEC, TPR, VPT>(t, j, p.C) ? v[j] - mean : 0.f;
+    s[0] = __builtin_fmaf(d, d, s[0]);
+  }
   row_sum<TPR, 1>(s, buf, turn, sub, t);
-  rstd = 1.0f / sqrtf(s[0] / (float)p.C + p.eps);
+  const float var = __builtin_fmaf(s[0], p.inv_c, p.eps);
+  rstd = var > 1e-30f ? __builtin_amdgcn_rsqf(var) : 1.0f / sqrtf(var);
 }
 
+// a vector of the columns, or `fill` where there is none (zero behind C)
+template <bool VEC, int TPR, int VPT>
+__device__ __forceinline__ void columns(const float* row, float fill, int t, int C, float (&o)[VPT]) {
+  if (row) {
+    loadf<VEC, TPR, VPT>(row, t, C, o);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) o[j] = inside<VEC, TPR, VPT>(t, j, C) ? fill : 0.f;
+  }
+}
+
+// Weights, biases and gates that are not given are ones and zeros in registers, so that the arithmetic has no cases; behind C they are zeros, and with them
+// whatever a sum over the row would take from there.
+//
 // Both directions: a workgroup of max(256, TPR) threads, TPR to a row, walks over the rows of one part of a gate row, or of several whole
 // gate rows, with the weights (and, backward, the parameter gradients) of its columns in registers.  The next row's loads are issued before
 // the current one is worked on, so that the reductions' barriers stand in the shadow of memory.
@@ -142,18 +179,18 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
   int turn = 0;
   float w1[VPT], w2[VPT], b1[VPT], b2[VPT];
-  if (p.w1) loadf<VEC, TPR, VPT>(p.w1, t, C, w1);
-  if (p.b1) loadf<VEC, TPR, VPT>(p.b1, t, C, b1);
-  if (p.w2) loadf<VEC, TPR, VPT>(p.w2, t, C, w2);
-  if (p.b2) loadf<VEC, TPR, VPT>(p.b2, t, C, b2);
+  columns<VEC, TPR, VPT>(p.w1, 1.f, t, C, w1);
+  columns<VEC, TPR, VPT>(p.b1, 0.f, t, C, b1);
+  columns<VEC, TPR, VPT>(p.w2, 1.f, t, C, w2);
+  columns<VEC, TPR, VPT>(p.b2, 0.f, t, C, b2);
   const long long g0 = (long long)(blockIdx.x / p.chunks) * p.gates_per_wg, g1 = min(p.gates, g0 + p.gates_per_wg);
   const int part = blockIdx.x % p.chunks;
   for (long long g = g0; g < g1; ++g) {
     const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
     float gate[VPT];
-    if (p.gate) loadf<VEC, TPR, VPT>(p.gate + g * C, t, C, gate);
-    Raw<X, VPT> xn;
-    Raw<Y, VPT> yn;
+    columns<VEC, TPR, VPT>(p.gate ? p.gate + g * C : nullptr, 1.f, t, C, gate);
+    Raw<X, VPT> xn{};
+    Raw<Y, VPT> yn{};
     auto fetch = [&](long long r) {
       const long long row = min(r + sub, last - 1);
       load<Y, VEC, TPR, VPT>((const Y*)p.y + row * C, t, C, yn);
@@ -171,28 +208,19 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const
       if (p.after) {
         statistics<VEC, TPR, VPT>(y, p, buf, turn, sub, t, m1, r1);
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-          y[j] = (y[j] - m1) * r1;
-          if (p.w1) y[j] *= w1[j];
-          if (p.b1) y[j] += b1[j];
-        }
+        for (int j = 0; j < VPT; ++j) y[j] = __builtin_fmaf((y[j] - m1) * r1, w1[j], b1[j]);
       }
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        if (p.gate) y[j] *= gate[j];
-        x[j] = inside<VEC, TPR, VPT>(t, j, C) ? p.a * x[j] + y[j] : 0.f;
-      }
-      if (there) store<X, VEC, TPR, VPT>((X*)p.h + row * C, t, C, x);
+      for (int j = 0; j < VPT; ++j) x[j] = __builtin_fmaf(y[j], gate[j], p.a * x[j]);
       if (p.before) {
         statistics<VEC, TPR, VPT>(x, p, buf, turn, sub, t, m2, r2);
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-          x[j] = (x[j] - m2) * r2;
-          if (p.w2) x[j] *= w2[j];
-          if (p.b2) x[j] += b2[j];
-        }
-        if (there) store<Y, VEC, TPR, VPT>((Y*)p.n + row * C, t, C, x);
+        for (int j = 0; j < VPT; ++j) y[j] = __builtin_fmaf((x[j] - m2) * r2, w2[j], b2[j]);
       }
+      landed(xn);
+      landed(yn);
+      if (there) store<X, VEC, TPR, VPT>((X*)p.h + row * C, t, C, x);
+      if (there && p.before) store<Y, VEC, TPR, VPT>((Y*)p.n + row * C, t, C, y);
       if (p.stats && there && t == 0) reinterpret_cast<float4*>(p.stats)[row] = make_float4(m1, r1, m2, r2);
     }
   }
@@ -206,9 +234,9 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
   int turn = 0;
   float w1[VPT], w2[VPT], b1[VPT];
-  if (p.w1) loadf<VEC, TPR, VPT>(p.w1, t, C, w1);
-  if (p.b1) loadf<VEC, TPR, VPT>(p.b1, t, C, b1);
-  if (p.w2) loadf<VEC, TPR, VPT>(p.w2, t, C, w2);
+  columns<VEC, TPR, VPT>(p.w1, 1.f, t, C, w1);
+  columns<VEC, TPR, VPT>(p.b1, 0.f, t, C, b1);
+  columns<VEC, TPR, VPT>(p.w2, 1.f, t, C, w2);
   float sw1[VPT], sb1[VPT], sw2[VPT], sb2[VPT], sg[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) sw1[j] = sb1[j] = sw2[j] = sb2[j] = 0.f;
@@ -234,11 +262,11 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
   for (long long g = g0; g < g1; ++g) {
     const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
     float gate[VPT];
-    if (p.gate) loadf<VEC, TPR, VPT>(p.gate + g * C, t, C, gate);
+    columns<VEC, TPR, VPT>(p.gate ? p.gate + g * C : nullptr, 1.f, t, C, gate);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) sg[j] = 0.f;
-    Raw<X, VPT> xn, dhn;
-    Raw<Y, VPT> yn, dnn;
+    Raw<X, VPT> xn{}, dhn{};
+    Raw<Y, VPT> yn{}, dnn{};
     float4 stn;
     auto fetch = [&](long long r) {
       const long long row = min(r + sub, last - 1);
@@ -261,59 +289,62 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
       if (r0 + SUB < last) fetch(r0 + SUB);
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
-        if (!p.dh) dh[j] = 0.f;
-        y[j] = p.after ? (y[j] - st.x) * st.y : y[j];
-        u[j] = y[j];
-        if (p.after && p.w1) u[j] *= w1[j];
-        if (p.after && p.b1) u[j] += b1[j];
+        y[j] = (y[j] - st.x) * st.y;                          // without the norm behind the block: mean 0, rstd 1
+        u[j] = __builtin_fmaf(y[j], w1[j], b1[j]);
       }
+      // `keep`: false only for the copies of the last row that fill up a set of rows
+      const bool keep = SUB == 1 || there;
       if (p.before && p.dn) {
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-          const float hat = (p.a * x[j] + (p.gate ? u[j] * gate[j] : u[j]) - st.z) * st.w;
-          x[j] = inside<VEC, TPR, VPT>(t, j, C) ? hat : 0.f;
-          if (there) {
-            sw2[j] += dn[j] * x[j];
-            sb2[j] += dn[j];
-          }
-          if (p.w2) dn[j] *= w2[j];
-          s[0] += dn[j];
-          s[1] += dn[j] * x[j];
+          x[j] = (__builtin_fmaf(u[j], gate[j], p.a * x[j]) - st.z) * st.w;
+          if (keep) sw2[j] = __builtin_fmaf(dn[j], x[j], sw2[j]);
         }
-        row_sum<TPR, 2>(s, buf, turn, sub, t);
-        const float c1 = p.rms ? 0.f : s[0] / (float)C, c2 = s[1] / (float)C;
+        if (p.want_b2 && keep)
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) dh[j] += st.w * (dn[j] - c1 - x[j] * c2);
-      }
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) x[j] = p.a * dh[j];
-      if (there && p.dx) store<X, VEC, TPR, VPT>((X*)p.dx + row * C, t, C, x);
-      if (p.gate) {
+          for (int j = 0; j < VPT; ++j) sb2[j] += dn[j];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-          if (there) sg[j] += dh[j] * u[j];
-          dh[j] *= gate[j];
+          dn[j] *= w2[j];
+          s[0] += dn[j];
+          s[1] = __builtin_fmaf(dn[j], x[j], s[1]);
         }
+        row_sum<TPR, 2>(s, buf, turn, sub, t);
+        const float c1 = p.rms ? 0.f : s[0] * p.inv_c, c2 = s[1] * p.inv_c;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) dh[j] = __builtin_fmaf(st.w, __builtin_fmaf(-x[j], c2, dn[j] - c1), dh[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        x[j] = p.a * dh[j];                                   // dx
+        if (keep) sg[j] = __builtin_fmaf(dh[j], u[j], sg[j]);
+        dh[j] *= gate[j];
       }
       if (p.after) {
         float s[2] = {0.f, 0.f};
+        if (keep)
+#pragma unroll
+          for (int j = 0; j < VPT; ++j) sw1[j] = __builtin_fmaf(dh[j], y[j], sw1[j]);
+        if (p.want_b1 && keep)
+#pragma unroll
+          for (int j = 0; j < VPT; ++j) sb1[j] += dh[j];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-          if (!inside<VEC, TPR, VPT>(t, j, C)) y[j] = dh[j] = 0.f;
-          if (there) {
-            sw1[j] += dh[j] * y[j];
-            sb1[j] += dh[j];
-          }
-          if (p.w1) dh[j] *= w1[j];
+          dh[j] *= w1[j];
           s[0] += dh[j];
-          s[1] += dh[j] * y[j];
+          s[1] = __builtin_fmaf(dh[j], y[j], s[1]);
         }
         row_sum<TPR, 2>(s, buf, turn, sub, t);
-        const float c1 = p.rms ? 0.f : s[0] / (float)C, c2 = s[1] / (float)C;
+        const float c1 = p.rms ? 0.f : s[0] * p.inv_c, c2 = s[1] * p.inv_c;
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) dh[j] = st.y * (dh[j] - c1 - y[j] * c2);
+        for (int j = 0; j < VPT; ++j) dh[j] = st.y * __builtin_fmaf(-y[j], c2, dh[j] - c1);
       }
+      landed(xn);
+      landed(yn);
+      landed(dhn);
+      landed(dnn);
+      if (there && p.dx) store<X, VEC, TPR, VPT>((X*)p.dx + row * C, t, C, x);
       if (there && p.dy) store<Y, VEC, TPR, VPT>((Y*)p.dy + row * C, t, C, dh);
     }
     if (p.want_gate) put(sg, p.chunks == 1 ? p.dgate + g * C : slot + V_GATE * C);
@@ -427,6 +458,7 @@ void fill(const asyrp_residual_norm* p, NormArgs& a) {
   a.before = p->before != 0;
   a.a = p->residual_scale;
   a.eps = p->eps;
+  a.inv_c = 1.0f / (float)p->width;
   a.per_gate = p->gates > 0 ? std::max<long long>(1, p->rows / p->gates) : std::max<long long>(1, p->rows);
 }
 bool aligned(std::initializer_list<const void*> ps) {
@@ -453,7 +485,7 @@ int asyrp_residual_norm_forward(int device, const asyrp_residual_norm* p, const 
   if (!aligned({stats})) return refuse("residual norm: the statistics must be 16-byte aligned");
   const bool vec = a.C % 8 == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, before_bias, h, n});
   unsigned wgs = 0;
-  deal(p, a, std::min<long long>(2048, a.rows), wgs);
+  deal(p, a, std::min<long long>(4096, a.rows), wgs);
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
   const hipError_t e = dispatch(p->stream_dtype, p->branch_dtype, a, vec, false, wgs, (hipStream_t)stream);

@@ -4,12 +4,15 @@ The reference steps its DeltaBlock with a torch optimiser (diffusion_latent.py:2
     opt = AdamW(model.layer_0.parameters(), lr=1e-4, state_bits=8, max_norm=1.0)
     opt.zero_grad(); loss.backward(); opt.step()
 """
-import ctypes as C
+import operator
+import struct
 
 import torch
 
 from . import _lib
-from .engine import AsyrpDeviceError, _ptr
+from .engine import AsyrpDeviceError
+
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle (torch.cuda.current_stream() without its object)
 
 BLOCK = 256          # values that share one exponent of the 8-bit moments; every parameter's moments start on a multiple of it
 
@@ -99,19 +102,21 @@ class AdamW(torch.optim.Optimizer):
 
     # ---- moments ---------------------------------------------------------------------------------------
     def _device(self):
-        dev = None
+        index = None
         for g in self.param_groups:
             for p in g["params"]:
-                if not p.is_cuda:
-                    raise AsyrpDeviceError("AdamW steps only parameters on an MI355X (device type 'cuda' under ROCm): there is no CPU path")
-                if dev is not None and p.device != dev:
-                    raise AsyrpDeviceError(f"parameters on {dev} and {p.device}: one optimiser steps one device")
-                dev = p.device
-        return dev
+                d = p.get_device()                         # -1 on the CPU
+                if d != index:
+                    if d < 0:
+                        raise AsyrpDeviceError("AdamW steps only parameters on an MI355X (device type 'cuda' under ROCm): there is no CPU path")
+                    if index is not None:
+                        raise AsyrpDeviceError(f"parameters on cuda:{index} and cuda:{d}: one optimiser steps one device")
+                    index = d
+        return None if index is None else torch.device("cuda", index)
 
     def _group_moments(self, k, device):
         g, mo = self.param_groups[k], self._moments.get(k)
-        if mo is not None and mo.device == device and len(mo.params) == len(g["params"]) and all(a is b for a, b in zip(mo.params, g["params"])):
+        if mo is not None and mo.device == device and len(mo.params) == len(g["params"]) and all(map(operator.is_, mo.params, g["params"])):
             return mo
         for p in g["params"]:
             if not p.is_contiguous():
@@ -145,7 +150,8 @@ class AdamW(torch.optim.Optimizer):
                 out.append((mo.m, mo.v))
                 continue
             m, v = (torch.empty(mo.n, device=device, dtype=torch.float32) for _ in range(2))
-            _lib.check(_lib.load().asyrp_adamw_moments(device.index, _ptr(mo.m), _ptr(mo.v), _ptr(mo.me), _ptr(mo.ve), mo.n, _ptr(m), _ptr(v), self._stream(device)))
+            _lib.check(_lib.load().asyrp_adamw_moments(device.index, *(t.data_ptr() for t in (mo.m, mo.v, mo.me, mo.ve)), mo.n, m.data_ptr(), v.data_ptr(),
+                                                       _raw_stream(device.index)))
             out.append((m, v))
         return out
 
@@ -170,10 +176,6 @@ class AdamW(torch.optim.Optimizer):
                 self.state[p] = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in saved[i].items()}
 
     # ---- the step --------------------------------------------------------------------------------------
-    @staticmethod
-    def _stream(device):
-        return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -183,48 +185,47 @@ class AdamW(torch.optim.Optimizer):
         device = self._device()
         if device is None:
             return loss
-        lib, stream, todo = _lib.load(), self._stream(device), []
+        lib, stream, todo = _lib.load(), _raw_stream(device.index), []
         held = []                                          # copies of gradients laid out otherwise live until the launches are queued
         for k, g in enumerate(self.param_groups):
-            mo = self._group_moments(k, device)
-            by_type = {}
-            for i, p in enumerate(mo.params):
+            mo, by_type = self._group_moments(k, device), {}
+            for p, n, at, i in zip(mo.params, mo.numels, mo.offsets, range(len(mo.params))):
                 grad = p.grad
                 if grad is None:
                     continue
-                if grad.is_sparse or grad.dtype != p.dtype or grad.device != device or grad.shape != p.shape:
-                    raise ValueError(f"the gradient of a {p.dtype} parameter {tuple(p.shape)} must be dense, of its type, shape and device")
-                if not p.is_contiguous():
-                    raise ValueError("parameters must be contiguous")
+                if grad.dtype != p.dtype or grad.layout != torch.strided or grad.numel() != n or grad.get_device() != device.index:
+                    raise ValueError(f"the gradient of a {p.dtype} parameter {tuple(p.shape)} must be dense, of its type, size and device")
+                if p.numel() != n or not p.is_contiguous():
+                    raise ValueError("parameters must be contiguous and keep their size")
                 if not grad.is_contiguous():
                     grad = grad.contiguous()
                     held.append(grad)
-                by_type.setdefault(p.dtype, []).append((p, grad, mo.numels[i], mo.offsets[i], i))
-            for dtype, rows in by_type.items():
-                flat = [v for p, grad, n, at, i in rows for v in (p.data_ptr(), grad.data_ptr(), n, at, i)]
-                todo.append((g, mo, _lib.DTYPES[dtype], len(rows), (C.c_int64 * len(flat))(*flat), [r[0] for r in rows]))
+                flat, params = by_type.setdefault(p.dtype, ([], []))
+                flat += (p.data_ptr(), grad.data_ptr(), n, at, i)
+                params.append(p)
+            todo += [(g, mo, _lib.DTYPES[dtype], len(params), struct.pack(f"{len(flat)}q", *flat), params) for dtype, (flat, params) in by_type.items()]
         if not todo:
             return loss
-        clip = None
+        sumsq, clip = None, (0, 0.0, 0, 0)
         if self.max_norm is not None:
             counts = [-(-n // _lib.ADAMW_TABLE) * _lib.ADAMW_PARTIALS for _, _, _, n, _, _ in todo]
-            partial = torch.empty(sum(counts), device=device, dtype=torch.float64)
-            at = 0
+            sumsq = torch.empty(sum(counts), device=device, dtype=torch.float64)
+            if self.grad_norm is None or self.grad_norm.device != device:
+                self.grad_norm = torch.zeros((), device=device, dtype=torch.float32)
+            at = sumsq.data_ptr()
+            clip = (at, self.max_norm, self.grad_norm.data_ptr(), sum(counts))
             for (_, _, dtype, n, table, _), c in zip(todo, counts):
-                _lib.check(lib.asyrp_grad_sumsq(device.index, table, n, dtype, C.c_void_p(partial.data_ptr() + 8 * at), stream))
-                at += c
-            both = torch.empty(4, device=device, dtype=torch.float32)
-            clip, self.grad_norm = both[0:2], both[2]
-            _lib.check(lib.asyrp_grad_clip(device.index, _ptr(partial), at, self.max_norm, _ptr(self.grad_norm), _ptr(clip), stream))
+                _lib.check(lib.asyrp_grad_sumsq(device.index, table, n, dtype, at, stream))
+                at += 8 * c
         for g, mo, dtype, n, table, params in todo:
             lr, lr_device = g["lr"], 0
             if isinstance(lr, torch.Tensor) and lr.is_cuda:
                 if lr.dtype != torch.float32 or lr.device != device:
                     raise ValueError(f"lr as a device tensor must be float32 on {device}")
                 lr, lr_device = 0.0, lr.data_ptr()
-            spec = _lib.ADAMW.pack(float(lr), *g["betas"], g["eps"], g["weight_decay"], lr_device, mo.steps.data_ptr(), 0 if clip is None else clip.data_ptr(),
-                                   mo.m.data_ptr(), mo.v.data_ptr(), *(p.data_ptr() if p is not None else 0 for p in (mo.me, mo.ve)), mo.bits, self.seed)
-            scratch = torch.empty(32 * n, device=device, dtype=torch.uint8)
-            _lib.check(lib.asyrp_adamw_step(device.index, spec, table, n, dtype, _ptr(scratch), stream))
-            torch.autograd.graph.increment_version(params)   # the engine re-uploads parameters whose version has moved
+            spec = _lib.ADAMW.pack(float(lr), *g["betas"], g["eps"], g["weight_decay"], lr_device, mo.steps.data_ptr(), *clip[:3], mo.m.data_ptr(), mo.v.data_ptr(),
+                                   *((mo.me.data_ptr(), mo.ve.data_ptr()) if mo.bits == 8 else (0, 0)), clip[3], mo.bits, self.seed)
+            scratch = torch.empty(4 * (n + 1) + n, device=device, dtype=torch.float32)
+            _lib.check(lib.asyrp_adamw_step(device.index, spec, table, n, dtype, scratch.data_ptr(), stream))
+            torch.autograd.graph.increment_version(params)   # the engine uploads parameters whose version has moved
         return loss

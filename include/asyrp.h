@@ -131,11 +131,14 @@ typedef struct asyrp_adamw {
   double lr, beta1, beta2, eps, weight_decay;
   const float* lr_device;         /* device, nullable: read in place of lr when the step runs (a captured step whose lr changes) */
   int32_t* steps;                 /* device: step counts, advanced by the call */
-  const float* clip;              /* device, nullable: {factor, skip} as asyrp_grad_clip writes them */
+  const double* sumsq;            /* device, nullable: partial sums of squares of every gradient that is clipped together */
+  double max_norm;                /* with sumsq: gradients are scaled by min(1, max_norm / (norm + 1e-6)); a norm that is not finite skips the step */
+  float* grad_norm;               /* device, nullable: takes the norm */
   void* exp_avg;                  /* device: flat moments, f32 or (state_bits = 8) one byte each */
   void* exp_avg_sq;
   uint8_t* exp_avg_scale;         /* device, state_bits = 8: one exponent byte per 256 values */
   uint8_t* exp_avg_sq_scale;
+  int32_t sumsq_count;
   int32_t state_bits;             /* 32 or 8 */
   uint32_t seed;                  /* of the 8-bit states' rounding */
 } asyrp_adamw;
@@ -313,12 +316,10 @@ int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const
                                  float* dgate, float* d_after_weight, float* d_after_bias, float* d_before_weight, float* d_before_bias, float* workspace,
                                  void* stream);
 
-/* AdamW over many tensors (host table).  asyrp_grad_sumsq writes ASYRP_ADAMW_PARTIALS fp64 sums of squares per 100 tensors; asyrp_grad_clip makes the
- * norm and {factor, skip} of them (factor = min(1, max_norm / (norm + 1e-6)); skip = 1 where the norm is not finite: the step then changes
- * nothing); asyrp_adamw_step advances the counts and updates parameters and moments; scratch: 32 bytes per tensor.
- * asyrp_adamw_moments reads 8-bit moments as f32 (n values, a multiple of 256). */
+/* AdamW over many tensors (host table).  asyrp_grad_sumsq writes ASYRP_ADAMW_PARTIALS fp64 sums of squares per 100 tensors; asyrp_adamw_step makes the
+ * norm of them where it is given them (and where that is not finite changes nothing, the counts included), advances the counts and updates parameters
+ * and moments; scratch: 16 + 20 bytes per tensor, 16-byte aligned.  asyrp_adamw_moments reads 8-bit moments as f32 (n values, a multiple of 256). */
 int asyrp_grad_sumsq(int device, const asyrp_adamw_tensor* tensors, int n, int dtype, double* partial, void* stream);
-int asyrp_grad_clip(int device, const double* partial, int n_partial, double max_norm, float* norm, float* clip, void* stream);
 int asyrp_adamw_step(int device, const asyrp_adamw* c, const asyrp_adamw_tensor* tensors, int n, int dtype, void* scratch, void* stream);
 int asyrp_adamw_moments(int device, const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const uint8_t* exp_avg_scale, const uint8_t* exp_avg_sq_scale,
                         int64_t n, float* out_avg, float* out_avg_sq, void* stream);
