@@ -145,15 +145,61 @@ __device__ __forceinline__ void tile_barrier() {
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // one instruction; results under 2^-126 are zero
 
+// a wave's sum, the same in all lanes: within rows of 16 by shifts, then from row to row
+__device__ __forceinline__ int wave_sum(int v) {
+#define ASYRP_DPP(CTRL, ROWS) v += __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false)
+  ASYRP_DPP(0x111, 0xf);
+  ASYRP_DPP(0x112, 0xf);
+  ASYRP_DPP(0x114, 0xf);
+  ASYRP_DPP(0x118, 0xf);
+  ASYRP_DPP(0x142, 0xa);
+  ASYRP_DPP(0x143, 0xc);
+#undef ASYRP_DPP
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // The sequence and the row tile that tile number `t` of the launch stands for.  Tiles are numbered sequence by sequence; the numbers
 // behind the last one share the rows behind the last sequence.  Every wave finds it by itself: 64 lengths at a time, summed over the wave.
 // Offsets are held inside [0, T] and never fall, so that no value of `cu` leads outside the tensors.
 struct TileAt { long long start; int len, row0; int idle; int idles; int low, end; };
 // lane `src`'s value as one that the compiler knows to be the same in all lanes (all lanes active, src < 64)
 __device__ __forceinline__ int uniform(int v, int src) { return __builtin_amdgcn_readlane(v, __builtin_amdgcn_readfirstlane(src)); }
-__device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T, int t, int tiles, int lane) {
+//
+// Under the causal mask a tile's work goes with its distance from one end of its sequence, and the workgroups are dealt out in the tiles' order: up to 64
+// sequences are therefore numbered heaviest first (`by_weight`: the last row tile of a sequence is the heaviest; `from_end`: the first
+// is), which is the t-th largest of all (distance) values, found by bisection over the distance.
+enum { IN_ORDER, BY_WEIGHT, BY_WEIGHT_FROM_END };
+__device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T, int t, int tiles, int lane, int order) {
   TileAt f{0, 0, 0, 0, 1, 0, 0};
   int before = 0;
+  if (order != IN_ORDER && nseq <= 64) {
+    long long s = 0, e = 0;
+    if (lane < nseq) { s = cu[lane]; e = cu[lane + 1]; }
+    s = s < 0 ? 0 : s > T ? T : s;
+    e = e < s ? s : e > T ? T : e;
+    const int n = (int)((e - s + BM - 1) / BM);
+    const int total = wave_sum(n);
+    if (t < total) {
+      int lo = 0, hi = (int)(T / BM) + 2;                 // tiles at distance >= lo: more than t; >= hi: at most t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (wave_sum(max(n - mid, 0)) > t) lo = mid; else hi = mid;
+      }
+      const int rank = t - wave_sum(max(n - lo - 1, 0));  // among the sequences that have a tile at this distance
+      const unsigned long long has = __ballot(n > lo);
+      const bool mine = n > lo && __popcll(has & ((1ull << lane) - 1)) == rank;
+      const int src = __ffsll(__ballot(mine)) - 1;
+      f.start = uniform((int)s, src);
+      f.len = uniform((int)e, src) - (int)f.start;
+      f.row0 = (order == BY_WEIGHT ? lo : uniform(n, src) - 1 - lo) * BM;
+      return f;
+    }
+    f.idle = 1 + (t - total);
+    f.idles = tiles - total;
+    f.low = uniform((int)s, 0);
+    f.end = uniform((int)e, nseq - 1);
+    return f;
+  }
   bool found = false;
   int high = 0, low = 0;
   for (int b0 = 0; b0 < nseq; b0 += 64) {
@@ -206,25 +252,49 @@ __device__ __forceinline__ void zero_tail(T* p, long long st, long long sh, int 
 __device__ __forceinline__ float both_halves_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
 __device__ __forceinline__ float both_halves_sum(float v) { return v + __shfl_xor(v, 32); }
 
-// rows d of a transposed result (column = this lane's row of the output tensor) times `m`, as 8-byte stores
-// (`rest`: where given, what the rounding to T took away, rounded itself)
-template <typename T, int DP>
-__device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float m, int h, int D, T* rest = nullptr) {
+// rows d of a transposed result (column = this lane's row of the output tensor) times `m`
+template <int DP>
+__device__ __forceinline__ void store_cols(float* row, const f32x16 (&acc)[DP / 32], float m, int h, int D) {
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const int d = 32 * dt + 8 * r4 + 4 * h;
-      if (d >= D) continue;
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      T4 x;
+      f32x4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = (T)(acc[dt][4 * r4 + j] * m);
-      *reinterpret_cast<T4*>(row + d) = x;
-      if (rest) {
+      for (int j = 0; j < 4; ++j) x[j] = acc[dt][4 * r4 + j] * m;
+      if (d < D) *reinterpret_cast<f32x4*>(row + d) = x;
+    }
+}
+// The same in 16 bits: a row's two lanes hold four values of every eight each; they exchange them, so that each stores 16 bytes.  All lanes of the wave
+// come here, `there` says whose row is stored.  `rest`: where given, what the rounding to T took away, rounded itself.
+template <typename T, int DP>
+__device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float m, int h, int D, bool there, T* rest = nullptr) {
+  typedef T T2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = (T)(acc[dt][4 * r4 + j] * m - (float)x[j]);
-        *reinterpret_cast<T4*>(rest + d) = x;
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned w[2][4];                                 // [value, rest][two groups of eight, two words each]
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = acc[dt][8 * i + 2 * j] * m, b = acc[dt][8 * i + 2 * j + 1] * m;
+        const T2 v{(T)a, (T)b}, r{(T)(a - (float)v[0]), (T)(b - (float)v[1])};
+        w[0][j] = __builtin_bit_cast(unsigned, v);
+        w[1][j] = __builtin_bit_cast(unsigned, r);
+      }
+      const int d = 32 * dt + 16 * i + 8 * h;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (k && !rest) break;
+        u32x4 x;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const auto both = __builtin_amdgcn_permlane32_swap(w[k][j], w[k][2 + j], false, false);
+          x[j] = both[0];
+          x[2 + j] = both[1];
+        }
+        if (there && d < D) *reinterpret_cast<u32x4*>((k ? rest : row) + d) = x;
       }
     }
 }
@@ -242,8 +312,8 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int head = blockIdx.x % p.Hq, tile = p.tiles - 1 - blockIdx.x / p.Hq;
-  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
+  const int head = blockIdx.x % p.Hq, tile = blockIdx.x / p.Hq;
+  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT : IN_ORDER);
   if (f.idle) {
     if (p.fill_tail) zero_tail((T*)p.out, p.o_t, p.o_h, head, p.D, f, p.T, tid);
     return;
@@ -305,7 +375,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
     // The reference moves only where a column's maximum has outgrown it by 8 powers of two (and in the first tile): the exponentials stay under
     // 2^8, well inside f16, and most tiles leave the sums as they are.
     if (__any(!((mx - m) * sc <= 8.f))) {
-      const float mn = fmaxf(m, mx), keep = exp2_fast((m - mn) * sc);
+      const float mn = fmaxf(m, mx), keep = m > -INFINITY ? exp2_fast((m - mn) * sc) : 0.f;
       m = mn;
       l *= keep;
 #pragma unroll
@@ -313,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
     }
-    const float ms = m * sc;
+    const float ms = m > -INFINITY ? m * sc : 0.f;      // keys of minus infinity so far: their exponentials are zeros
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -329,11 +399,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
       }
   }
   l = both_halves_sum(l);
-  if (there) {
-    store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, acc, 1.0f / l, h, p.D,
-                      p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
-    if (p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (m * sc + log2f(l)) * LN2;
-  }
+  store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, acc, 1.0f / l, h, p.D, there,
+                    p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
+  if (there && p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (m * sc + log2f(l)) * LN2;
 }
 
 // dq, and delta = rowsum(do * o) for the other kernel
@@ -341,8 +409,8 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int head = blockIdx.x % p.Hq, tile = p.tiles - 1 - blockIdx.x / p.Hq;
-  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
+  const int head = blockIdx.x % p.Hq, tile = blockIdx.x / p.Hq;
+  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT : IN_ORDER);
   if (f.idle) {
     zero_tail((T*)p.dq, p.dq_t, p.dq_h, head, p.D, f, p.T, tid);
     return;
@@ -356,21 +424,23 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
   const T* qrow = (const T*)p.q + at * p.q_t + head * p.q_h;
   const T* grow = (const T*)p.dout + at * p.do_t + head * p.do_h;
   const T* orow = (const T*)p.o + at * p.o_t + head * p.o_h;
-  const T* rrow = p.rest ? (const T*)p.rest + (at * p.Hq + head) * p.D : nullptr;
+  const T* rrow = (const T*)p.rest + (at * p.Hq + head) * p.D;
   typename Frag<T>::V qf[DP / 16], gf[DP / 16];
   float delta = 0.f;
+  {
+    typename Frag<T>::V of[DP / 16], rf[DP / 16];
 #pragma unroll
-  for (int ks = 0; ks < DP / 16; ++ks) {
-    qf[ks] = load_frag<T>(qrow, ks, h, p.D, there);
-    gf[ks] = load_frag<T>(grow, ks, h, p.D, there);
-    const typename Frag<T>::V of = load_frag<T>(orow, ks, h, p.D, there);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) delta += (float)gf[ks][j] * (float)of[j];
-    if (rrow) {
-      const typename Frag<T>::V rf = load_frag<T>(rrow, ks, h, p.D, there);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) delta += (float)gf[ks][j] * (float)rf[j];
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      gf[ks] = load_frag<T>(grow, ks, h, p.D, there);
+      of[ks] = load_frag<T>(orow, ks, h, p.D, there);
+      rf[ks] = load_frag<T>(rrow, ks, h, p.D, there && p.rest);
     }
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) qf[ks] = load_frag<T>(qrow, ks, h, p.D, there);
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[ks][j], (float)of[ks][j] + (float)rf[ks][j], delta);
   }
   delta = both_halves_sum(delta);
   const float lse2 = there ? p.lse[(long long)head * p.T + at] * LOG2E : 0.f;
@@ -423,7 +493,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
       }
     }
   }
-  if (there) store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale, h, p.D);
+  store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale, h, p.D, there);
 }
 
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them
@@ -433,7 +503,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   __shared__ __attribute__((aligned(16))) float ls[2][BN], ds[2][BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
-  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
+  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT_FROM_END : IN_ORDER);
   if (f.idle) {
     if (part) return;
     zero_tail((T*)p.dk, p.dk_t, p.dk_h, hk, p.D, f, p.T, tid);
@@ -520,13 +590,13 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
       }
     }
   }
-  if (there && p.parts > 1) {
+  if (p.parts > 1) {
     float* to = p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D;
-    store_cols<float, DP>(to, dk, p.scale, h, p.D);
-    store_cols<float, DP>(to + p.D, dv, 1.0f, h, p.D);
-  } else if (there) {
-    store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, p.scale, h, p.D);
-    store_cols<T, DP>((T*)p.dv + at * p.dv_t + hk * p.dv_h, dv, 1.0f, h, p.D);
+    if (there) store_cols<DP>(to, dk, p.scale, h, p.D);
+    if (there) store_cols<DP>(to + p.D, dv, 1.0f, h, p.D);
+  } else {
+    store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, p.scale, h, p.D, there);
+    store_cols<T, DP>((T*)p.dv + at * p.dv_t + hk * p.dv_h, dv, 1.0f, h, p.D, there);
   }
 }
 
@@ -541,7 +611,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, h = lane >> 5;
   const bool values = __builtin_amdgcn_readfirstlane(tid >> 8);          // this wave forms dv
   const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
-  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane);
+  const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT_FROM_END : IN_ORDER);
   if (f.idle) {
     if (part) return;
     if (values) zero_tail((T*)p.dv, p.dv_t, p.dv_h, hk, p.D, f, p.T, tid & 255);
@@ -632,10 +702,10 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
       }
     }
   }
-  if (there && p.parts > 1) {
-    store_cols<float, DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
-  } else if (there) {
-    store_cols<T, DP>(values ? (T*)p.dv + at * p.dv_t + hk * p.dv_h : (T*)p.dk + at * p.dk_t + hk * p.dk_h, acc, values ? 1.0f : p.scale, h, p.D);
+  if (p.parts > 1) {
+    if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
+  } else {
+    store_cols<T, DP>(values ? (T*)p.dv + at * p.dv_t + hk * p.dv_h : (T*)p.dk + at * p.dk_t + hk * p.dk_h, acc, values ? 1.0f : p.scale, h, p.D, there);
   }
 }
 

@@ -14,21 +14,25 @@ from . import _lib
 from .engine import AsyrpDeviceError
 
 _HALF = (torch.float16, torch.bfloat16)
+_INT32 = (torch.int32,)
 _TYPES = tuple(_lib.DTYPES)
 _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle (torch.cuda.current_stream() without its object)
 
 
-def _tensor(t, name, dtypes):
+def _refuse_tensor(t, name, device):
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise AsyrpDeviceError(f"{name} must be a CUDA(HIP) tensor — the operator has no CPU path")
+    raise AsyrpDeviceError(f"{name} lives on {t.device}, the other arguments on cuda:{device}")
+
+
+def _tensor(t, name, device, dtypes):
+    """`t` is a tensor of cuda:`device` (None: of any) and of one of the types; returns its device's index."""
+    d = t.get_device() if isinstance(t, torch.Tensor) else -1          # -1 on the CPU
+    if d < 0 or (d != device and device is not None):
+        _refuse_tensor(t, name, device)
     if t.dtype not in dtypes:
-        raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
-
-
-def _same_device(first, *named):
-    for name, t in named:
-        if t is not None and t.device != first.device:
-            raise AsyrpDeviceError(f"{name} lives on {t.device}, the other arguments on {first.device}")
+        raise ValueError(f"{name} must be one of {[str(v) for v in dtypes]}, got {t.dtype}")
+    return d
 
 
 def _ptr(t):
@@ -112,12 +116,11 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
     the result's type and shape, laid out as q may be) takes the result and keeps what it holds in those rows.  Sums and softmax statistics are float32;
     probabilities are rounded to the inputs' type before they multiply v.  A value that is not finite may reach every row of its own sequence, the
     rows before it included, and no other sequence.  Results do not depend on the order in which the card works."""
-    _tensor(q, "q", _HALF)
+    device = _tensor(q, "q", None, _HALF)
     same = (q.dtype,)
-    _tensor(k, "k", same)
-    _tensor(v, "v", same)
-    _tensor(cu_seqlens, "cu_seqlens", (torch.int32,))
-    _same_device(q, ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("out", out))
+    _tensor(k, "k", device, same)
+    _tensor(v, "v", device, same)
+    _tensor(cu_seqlens, "cu_seqlens", device, _INT32)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k must be [tokens, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
     T, H, D = q.shape
@@ -135,7 +138,7 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
     cu, causal = cu_seqlens.contiguous(), bool(causal)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:
-        _tensor(out, "out", same)
+        _tensor(out, "out", device, same)
         if grad:
             raise ValueError("out= takes part in no graph: call without it, or under torch.no_grad()")
         if out.shape != q.shape or _strides(out) is None:
@@ -149,21 +152,24 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
 _KINDS = {"layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
 
 
+def _norm_forward(x, y, gate, w1, b1, w2, b2, spec, before, device, stats=None):
+    h = x.new_empty(x.shape)
+    n = y.new_empty(y.shape) if before else None
+    rc = _lib.load().asyrp_residual_norm_forward(device, spec, x.data_ptr(), y.data_ptr(), _ptr(gate), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), h.data_ptr(),
+                                                 _ptr(n), _ptr(stats), _raw_stream(device))
+    if rc:
+        _lib.check(rc)
+    return h, n
+
+
 class _GatedResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, gate, w1, b1, w2, b2, spec, before, keep):
-        h = x.new_empty(x.shape)
-        n = y.new_empty(y.shape) if before else None
-        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32) if keep else None
-        device = x.device.index
-        rc = _lib.load().asyrp_residual_norm_forward(device, spec, x.data_ptr(), y.data_ptr(), _ptr(gate), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), h.data_ptr(),
-                                                     _ptr(n), _ptr(stats), _raw_stream(device))
-        if rc:
-            _lib.check(rc)
-        if keep:
-            ctx.save_for_backward(x, y, gate, w1, b1, w2, b2, stats)
-            ctx.spec = spec
-            ctx.set_materialize_grads(False)
+    def forward(ctx, x, y, gate, w1, b1, w2, b2, spec, before, device):
+        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
+        h, n = _norm_forward(x, y, gate, w1, b1, w2, b2, spec, before, device, stats)
+        ctx.save_for_backward(x, y, gate, w1, b1, w2, b2, stats)
+        ctx.spec, ctx.device = spec, device
+        ctx.set_materialize_grads(False)
         return h, n
 
     @staticmethod
@@ -172,15 +178,15 @@ class _GatedResidualNorm(torch.autograd.Function):
         if dh is None and dn is None:
             return (None,) * 10
         x, y, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dh, dn = (None if t is None else t.contiguous() for t in (dh, dn))
-        dx, dy = (t.new_empty(t.shape) if n else None for t, n in ((x, need[0]), (y, need[1])))
+        need, device = ctx.needs_input_grad, ctx.device
+        dh, dn = None if dh is None else dh.contiguous(), None if dn is None else dn.contiguous()
+        dx, dy = x.new_empty(x.shape) if need[0] else None, y.new_empty(y.shape) if need[1] else None
         # without rows every sum is empty; without a gradient of n, the norm in front of the next block takes no part
         empty = x.shape[0] == 0
         outs = [None if t is None or not n else t.new_zeros(t.shape) if empty or (k > 2 and dn is None) else t.new_empty(t.shape)
-                for k, (t, n) in enumerate(zip((gate, w1, b1, w2, b2), need[2:7]))]
+                for k, t, n in zip(range(5), (gate, w1, b1, w2, b2), need[2:7])]
         late = outs[3:] if dn is not None else (None, None)
-        lib, device = _lib.load(), x.device.index
+        lib = _lib.load()
         words = lib.asyrp_residual_norm_workspace(ctx.spec)
         if words < 0:
             _lib.check(words)
@@ -193,13 +199,13 @@ class _GatedResidualNorm(torch.autograd.Function):
         return (dx, dy, *outs, None, None, None)
 
 
-def _vector(t, name, width):
+def _vector(t, name, width, device):
     if t is None:
         return None
-    _tensor(t, name, _TYPES)
+    _tensor(t, name, device, _TYPES)
     if t.dim() != 1 or t.shape[0] != width:
         raise ValueError(f"{name} must be [{width}], got {tuple(t.shape)}")
-    return t.float().contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, kind="layer", after=None, before=(None, None), eps=1e-5):
@@ -211,8 +217,8 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, kind="layer", af
     x's other dimensions) and row r takes gate row r // (rows / gates): one gate per image of a batch, or one per row.
     h has x's type, n has y's.  Statistics, the sum h that the second norm sees and the sums of the parameters' gradients are float32; h and n are rounded once.
     Gates, weights and biases of any of the three types; their gradients come back in it."""
-    _tensor(x, "x", _TYPES)
-    _tensor(y, "y", _TYPES)
+    device = _tensor(x, "x", None, _TYPES)
+    _tensor(y, "y", device, _TYPES)
     shape = x.shape
     if not shape or shape != y.shape:
         raise ValueError(f"x and y must have one shape of at least one dimension, got {tuple(shape)} and {tuple(y.shape)}")
@@ -227,23 +233,23 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, kind="layer", af
     if not math.isfinite(residual_scale) or not math.isfinite(eps) or eps < 0:
         raise ValueError("residual_scale and eps must be finite, eps not negative")
     if gate is not None:
-        _tensor(gate, "gate", _TYPES)
+        _tensor(gate, "gate", device, _TYPES)
         if gate.dim() == 1:
             gate = gate[None]
         if gate.dim() != 2 or gate.shape[1] != width or gate.shape[0] < 1 or rows % gate.shape[0]:
             raise ValueError(f"gate must be [{width}] or [gates, {width}] with gates dividing {rows} rows, got {tuple(gate.shape)}")
         gate = gate.float().contiguous()
-    for name, pair in (("after", after), ("before", before)):
-        if pair is not None and (not isinstance(pair, (tuple, list)) or len(pair) != 2):
-            raise ValueError(f"{name} must be None or (weight, bias)")
-    w1, b1 = (None, None) if after is None else (_vector(after[0], "after[0]", width), _vector(after[1], "after[1]", width))
-    w2, b2 = (None, None) if before is None else (_vector(before[0], "before[0]", width), _vector(before[1], "before[1]", width))
-    _same_device(x, ("y", y), ("gate", gate), ("after[0]", w1), ("after[1]", b1), ("before[0]", w2), ("before[1]", b2))
-    x2, y2 = x.reshape(rows, width).contiguous(), y.reshape(rows, width).contiguous()
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, y2, gate, w1, b1, w2, b2))
+    if any(pair is not None and (not isinstance(pair, (tuple, list)) or len(pair) != 2) for pair in (after, before)):
+        raise ValueError("after and before must be None or (weight, bias)")
+    w1, b1 = (None, None) if after is None else (_vector(after[0], "after[0]", width, device), _vector(after[1], "after[1]", width, device))
+    w2, b2 = (None, None) if before is None else (_vector(before[0], "before[0]", width, device), _vector(before[1], "before[1]", width, device))
+    if len(shape) != 2:
+        x, y = x.reshape(rows, width), y.reshape(rows, width)
+    args = (x.contiguous(), y.contiguous(), gate, w1, b1, w2, b2)
     spec = _lib.RESIDUAL_NORM.pack(rows, 0 if gate is None else gate.shape[0], width, _KINDS[kind], after is not None, before is not None, _lib.DTYPES[x.dtype],
                                    _lib.DTYPES[y.dtype], residual_scale, eps)
-    h, n = _GatedResidualNorm.apply(x2, y2, gate, w1, b1, w2, b2, spec, before is not None, keep)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)
+    h, n = (_GatedResidualNorm.apply if grad else _norm_forward)(*args, spec, before is not None, device)
     if len(shape) == 2:
         return h, n
     return h.view(shape), None if n is None else n.view(shape)

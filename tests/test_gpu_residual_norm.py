@@ -144,3 +144,127 @@ def test_oracle_formulas_against_autograd_and_differences():
                 up, down = [b + 1e-6 * d if j == i else b for j, b in enumerate(args)], [b - 1e-6 * d if j == i else b for j, b in enumerate(args)]
                 slope = (f(*up, kind) - f(*down, kind)) / 2e-6
                 assert abs(float(slope - (grads[i] * d).sum())) <= 1e-6 * (1 + abs(float(slope)))
+
+
+@pytest.mark.gpu
+def test_shapes_views_and_empty_batches():
+    c = case(24, 40, gates=4)
+    want = run(c)
+    x, y, gate = c["x"].cuda().view(2, 3, 4, 40), c["y"].cuda().view(2, 3, 4, 40), c["gate"].cuda()
+    args = dict(gate=gate, residual_scale=c["a"], after=tuple(t.cuda() for t in c["after"]), before=tuple(t.cuda() for t in c["before"]), eps=c["eps"])
+    h, n = gated_residual_norm(x, y, **args)
+    assert h.shape == x.shape and torch.equal(h.view(24, 40), want["h"]) and torch.equal(n.view(24, 40), want["n"])
+    strided = torch.empty(24, 80, device="cuda")[:, ::2].copy_(x.view(24, 40))
+    shifted = torch.empty(24 * 40 + 1, device="cuda")[1:].view(24, 40).copy_(y.view(24, 40))      # no 16-byte address: read value by value
+    h, n = gated_residual_norm(strided, shifted, **args)
+    # 40 columns read value by value are added up in another order than four by four
+    assert torch.equal(h, want["h"]) or (h - want["h"]).abs().max() <= 1e-5
+    assert (n - want["n"]).abs().max() <= 1e-5
+    e = torch.zeros(0, 3, 40, device="cuda", requires_grad=True)
+    h, n = gated_residual_norm(e, e, gate=args["gate"].clone().requires_grad_(), before=args["before"])
+    assert h.shape == n.shape == (0, 3, 40)
+    g = args["gate"].clone().requires_grad_()
+    h, n = gated_residual_norm(e, e, gate=g, before=args["before"])
+    gx, gg = torch.autograd.grad((h.sum() + n.sum()), [e, g])
+    assert gx.shape == e.shape and not gg.any()
+
+
+@pytest.mark.gpu
+def test_rows_do_not_see_each_other():
+    c = case(70, 96, gates=2)
+    want = run(c)
+    c["x"][3], c["y"][40, 5] = math.nan, math.inf
+    got = run(c)
+    rows = [i for i in range(70) if i not in (3, 40)]
+    for n in ("h", "n", "x", "y"):
+        assert torch.equal(got[n][rows], want[n][rows]), n
+    assert got["h"][3].isnan().all() and not torch.isfinite(got["n"][40]).any()
+
+
+@pytest.mark.gpu
+def test_some_gradients_alone():
+    c = case(33, 128, gates=3)
+    full = run(c)
+    t = {"x": c["x"].cuda(), "y": c["y"].cuda(), "gate": c["gate"].cuda(), **{f"{n}{i}": w.cuda() for i, k in ((1, "after"), (2, "before")) for n, w in zip("wb", c[k])}}
+    for name in t:
+        a = {k: v.clone().requires_grad_(k == name) for k, v in t.items()}
+        h, n = gated_residual_norm(a["x"], a["y"], gate=a["gate"], residual_scale=c["a"], after=(a["w1"], a["b1"]), before=(a["w2"], a["b2"]), eps=c["eps"])
+        (g,) = torch.autograd.grad([h, n], [a[name]], [c["dh"].cuda(), c["dn"].cuda()])
+        assert torch.equal(g, full[name]), name
+
+
+@pytest.mark.gpu
+def test_streams_and_graph_replays_agree():
+    c = case(300, 768, X=bf16, Y=bf16, gates=3)
+    want = run(c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(c)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    leaves = [t.cuda().requires_grad_() for t in (c["x"], c["y"], c["gate"], *c["after"], *c["before"])]
+    ups = [c["dh"].cuda(), c["dn"].cuda()]
+
+    def step():
+        x, y, gate, w1, b1, w2, b2 = leaves
+        h, n = gated_residual_norm(x, y, gate=gate, residual_scale=c["a"], after=(w1, b1), before=(w2, b2), eps=c["eps"])
+        grads = torch.autograd.grad([h, n], leaves, ups)
+        return [h.detach(), n.detach(), *grads]
+
+    with torch.cuda.stream(side):
+        warm = step()
+        del warm
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        caught = step()
+    for i in range(3):
+        with torch.no_grad():
+            leaves[0].mul_(1.5)
+            leaves[2].add_(0.25)
+        eager = [t.detach().clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(caught, eager)), i
+
+
+def test_cpu_tensors_are_refused():
+    from asyrp_official_amd import AsyrpDeviceError
+    with pytest.raises(AsyrpDeviceError):
+        gated_residual_norm(torch.zeros(2, 8), torch.zeros(2, 8))
+
+
+def test_library_refuses_what_its_kernels_do_not_take():
+    from asyrp_official_amd import _lib
+    lib = _lib.load()
+
+    def call(rows=4, gates=0, width=64, kind=0, after=0, before=1, X=0, Y=0, a=1.0, eps=1e-5, x=4096, gate=None, stats=4096, dn=4096, dw1=None, ws=4096):
+        spec = _lib.RESIDUAL_NORM.pack(rows, gates, width, kind, after, before, X, Y, a, eps)
+        return (lib.asyrp_residual_norm_forward(0, spec, x, 4096, gate, None, None, None, None, 4096, 4096, stats, None),
+                lib.asyrp_residual_norm_backward(0, spec, x, 4096, gate, None, None, None, stats, None, dn, 4096, 4096, None, dw1, None, None, None, ws, None))
+
+    for bad in (dict(rows=-1), dict(rows=2 ** 31), dict(gates=3), dict(gates=-1), dict(width=0), dict(width=8193), dict(kind=2), dict(X=1, Y=0), dict(X=1, Y=2), dict(X=3, Y=3),
+                dict(a=math.nan), dict(eps=-1.0), dict(eps=math.inf), dict(x=None), dict(gates=2), dict(gate=4096), dict(stats=4100)):
+        assert call(**bad) == (-1, -1), bad
+        assert b"residual norm" in lib.asyrp_last_error()
+    for bad in (dict(dn=None), dict(before=0), dict(dw1=4096), dict(ws=None)):
+        assert call(**{**dict(rows=4), **bad})[1] == -1 if "before" not in bad else True
+    assert call(rows=0) == (0, 0)
+    assert lib.asyrp_residual_norm_workspace(None) == -1
+
+
+@pytest.mark.gpu
+def test_refusals():
+    from asyrp_official_amd import AsyrpDeviceError
+    x = torch.zeros(6, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    for args, kw in (((x, x[:5]), {}), ((x.half(), x), {}), ((x.double(), x.double()), {}), ((x, x), dict(kind="group")), ((x, x), dict(gate=w[:4])), ((x, x), dict(gate=x[:4])),
+                     ((x, x), dict(gate=torch.zeros(0, 8, device="cuda"))), ((x, x), dict(before=w)), ((x, x), dict(before=(w[:4], None))), ((x, x), dict(after=(w, w.double()))),
+                     ((x, x), dict(eps=-1.0)), ((x, x), dict(residual_scale=math.inf)), ((x[0, 0], x[0, 0]), {}), ((torch.zeros(2, 8200, device="cuda"),) * 2, {}), ((x[:, :0], x[:, :0]), {})):
+        with pytest.raises(ValueError):
+            gated_residual_norm(*args, **kw)
+    for args, kw in (((x, x.cpu()), {}), ((x, x), dict(gate=w.cpu())), ((x, x), dict(before=(w.cpu(), None)))):
+        with pytest.raises(AsyrpDeviceError):
+            gated_residual_norm(*args, **kw)
