@@ -13,7 +13,7 @@ import torch
 from asyrp_official_amd import AdamW, AsyrpDeviceError
 
 U = 2.0 ** -24
-pytestmark = pytest.mark.gpu
+
 
 
 def tensors(shapes, dtype=torch.float32, seed=0, std=1.0):
@@ -54,6 +54,7 @@ SHAPES = {
 }
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("max_norm", [None, 0.5], ids=["free", "clipped"])
 @pytest.mark.parametrize("name", list(SHAPES))
 def test_32_bit_steps_follow_fp64(name, max_norm):
@@ -80,6 +81,7 @@ def test_32_bit_steps_follow_fp64(name, max_norm):
         assert ((p.detach().double().cpu() - plain.p[i]).abs() <= n * (3 * U * (plain.p[i].abs() + 0.1) + 1e-2 * (10 * U * 10 + 10 * noise))).all()
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,half", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)], ids=["bf16", "f16"])
 def test_16_bit_parameters_are_rounded_once(dtype, half):
     init, grads = tensors([(300,), (17, 31)], dtype), tensors([(300,), (17, 31)], dtype, seed=1)
@@ -127,6 +129,7 @@ def coins(i, seed, step):
     return x & 0xFFFFF, ((x * 0x9E3779B1) & M) >> 12
 
 
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 255, 256, 700])
 def test_8_bit_moments_are_the_codes_values(n):
     import numpy as np
@@ -158,3 +161,295 @@ def test_8_bit_moments_are_the_codes_values(n):
         gm, gv = (t[256:256 + n].cpu().numpy() for t in opt.moments()[0])
         assert np.array_equal(gm, m) and np.array_equal(gv, v)
         assert not opt.moments()[0][0][256 + n:].any() and not opt.moments()[0][1][256 + n:].any()
+
+
+def same_run(opt_a, ps_a, opt_b, ps_b, steps=2, seed=50):
+    """Both take the same gradients; their parameters and moments are equal to the bit afterwards."""
+    for k in range(steps):
+        for p, q, g in zip(ps_a, ps_b, tensors([p.shape for p in ps_a], seed=seed + k)):
+            p.grad = g.cuda().to(p.dtype)
+            q.grad = p.grad.clone()
+        opt_a.step()
+        opt_b.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps_a, ps_b))
+    for (m, v), (m2, v2) in zip(opt_a.moments(), opt_b.moments()):
+        assert torch.equal(m, m2) and torch.equal(v, v2)
+
+
+def trained(bits=32, shapes=((300,), (5, 7), (256,)), dtype=torch.float32, steps=3, **kw):
+    ps = params_of(tensors(shapes, dtype))
+    opt = AdamW(ps, lr=1e-2, state_bits=bits, seed=9, **kw)
+    for k in range(steps):
+        for p, g in zip(ps, tensors(shapes, dtype, seed=20 + k)):
+            p.grad = g.cuda()
+        opt.step()
+    return opt, ps
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_travels_through_files_copies_and_pickles(bits):
+    opt, ps = trained(bits)
+    buf = io.BytesIO()
+    torch.save(opt.state_dict(), buf)
+    buf.seek(0)
+    qs = [p.detach().clone().requires_grad_() for p in ps]
+    other = AdamW(qs, lr=5.0, state_bits=bits, seed=9)
+    other.load_state_dict(torch.load(buf, weights_only=True))
+    assert other.param_groups[0]["lr"] == 1e-2 and int(other.state[qs[0]]["step"]) == 3
+    same_run(opt, ps, other, qs)
+    opt, ps = trained(bits)
+    twin = copy.deepcopy({"opt": opt, "ps": ps})
+    same_run(opt, ps, twin["opt"], twin["ps"])
+    started, qs = trained(bits, steps=5)                        # into an optimiser that has moments of its own
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    started.load_state_dict(opt.state_dict())
+    same_run(opt, ps, started, qs)
+    with pytest.raises(ValueError):
+        AdamW(qs, state_bits=40 - bits).load_state_dict(opt.state_dict())
+    with pytest.raises(ValueError):
+        AdamW(qs[:2], state_bits=bits).load_state_dict(opt.state_dict())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_without_a_gradient_stands_still(bits):
+    init = tensors([(300,), (40,), (7,)])
+    ps = params_of(init)
+    opt, plain = AdamW(ps, lr=1e-2, state_bits=bits), Plain(init, 1e-2, (0.9, 0.999), 1e-8, 1e-2)
+    for k in range(3):
+        gs = tensors([p.shape for p in init], seed=k)
+        gs[1] = None if k < 2 else gs[1]
+        for p, g in zip(ps, gs):
+            p.grad = None if g is None else g.cuda()
+        opt.step()
+        plain.step(gs)
+        assert (k == 2) != torch.equal(ps[1].detach().cpu(), init[1])
+    assert [int(opt.state[p]["step"]) for p in ps] == [3, 1, 3]
+    # its first step is corrected as a first one: the whole rate, not a third of it.  (1 - lr wd), its product with p and the difference are rounded
+    # (u |p| each), and the update of at most lr in about ten places
+    assert ((ps[1].detach().double().cpu() - plain.p[1]).abs() <= 3 * U * plain.p[1].abs() + 10 * U * 1e-2).all()
+    before = [p.detach().clone() for p in ps]
+    opt.zero_grad()
+    opt.step()                                                  # no gradient at all
+    assert all(torch.equal(p, b) for p, b in zip(ps, before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_norm_that_is_not_finite_skips_the_step(bits, bad):
+    opt, ps = trained(bits, max_norm=1.0)
+    before = [p.detach().clone() for p in ps], [t.clone() for pair in opt.moments() for t in pair]
+    ps[2].grad[17] = bad
+    opt.step()
+    assert not math.isfinite(float(opt.grad_norm))
+    assert all(torch.equal(p, b) for p, b in zip(ps, before[0])) and all(torch.equal(t, b) for t, b in zip([t for pair in opt.moments() for t in pair], before[1]))
+    assert int(opt.state[ps[0]]["step"]) == 3
+
+
+@pytest.mark.gpu
+def test_without_a_norm_it_goes_its_way():
+    for bits in (32, 8):
+        opt, ps = trained(bits)
+        ps[0].grad[3] = math.nan
+        opt.step()
+        assert ps[0][3].isnan() and torch.isfinite(ps[1]).all() and int(ps[0].isnan().sum()) == 1
+        m, v = opt.moments()[0]
+        assert m[3].isnan() and v[3].isnan()
+        if bits == 8:                                           # the block that held it, and nothing else
+            assert m[:256].isnan().all() and torch.isfinite(m[256:]).all() and torch.isfinite(v[256:]).all()
+
+
+@pytest.mark.gpu
+def test_groups_types_and_layouts_of_one_step():
+    """Two groups with rates of their own, three types, gradients laid out otherwise, odd addresses: like one optimiser each."""
+    shapes = [(6, 4, 3, 3), (300,), (129,), (64, 2)]
+    types = [torch.float32, torch.bfloat16, torch.float16, torch.float32]
+    init = [t.to(d) for t, d in zip(tensors(shapes), types)]
+    ps = params_of(init)
+    flat = torch.zeros(129 + 3, device="cuda", dtype=torch.float16)
+    ps[2] = flat[3:].copy_(ps[2].detach()).requires_grad_()     # an address that no wide load may take
+    opt = AdamW([{"params": ps[:2], "lr": 1e-2}, {"params": ps[2:], "weight_decay": 0.5, "betas": (0.5, 0.9)}], lr=1e-3, max_norm=0.1)
+    alone = [AdamW([p.detach().clone().requires_grad_()], lr=lr, weight_decay=wd, betas=b) for p, lr, wd, b in
+             zip(ps, (1e-2, 1e-2, 1e-3, 1e-3), (1e-2, 1e-2, 0.5, 0.5), ((0.9, 0.999),) * 2 + ((0.5, 0.9),) * 2)]
+    for k in range(2):
+        gs = [t.to(d).cuda() for t, d in zip(tensors(shapes, seed=k), types)]
+        ps[0].grad = gs[0].to(memory_format=torch.channels_last)
+        ps[1].grad, ps[2].grad, ps[3].grad = gs[1], gs[2], gs[3].t().contiguous().t()
+        opt.step()
+        norm = math.sqrt(sum(float((g.double() ** 2).sum()) for g in gs))
+        assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+        for o, g in zip(alone, gs):
+            (q,) = o.param_groups[0]["params"]
+            q.grad = g
+            o.max_norm = None
+            q.grad = (g.float() * torch.tensor(min(1.0, 0.1 / (norm + 1e-6)), dtype=torch.float64).float().cuda()).to(torch.float32) if q.dtype == torch.float32 else g
+        for o, p in list(zip(alone, ps))[:1] + list(zip(alone, ps))[3:]:
+            o.step()
+            assert torch.equal(o.param_groups[0]["params"][0], p)
+    assert all(torch.isfinite(p).all() and not torch.equal(p.detach().cpu(), t) for p, t in zip(ps, init))
+    assert not flat[:3].any()
+
+
+@pytest.mark.gpu
+def test_a_captured_step_counts_and_follows_a_rate_on_the_device():
+    shapes = [(1000,), (33, 5)]
+    init = tensors(shapes)
+    for bits in (32, 8):
+        ps, qs = params_of(init), params_of(init)
+        lr = torch.tensor(1e-2, device="cuda")
+        opt = AdamW(ps, lr=lr, state_bits=bits, max_norm=2.0, seed=3)
+        eager = AdamW(qs, lr=1e-2, state_bits=bits, max_norm=2.0, seed=3)
+        for p, g in zip(ps, tensors(shapes, seed=1)):
+            p.grad = g.cuda()
+        opt.prepare()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        for k in range(4):
+            rate = float(torch.tensor(1e-2 / (k + 1)))          # what a float32 holds of it
+            lr.fill_(rate)
+            for p, q, g in zip(ps, qs, tensors(shapes, seed=10 + k)):
+                p.grad.copy_(g)
+                q.grad = g.cuda()
+            eager.param_groups[0]["lr"] = rate
+            graph.replay()
+            eager.step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(ps, qs)), (bits, k)
+            assert float(opt.grad_norm) == float(eager.grad_norm)
+        assert int(opt.state[ps[0]]["step"]) == 4
+
+
+@pytest.mark.gpu
+def test_another_stream_and_two_optimisers_at_once():
+    a, pa = trained(8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b, pb = trained(8)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(p, q) for p, q in zip(pa, pb))
+    c, pc = trained(8)
+    assert all(torch.equal(p, q) for p, q in zip(pa, pc))        # one seed, one result
+    # another seed rounds otherwise
+    d = AdamW(params_of(tensors([(300,)])), state_bits=8, seed=1)
+    e = AdamW(params_of(tensors([(300,)])), state_bits=8, seed=2)
+    for o in (d, e):
+        (p,) = o.param_groups[0]["params"]
+        p.grad = tensors([(300,)], seed=5)[0].cuda()
+        o.step()
+    assert not torch.equal(d.moments()[0][0], e.moments()[0][0])
+
+
+@pytest.mark.gpu
+def test_8_bit_rounding_keeps_the_mean():
+    """20000 values of one size, each block with a larger one beside them: the mean of what is kept is theirs within five standard errors (a code's
+    step is at most 1/8 of a value, so one rounding's deviation is at most 1/16)."""
+    n = 256 * 80
+    g = torch.full((n,), 0.731)
+    g[::256] = 100.0
+    p = torch.zeros(n, device="cuda", requires_grad=True)
+    opt = AdamW([p], state_bits=8, seed=77)
+    p.grad = g.cuda()
+    opt.step()
+    m, v = (t.double().cpu() for t in opt.moments()[0])
+    some = torch.ones(n, dtype=torch.bool)
+    some[::256] = False
+    for kept, want in ((m[some], 0.1 * 0.731), (v[some], 0.001 * 0.731 ** 2)):
+        assert abs(float(kept.mean()) / want - 1) <= 5 * (1 / 16) / math.sqrt(int(some.sum()))
+        assert float((kept / want - 1).abs().max()) <= 1 / 8
+
+
+@pytest.mark.gpu
+def test_the_deltablock_is_uploaded_again_behind_a_step():
+    """The engine keeps a copy of the DeltaBlock's weights and takes what a step changed."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+    from oracle import sampler as osamp
+    from oracle.weights import SMALL, hash_normal
+    from util_models import hip_model, synthetic
+    from asyrp_official_amd import denoising_step
+    model = hip_model(SMALL, synthetic(SMALL, 1, seed=11), 1, max_batch=1)
+    for p in model.parameters():
+        p.requires_grad_(False)
+    for p in model.layer_0.parameters():
+        p.requires_grad_(True)
+    b = osamp.beta_schedule().cuda()
+    x, tgt = (hash_normal(f"adamw.{k}", (1, 3, SMALL.resolution, SMALL.resolution)).cuda() for k in "xt")
+    one = torch.ones(1, device="cuda")
+    kw = dict(models=model, logvars=None, b=b, sampling_type="ddim", eta=0.0, index=0, t_edit=500, hs_coeff=(1.0, 1.0))
+    step = lambda: denoising_step(x, t=one * 768.0, t_next=one * 743.0, **kw)[1]  # noqa: E731
+    opt = AdamW(model.layer_0.parameters(), lr=1e-2, state_bits=8, max_norm=1.0)
+    seen = []
+    for _ in range(3):
+        opt.zero_grad()
+        x0 = step()
+        seen.append(x0.detach().clone())
+        torch.nn.functional.l1_loss(x0, tgt).backward()
+        opt.step()
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+    # a model that is given the stepped weights as new ones computes the same
+    fresh = hip_model(SMALL, {k: v.detach().cpu() for k, v in model.state_dict().items()}, 1, max_batch=1)
+    with torch.no_grad():
+        a = step()
+        kw["models"] = fresh
+        assert torch.equal(a, step())
+
+
+@pytest.mark.gpu
+def test_refusals():
+    p = torch.zeros(8, device="cuda", requires_grad=True)
+    for kw in (dict(state_bits=16), dict(max_norm=0.0), dict(max_norm=math.inf), dict(lr=-1.0), dict(lr=math.nan), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1),
+               dict(lr=torch.ones(2))):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    with pytest.raises(ValueError):
+        AdamW([torch.zeros(3, device="cuda", dtype=torch.float64, requires_grad=True)])
+    cpu = torch.zeros(3, requires_grad=True)
+    cpu.grad = torch.ones(3)
+    with pytest.raises(AsyrpDeviceError):
+        AdamW([cpu]).step()
+    bad = torch.zeros(4, 6, device="cuda").t().requires_grad_()
+    bad.grad = torch.ones_like(bad)
+    with pytest.raises(ValueError):
+        AdamW([bad]).step()
+    opt = AdamW([p], lr=torch.tensor(1e-3, device="cuda", dtype=torch.float64))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError):
+        opt.step()
+    opt = AdamW([p])
+    opt.step()
+    p.data = torch.zeros(4, device="cuda")                       # the moments are of eight values
+    p.grad = None
+    p.grad = torch.ones(4, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step()
+
+
+def test_library_refuses_what_its_kernels_do_not_take():
+    import struct
+    from asyrp_official_amd import _lib
+    lib = _lib.load()
+
+    def call(numel=8, at=0, index=0, p=4096, g=4096, n=1, dtype=_lib.F32, lr=1e-3, b1=0.9, eps=1e-8, wd=0.0, steps=4096, sumsq=0, max_norm=0.0, count=0, m=4096, v=4096, me=4096,
+             bits=32, scratch=4096):
+        spec = _lib.ADAMW.pack(lr, b1, 0.999, eps, wd, 0, steps, sumsq, max_norm, 0, m, v, me, me, count, bits, 0)
+        return lib.asyrp_adamw_step(0, spec, struct.pack("5q", p, g, numel, at, index), n, dtype, scratch, None)
+
+    for bad in (dict(numel=-1), dict(at=100), dict(at=-256), dict(index=-1), dict(p=0), dict(g=0), dict(p=4098), dict(g=4097), dict(n=-1), dict(dtype=3), dict(lr=math.nan), dict(b1=1.0),
+                dict(b1=-0.1), dict(eps=-1.0), dict(eps=math.nan), dict(wd=math.inf), dict(steps=0), dict(sumsq=4096), dict(sumsq=4096, max_norm=1.0, count=-1), dict(m=0), dict(v=4104),
+                dict(me=0, bits=8), dict(bits=16), dict(scratch=None), dict(scratch=4100)):
+        assert call(**bad) == -1, bad
+        assert b"AdamW" in lib.asyrp_last_error()
+    one = struct.pack("5q", 4096, 4096, 8, 0, 0)
+    assert lib.asyrp_adamw_step(0, None, one, 1, 0, 4096, None) == -1
+    assert lib.asyrp_grad_sumsq(0, one, 1, 0, None, None) == -1 and lib.asyrp_grad_sumsq(0, None, 1, 0, 4096, None) == -1
+    assert lib.asyrp_adamw_moments(0, 4096, 4096, 4096, 4096, 100, 4096, 4096, None) == -1
+    assert lib.asyrp_adamw_moments(0, None, 4096, 4096, 4096, 256, 4096, 4096, None) == -1
+    assert lib.asyrp_adamw_moments(0, None, None, None, None, 0, None, None, None) == 0
