@@ -601,15 +601,18 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
 }
 
 // The same for heads wider than 64, where one wave cannot hold both sums, its keys' and values' fragments and the scores in half a SIMD's registers, and a
-// wave alone on its SIMD waits out every exponential: eight waves, of which the first four form dk and the others dv of the same 128 keys
-// from the same tiles.  S is formed by both (5 products instead of 4), and in return two waves share each SIMD, one in its products
-// while the other is in its exponentials: 435 us with one wave per SIMD, XXX so (16 query heads on 4, 128 wide, 8192 rows, causal).
+// wave alone on its SIMD waits out every exponential: eight waves, two on each SIMD, share the four products of 128 keys.  The first of a pair forms S and P
+// and sums dv; it hands P over through LDS (as f16 whatever the operands' type: P <= 1, and rounding it like the operands before it multiplies dP would
+// double what dk is off), and the second forms dP and dS and sums dk one tile behind, so that the only wait is the barrier that there is for the
+// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, XXX us so.
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const PackedAttnArgs p) {
-  __shared__ __attribute__((aligned(16))) char qt[2][BN * DP * 2], gt[2][BN * DP * 2];
-  __shared__ __attribute__((aligned(16))) float ls[2][BN], ds[2][BN];
+  __shared__ __attribute__((aligned(16))) char qt[3][BN * DP * 2], gt[3][BN * DP * 2];
+  __shared__ __attribute__((aligned(16))) _Float16 pt[2][4][4][64][8];      // [tile's parity][pair][half of the tile x half of its rows][lane]
+  __shared__ __attribute__((aligned(16))) float ls[3][BN], ds[3][BN];
+  typedef typename Frag<_Float16>::V Half8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, h = lane >> 5;
-  const bool values = __builtin_amdgcn_readfirstlane(tid >> 8);          // this wave forms dv
+  const bool values = __builtin_amdgcn_readfirstlane(tid >> 8);          // this wave forms P and dv, its partner dk
   const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT_FROM_END : IN_ORDER);
   if (f.idle) {
@@ -621,14 +624,10 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   const int row = f.row0 + wave * 32 + (lane & 31);     // this lane's key
   const bool there = row < f.len;
   const long long at = f.start + (there ? row : 0);
-  const T* krow = (const T*)p.k + at * p.k_t + hk * p.k_h;
-  const T* vrow = (const T*)p.v + at * p.v_t + hk * p.v_h;
-  typename Frag<T>::V kf[DP / 16], vf[DP / 16];
+  const T* krow = values ? (const T*)p.k + at * p.k_t + hk * p.k_h : (const T*)p.v + at * p.v_t + hk * p.v_h;
+  typename Frag<T>::V kf[DP / 16];                      // the keys for S, or the values for dP
 #pragma unroll
-  for (int ks = 0; ks < DP / 16; ++ks) {
-    kf[ks] = load_frag<T>(krow, ks, h, p.D, there);
-    vf[ks] = load_frag<T>(vrow, ks, h, p.D, there);
-  }
+  for (int ks = 0; ks < DP / 16; ++ks) kf[ks] = load_frag<T>(krow, ks, h, p.D, there);
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -643,9 +642,9 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   const T* base = values ? (const T*)p.dout + f.start * p.do_t : (const T*)p.q + f.start * p.q_t;
   const long long st = values ? p.do_t : p.q_t, sh = values ? p.do_h : p.q_h;
   float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
-  auto fetch = [&](int i, int buf) {
+  auto fetch = [&](int i, int slot) {
     const int head = hk * G + i / per, q0 = qbeg + (i % per) * BN;
-    ts.load(base + q0 * st + head * sh, f.len - q0, values ? lds_offset(gt[buf]) : lds_offset(qt[buf]), p.D, tid & 255);
+    ts.load(base + q0 * st + head * sh, f.len - q0, values ? lds_offset(gt[slot]) : lds_offset(qt[slot]), p.D, tid & 255);
     if (tid < BN) {
       const long long a = (long long)head * p.T + f.start + min(q0 + tid, f.len - 1);
       lv_ = p.lse[a] * LOG2E;
@@ -653,54 +652,72 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     }
   };
   if (i0 < i1) fetch(i0, 0);
-  int buf = 0;
-  for (int i = i0; i < i1; ++i, buf ^= 1) {
-    const int q0 = qbeg + (i % per) * BN;
-    if (tid < BN) {
-      ls[buf][tid] = lv_;
-      ds[buf][tid] = dl_;
+  // slots of the tile before, of this one and of the next
+  for (int i = i0, prev = 2, cur = 0, next = 1; i <= i1 && i0 < i1; ++i) {
+    if (tid < BN && i < i1) {
+      ls[cur][tid] = lv_;
+      ds[cur][tid] = dl_;
     }
     tile_barrier();
-    if (i + 1 < i1) fetch(i + 1, buf ^ 1);
-    if (p.causal && q0 + BN <= f.row0 + wave * 32) continue;      // every query lies before this wave's keys
-    const bool edge = q0 + BN > f.len || (p.causal && q0 < f.row0 + wave * 32 + 31);
+    if (i + 1 < i1) fetch(i + 1, next);
+    const int mine = values ? i : i - 1, q0 = qbeg + (mine % per) * BN;
+    // (under the causal mask, nothing to do where every query lies before this pair's keys)
+    if (mine >= i0 && mine < i1 && !(p.causal && q0 + BN <= f.row0 + wave * 32)) {
+      if (values) {
+        const bool edge = q0 + BN > f.len || (p.causal && q0 < f.row0 + wave * 32 + 31);
 #pragma unroll
-    for (int n = 0; n < BN / 32; ++n) {
-      f32x16 s, g;
+        for (int n = 0; n < BN / 32; ++n) {
+          f32x16 s;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+          for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(qt[buf], 32 * n, ks, lane), kf[ks], s);
-      if (!values)
+          for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(qt[cur], 32 * n, ks, lane), kf[ks], s);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[buf], 32 * n, ks, lane), vf[ks], g);
+          for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[cur][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * n + 8 * r4 + 4 * h]);
+            for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
+          }
+          if (edge)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
-      }
-      if (!values)
+            for (int r = 0; r < 16; ++r) {
+              const int q = q0 + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
+              if (q >= f.len || (p.causal && q < row)) s[r] = 0.f;
+            }
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[buf][32 * n + 8 * r4 + 4 * h]);
+          for (int b = 0; b < 2; ++b) {
+            *reinterpret_cast<Half8*>(pt[mine & 1][wave][2 * n + b][lane]) = pack8<_Float16>(s, b);
+            const typename Frag<T>::V pf = pack8<T>(s, b);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[4 * r4 + j] *= g[4 * r4 + j] - dl[j];
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(gt[cur], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
+          }
         }
-      if (edge)
+      } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int q = q0 + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-          if (q >= f.len || (p.causal && q < row)) s[r] = 0.f;
+        for (int n = 0; n < BN / 32; ++n) {
+          f32x16 g;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) g[r] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[prev], 32 * n, ks, lane), kf[ks], g);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const Half8 pr = *reinterpret_cast<const Half8*>(pt[mine & 1][wave][2 * n + b][lane]);
+#pragma unroll
+            for (int r4 = 2 * b; r4 < 2 * b + 2; ++r4) {
+              const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[prev][32 * n + 8 * r4 + 4 * h]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) g[4 * r4 + j] = (float)pr[4 * (r4 - 2 * b) + j] * (g[4 * r4 + j] - dl[j]);
+            }
+            const typename Frag<T>::V zf = pack8<T>(g, b);
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(qt[prev], 32 * n + 16 * b, dt, lane), zf, acc[dt]);
+          }
         }
-      const char* from = values ? gt[buf] : qt[buf];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const typename Frag<T>::V pf = pack8<T>(s, b);
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(from, 32 * n + 16 * b, dt, lane), pf, acc[dt]);
       }
     }
+    const int free = prev;
+    prev = cur; cur = next; next = free;
   }
   if (p.parts > 1) {
     if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
