@@ -89,6 +89,9 @@ __device__ __forceinline__ typename Frag<T>::V read_cols(const char* tile, int r
   return u.v;
 }
 
+// Stands in a branch that few tiles take: without it the compiler computes the branch's selects for every tile.
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+
 // one row's fragment from global memory: d = 16 * ks + 8 * h + 0..7, zero beyond D or where the row is not there
 template <typename T>
 __device__ __forceinline__ typename Frag<T>::V load_frag(const T* row, int ks, int h, int D, bool there) {
@@ -453,7 +456,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
   const float sc = p.scale * LOG2E;
   const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
-  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;
+  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
   Tile<T, DP> ks_, vs_;
   ks_.init(p.k_t, f.len, p.D, tid);
   vs_.init(p.v_t, f.len, p.D, tid);
@@ -481,10 +484,12 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], sc, -lse2)) * (g[r] - delta);
-      if (edge)
+      if (edge) {
+        stay_a_branch();
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (32 * n + 8 * (r >> 2) + (r & 3) > last) s[r] = 0.f;
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const typename Frag<T>::V pf = pack8<T>(s, b);
@@ -534,8 +539,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   qs.init(p.q_t, f.len - qbeg, p.D, tid);
   gs.init(p.do_t, f.len - qbeg, p.D, tid);
   float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
-  auto fetch = [&](int i, int buf) {
-    const int head = hk * G + i / per, q0 = qbeg + (i % per) * BN;
+  int head = hk * G + i0 / per, q0 = qbeg + i0 % per * BN;      // of the tile that is fetched next
+  auto fetch = [&](int buf) {
     qs.load((const T*)p.q + (f.start + q0) * p.q_t + head * p.q_h, f.len - q0, lds_offset(qt[buf]), p.D, tid);
     gs.load((const T*)p.dout + (f.start + q0) * p.do_t + head * p.do_h, f.len - q0, lds_offset(gt[buf]), p.D, tid);
     if (tid < BN) {
@@ -544,18 +549,24 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
       dl_ = p.delta[a];
     }
   };
-  if (i0 < i1) fetch(i0, 0);
+  if (i0 < i1) fetch(0);
   int buf = 0;
   for (int i = i0; i < i1; ++i, buf ^= 1) {
-    const int q0 = qbeg + (i % per) * BN;
+    const int at0 = q0;                                 // first query of this tile
     if (tid < BN) {
       ls[buf][tid] = lv_;
       ds[buf][tid] = dl_;
     }
     tile_barrier();
-    if (i + 1 < i1) fetch(i + 1, buf ^ 1);
-    if (p.causal && q0 + BN <= f.row0 + wave * 32) continue;      // every query lies before this wave's keys
-    const bool edge = q0 + BN > f.len || (p.causal && q0 < f.row0 + wave * 32 + 31);
+    q0 += BN;
+    if (q0 >= f.len) {
+      q0 = qbeg;
+      ++head;
+    }
+    if (i + 1 < i1) fetch(buf ^ 1);
+    // queries that see this lane's key: from `first` on, `seen` of them
+    const int first = (p.causal ? row : 0) - at0 - 4 * h, seen = f.len - (p.causal ? row : 0);
+    const bool edge = at0 + BN > f.len || (p.causal && at0 < f.row0 + wave * 32 + 31);
 #pragma unroll
     for (int n = 0; n < BN / 32; ++n) {
       f32x16 s, g;
@@ -569,15 +580,20 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * n + 8 * r4 + 4 * h]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
+      }
+      if (edge) {
+        stay_a_branch();
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if ((unsigned)(32 * n + 8 * (r >> 2) + (r & 3) - first) >= (unsigned)seen) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
         const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[buf][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * r4 + j, q = q0 + 32 * n + 8 * r4 + 4 * h + j;
-          float e = exp2_fast(__builtin_fmaf(s[r], sc, -lv[j]));
-          if (edge && (q >= f.len || (p.causal && q < row))) e = 0.f;
-          s[r] = e;
-          g[r] = e * (g[r] - dl[j]);
-        }
+        for (int j = 0; j < 4; ++j) g[4 * r4 + j] = s[4 * r4 + j] * (g[4 * r4 + j] - dl[j]);
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -642,8 +658,8 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   const T* base = values ? (const T*)p.dout + f.start * p.do_t : (const T*)p.q + f.start * p.q_t;
   const long long st = values ? p.do_t : p.q_t, sh = values ? p.do_h : p.q_h;
   float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
-  auto fetch = [&](int i, int slot) {
-    const int head = hk * G + i / per, q0 = qbeg + (i % per) * BN;
+  int head = hk * G + i0 / per, q0 = qbeg + i0 % per * BN;      // of the tile that is fetched next
+  auto fetch = [&](int slot) {
     ts.load(base + q0 * st + head * sh, f.len - q0, values ? lds_offset(gt[slot]) : lds_offset(qt[slot]), p.D, tid & 255);
     if (tid < BN) {
       const long long a = (long long)head * p.T + f.start + min(q0 + tid, f.len - 1);
@@ -651,73 +667,93 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
       dl_ = p.delta[a];
     }
   };
-  if (i0 < i1) fetch(i0, 0);
-  // slots of the tile before, of this one and of the next
-  for (int i = i0, prev = 2, cur = 0, next = 1; i <= i1 && i0 < i1; ++i) {
+  if (i0 < i1) fetch(0);
+  int prev = 2, cur = 0, next = 1;                      // slots of the tile before, of this one and of the next
+  int here = q0;                                        // first query of this one
+  // the barrier of tile i, and behind it the loads of the next one
+  auto begin = [&](int i) {
     if (tid < BN && i < i1) {
       ls[cur][tid] = lv_;
       ds[cur][tid] = dl_;
     }
     tile_barrier();
-    if (i + 1 < i1) fetch(i + 1, next);
-    const int mine = values ? i : i - 1, q0 = qbeg + (mine % per) * BN;
-    // (under the causal mask, nothing to do where every query lies before this pair's keys)
-    if (mine >= i0 && mine < i1 && !(p.causal && q0 + BN <= f.row0 + wave * 32)) {
-      if (values) {
-        const bool edge = q0 + BN > f.len || (p.causal && q0 < f.row0 + wave * 32 + 31);
-#pragma unroll
-        for (int n = 0; n < BN / 32; ++n) {
-          f32x16 s;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(qt[cur], 32 * n, ks, lane), kf[ks], s);
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[cur][32 * n + 8 * r4 + 4 * h]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
-          }
-          if (edge)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int q = q0 + 32 * n + 8 * (r >> 2) + 4 * h + (r & 3);
-              if (q >= f.len || (p.causal && q < row)) s[r] = 0.f;
-            }
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            *reinterpret_cast<Half8*>(pt[mine & 1][wave][2 * n + b][lane]) = pack8<_Float16>(s, b);
-            const typename Frag<T>::V pf = pack8<T>(s, b);
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(gt[cur], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < BN / 32; ++n) {
-          f32x16 g;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) g[r] = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[prev], 32 * n, ks, lane), kf[ks], g);
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const Half8 pr = *reinterpret_cast<const Half8*>(pt[mine & 1][wave][2 * n + b][lane]);
-#pragma unroll
-            for (int r4 = 2 * b; r4 < 2 * b + 2; ++r4) {
-              const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[prev][32 * n + 8 * r4 + 4 * h]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) g[4 * r4 + j] = (float)pr[4 * (r4 - 2 * b) + j] * (g[4 * r4 + j] - dl[j]);
-            }
-            const typename Frag<T>::V zf = pack8<T>(g, b);
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(qt[prev], 32 * n + 16 * b, dt, lane), zf, acc[dt]);
-          }
-        }
-      }
+    here = q0;
+    q0 += BN;
+    if (q0 >= f.len) {
+      q0 = qbeg;
+      ++head;
     }
+    if (i + 1 < i1) fetch(next);
+  };
+  auto end = [&] {
     const int free = prev;
     prev = cur; cur = next; next = free;
+  };
+  // (each kind of wave has its loop, so that its sums stay where they are; both pass the barriers of i0 .. i1)
+  if (i0 < i1 && values) {
+    for (int i = i0; i < i1; ++i) {
+      begin(i);
+      // queries that see this lane's key: from `first` on, `seen` of them
+      const int first = (p.causal ? row : 0) - here - 4 * h, seen = f.len - (p.causal ? row : 0);
+      const bool edge = here + BN > f.len || (p.causal && here < f.row0 + wave * 32 + 31);
+#pragma unroll
+      for (int n = 0; n < BN / 32; ++n) {
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(qt[cur], 32 * n, ks, lane), kf[ks], s);
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[cur][32 * n + 8 * r4 + 4 * h]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
+        }
+        if (edge) {
+          stay_a_branch();
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((unsigned)(32 * n + 8 * (r >> 2) + (r & 3) - first) >= (unsigned)seen) s[r] = 0.f;
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          *reinterpret_cast<Half8*>(pt[i & 1][wave][2 * n + b][lane]) = pack8<_Float16>(s, b);
+          const typename Frag<T>::V pf = pack8<T>(s, b);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(gt[cur], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
+        }
+      }
+      end();
+    }
+    begin(i1);
+  } else if (i0 < i1) {
+    begin(i0);
+    end();
+    for (int i = i0; i < i1; ++i) {
+      begin(i + 1);
+#pragma unroll
+      for (int n = 0; n < BN / 32; ++n) {
+        f32x16 g;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) g[r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[prev], 32 * n, ks, lane), kf[ks], g);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const Half8 pr = *reinterpret_cast<const Half8*>(pt[i & 1][wave][2 * n + b][lane]);
+#pragma unroll
+          for (int r4 = 2 * b; r4 < 2 * b + 2; ++r4) {
+            const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[prev][32 * n + 8 * r4 + 4 * h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[4 * r4 + j] = (float)pr[4 * (r4 - 2 * b) + j] * (g[4 * r4 + j] - dl[j]);
+          }
+          const typename Frag<T>::V zf = pack8<T>(g, b);
+#pragma unroll
+          for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(qt[prev], 32 * n + 16 * b, dt, lane), zf, acc[dt]);
+        }
+      }
+      end();
+    }
   }
   if (p.parts > 1) {
     if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
