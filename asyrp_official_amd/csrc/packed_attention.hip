@@ -311,9 +311,61 @@ __device__ __forceinline__ typename Frag<T>::V pack8(const f32x16& s, int half) 
   return v;
 }
 
+// What a wave of the forward carries from one half tile (32 keys) to the next
+template <typename T, int DP>
+struct FwdWave {
+  typename Frag<T>::V qf[DP / 16];
+  f32x16 acc[DP / 32];
+  float m, l, mx;            // reference and sum of each column, and the maximum of the next half's scores, in the scores' own units
+  float sc;
+
+  __device__ __forceinline__ void scores(f32x16& s, const char* k, int row0, int lane) const {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(k, row0, ks, lane), qf[ks], s);
+  }
+  __device__ __forceinline__ void maximum(const f32x16& s) {
+    float a = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) a = fmaxf(a, s[r]);
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(a), false, false);
+    mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+  }
+  // Half a tile: the exponentials and sums of `cur` (values from row `vrow` of `v` on) together with the scores `next` of the half behind it (keys from row
+  // `krow` of `k` on), so that one's products run under the other's exponentials.
+  __device__ __forceinline__ void half(f32x16& cur, f32x16& next, const char* k, int krow, const char* v, int vrow, int lane) {
+    // The reference moves only where a column's maximum has outgrown it by 8 powers of two (and in the first half): the exponentials stay under
+    // 2^8, well inside f16, and most halves leave the sums as they are.
+    if (__any(!((mx - m) * sc <= 8.f))) {
+      const float mn = fmaxf(m, mx), keep = m > -INFINITY ? exp2_fast((m - mn) * sc) : 0.f;
+      m = mn;
+      l *= keep;
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
+    }
+    const float ms = m > -INFINITY ? m * sc : 0.f;      // keys of minus infinity so far: their exponentials are zeros
+    scores(next, k, krow, lane);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int r = 8 * b; r < 8 * b + 8; ++r) {
+        cur[r] = exp2_fast(__builtin_fmaf(cur[r], sc, -ms));
+        l += cur[r];
+      }
+      const typename Frag<T>::V pf = pack8<T>(cur, b);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(v, vrow + 16 * b, dt, lane), pf, acc[dt]);
+    }
+    maximum(next);
+  }
+};
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAttnArgs p) {
-  __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
+  __shared__ __attribute__((aligned(16))) char kt[3][BN * DP * 2], vt[2][BN * DP * 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int head = blockIdx.x % p.Hq, tile = blockIdx.x / p.Hq;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT : IN_ORDER);
@@ -328,83 +380,69 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   const bool there = row < f.len;
   const T* qrow = (const T*)p.q + (f.start + (there ? row : 0)) * p.q_t + head * p.q_h;
   const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
-  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
+  // keys that all of this wave's queries see, in whole tiles, and keys that it has to look at
+  const int open = (p.causal ? min(f.len, f.row0 + wave * 32 + 1) : f.len) / BN * BN;
+  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;
   Tile<T, DP> ks_, vs_;
   ks_.init(p.k_t, f.len, p.D, tid);
   vs_.init(p.v_t, f.len, p.D, tid);
   ks_.load(k, f.len, lds_offset(kt[0]), p.D, tid);
   vs_.load(v, f.len, lds_offset(vt[0]), p.D, tid);
-  typename Frag<T>::V qf[DP / 16];
+  if (BN < kend) ks_.load(k + BN * p.k_t, f.len - BN, lds_offset(kt[1]), p.D, tid);
+  FwdWave<T, DP> w;
 #pragma unroll
-  for (int ks = 0; ks < DP / 16; ++ks) qf[ks] = load_frag<T>(qrow, ks, h, p.D, there);
-
-  f32x16 acc[DP / 32];
+  for (int ks = 0; ks < DP / 16; ++ks) w.qf[ks] = load_frag<T>(qrow, ks, h, p.D, there);
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
-  float m = -INFINITY, l = 0.f;                         // reference and sum, in the scores' own units and of this lane's rows
-  const float sc = p.scale * LOG2E;
-  int buf = 0;
-  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
+    for (int r = 0; r < 16; ++r) w.acc[dt][r] = 0.f;
+  w.m = -INFINITY;
+  w.l = 0.f;
+  w.sc = p.scale * LOG2E;
+  f32x16 s0, s1;
+  tile_barrier();
+  w.scores(s0, kt[0], 0, lane);
+  w.maximum(s0);
+  int k0 = 0, ka = 0, kb = 1, kc = 2, vb = 0;           // key tiles of this, the next and the next but one; parity of the value tile
+  // Loads of the tiles behind: the keys run one tile ahead of the values, since a tile's last scores are those of the next one's first half
+  auto fetch = [&] {
+    if (k0 + 2 * BN < kend) ks_.load(k + (long long)(k0 + 2 * BN) * p.k_t, f.len - k0 - 2 * BN, lds_offset(kt[kc]), p.D, tid);
+    if (k0 + BN < kend) vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(vt[vb ^ 1]), p.D, tid);
+  };
+  auto advance = [&] {
+    const int t = ka;
+    ka = kb; kb = kc; kc = t;
+    vb ^= 1;
+    k0 += BN;
     tile_barrier();
-    if (k0 + BN < kend) {
-      ks_.load(k + (long long)(k0 + BN) * p.k_t, f.len - k0 - BN, lds_offset(kt[buf ^ 1]), p.D, tid);
-      vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(vt[buf ^ 1]), p.D, tid);
-    }
-    if (k0 >= wend) continue;
-    f32x16 s[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) s[n] = Frag<T>::mma(read_rows<T, DP>(kt[buf], 32 * n, ks, lane), qf[ks], s[n]);
-    }
-    if (k0 + BN > f.len || (p.causal && k0 + BN - 1 > f.row0 + wave * 32)) {
+  };
+  while (k0 < open) {
+    fetch();
+    w.half(s0, s1, kt[ka], 32, vt[vb], 0, lane);
+    w.half(s1, s0, kt[kb], 0, vt[vb], 32, lane);        // (behind the last tile: scores of nothing, which nobody reads)
+    advance();
+  }
+  while (k0 < kend) {                                   // tiles that end or are cut by the mask
+    fetch();
+    if (k0 < wend) {
       const int last = (p.causal ? min(row, f.len - 1) : f.len - 1) - k0 - 4 * h;    // the last key this column sees
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) > last) s0[r] = -INFINITY;
+      w.maximum(s0);
+      w.half(s0, s1, kt[ka], 32, vt[vb], 0, lane);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * n + 8 * (r >> 2) + (r & 3) > last) s[n][r] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (32 + 8 * (r >> 2) + (r & 3) > last) s1[r] = -INFINITY;
+      w.maximum(s1);
+      w.half(s1, s0, kt[kb], 0, vt[vb], 32, lane);
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-    mx = both_halves_max(mx);
-    // The reference moves only where a column's maximum has outgrown it by 8 powers of two (and in the first tile): the exponentials stay under
-    // 2^8, well inside f16, and most tiles leave the sums as they are.
-    if (__any(!((mx - m) * sc <= 8.f))) {
-      const float mn = fmaxf(m, mx), keep = m > -INFINITY ? exp2_fast((m - mn) * sc) : 0.f;
-      m = mn;
-      l *= keep;
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
-    }
-    const float ms = m > -INFINITY ? m * sc : 0.f;      // keys of minus infinity so far: their exponentials are zeros
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int r = 8 * b; r < 8 * b + 8; ++r) {
-          s[n][r] = exp2_fast(__builtin_fmaf(s[n][r], sc, -ms));
-          l += s[n][r];
-        }
-        const typename Frag<T>::V pf = pack8<T>(s[n], b);
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(vt[buf], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
-      }
+    advance();
   }
-  l = both_halves_sum(l);
-  store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, acc, 1.0f / l, h, p.D, there,
+  const float l = both_halves_sum(w.l);
+  store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, w.acc, 1.0f / l, h, p.D, there,
                     p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
-  if (there && p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (m * sc + log2f(l)) * LN2;
+  if (there && p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (w.m * w.sc + log2f(l)) * LN2;
 }
 
 // dq, and delta = rowsum(do * o) for the other kernel
