@@ -853,7 +853,7 @@ hipError_t launch(const PackedAttnArgs& a, bool backward, hipStream_t s) {
 int dkv_parts(long long T, int nseq, int Hq, int Hkv) {
   const long long wgs = std::max<long long>(1, T / BM) * Hkv;       // full tiles; the ragged ones are light
   int parts = 1;
-  while (parts < 8 && wgs * parts < 1024 && T / nseq * (Hq / Hkv) >= 1024LL * parts) parts *= 2;
+  while (parts < 8 && wgs * parts < 512 && T / nseq * (Hq / Hkv) >= 1024LL * parts) parts *= 2;
   return parts;
 }
 

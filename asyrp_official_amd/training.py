@@ -7,13 +7,15 @@ The reference trains `layer_0` with
 with `requires_grad` switched on for the DeltaBlock parameters only (:282-290).  Here the same lines keep working: when
 gradients are enabled and a DeltaBlock parameter requires grad, `asyrp_official_amd.denoising_step` routes the step through
 `AsyrpTrainStep`, an autograd node whose backward runs the engine's decoder-#2 backward pass (asyrp_train_backward) and hands
-autograd the gradients of the DeltaBlock parameters.  The loss (CLIP, L1, id) and the optimiser stay in PyTorch.
+autograd the gradients of the DeltaBlock parameters.  The loss (CLIP, L1, id) stays in PyTorch; `training.AdamW` steps the
+DeltaBlock (or any parameters) in a few launches, and any torch optimiser does as well.
 """
 import weakref
 
 import torch
 
 from .engine import alphas_cumprod_from_betas
+from .optim import AdamW  # noqa: F401
 
 
 def delta_block_params(model, index=0):

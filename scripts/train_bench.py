@@ -3,7 +3,9 @@
 CLIP network): CelebA-HQ 256x256 DDPM, seeded random-init weights, the reference's loop shape
     optim.zero_grad(); denoising_step(..., index=0, t_edit=...); loss(x0_t).backward(); optim.step()
 timed per step with the stream synchronised on both sides, next to the inference step that computes the same forward.
-The reference trains with bs_train = 1 (diffusion_latent.py:1010).  usage: scripts/train_bench.py [B ...]"""
+The reference trains with bs_train = 1 (diffusion_latent.py:1010).
+usage: scripts/train_bench.py [--optimizer sgd|adamw|adamw8] [B ...]     (adamw, adamw8: the package's own, moments in 32 / 8 bits)"""
+import argparse
 import json
 import os
 import sys
@@ -13,12 +15,16 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tests"))
 import torch
 
-from asyrp_official_amd import denoising_step
+from asyrp_official_amd import AdamW, denoising_step
 from oracle import sampler as osamp          # schedule helper only (a benchmark script, like bench.py's cpu_baseline leg)
 from oracle.weights import CELEBA, hash_normal
 from util_models import hip_model, synthetic
 
-batches = [int(v) for v in sys.argv[1:]] or [1, 4, 8]
+ap = argparse.ArgumentParser()
+ap.add_argument("--optimizer", choices=("sgd", "adamw", "adamw8"), default="sgd")
+ap.add_argument("batches", nargs="*", type=int)
+args = ap.parse_args()
+batches = args.batches or [1, 4, 8]
 b = osamp.beta_schedule().cuda()
 out = []
 for B in batches:
@@ -27,7 +33,8 @@ for B in batches:
         p.requires_grad = False
     for p in m.layer_0.parameters():
         p.requires_grad = True
-    opt = torch.optim.SGD(list(m.layer_0.parameters()), lr=1e-4)
+    params = list(m.layer_0.parameters())
+    opt = torch.optim.SGD(params, lr=1e-4) if args.optimizer == "sgd" else AdamW(params, lr=1e-4, state_bits=8 if args.optimizer == "adamw8" else 32, max_norm=1.0)
     x = hash_normal("celeba.x", (B, 3, 256, 256), seed=1234).cuda()
     tgt = hash_normal("train.tgt256", (B, 3, 256, 256), seed=5).cuda()
     one = torch.ones(B, device="cuda")
@@ -43,7 +50,7 @@ for B in batches:
         with torch.no_grad():
             denoising_step(x, t=one * 768.0, t_next=one * 743.0, **kw)
 
-    res = {"B": B}
+    res = {"B": B, "optimizer": args.optimizer}
     for name, fn, n in (("train_step_ms", train_step, 10), ("inference_dual_step_ms", infer_step, 10)):
         for _ in range(3):
             fn()
