@@ -8,7 +8,7 @@ Inputs (x0, weights) are resident in HBM before the timed region; synthetic data
 weights of the reference architecture (no checkpoints offline).
 
   python bench.py [--gpus N] [--steps K] [--warmup W] [--batch B]
-      N > 1 without a launcher: bench.py re-executes itself under torch.distributed.run with N ranks
+      N > 1 without a launcher: bench.py runs itself under torch.distributed.run with N ranks
       (one process per GPU, RCCL), and fails loudly when fewer than N GPUs are visible.
   python -m torch.distributed.run --nproc-per-node N ... bench.py --gpus N ...   (the driver's form)
 
@@ -19,6 +19,7 @@ import argparse
 import json
 import os
 import socket
+import subprocess
 import sys
 import time
 from argparse import Namespace
@@ -175,7 +176,8 @@ def _free_port():
 
 
 def _self_launch(n):
-    """`python bench.py --gpus N` without a launcher: become `torch.distributed.run` with N ranks on this node."""
+    """`python bench.py --gpus N` without a launcher: run `torch.distributed.run` with N ranks on this node as a child process (this one has
+    initialised the GPU and must not be replaced by another program) and end with its exit status."""
     backend = os.environ.get("ASYRP_BENCH_BACKEND", "nccl")
     have = torch.cuda.device_count()
     if backend == "nccl" and have < n:
@@ -185,7 +187,7 @@ def _self_launch(n):
     env["ASYRP_BENCH_SELF_LAUNCHED"] = "1"
     cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={n}", "--master-addr", "127.0.0.1",
            "--master-port", str(_free_port()), os.path.abspath(__file__)] + sys.argv[1:]
-    os.execvpe(cmd[0], cmd, env)
+    sys.exit(subprocess.run(cmd, env=env).returncode)
 
 
 def paste_traffic(res, tpath, lib_path, dt, steps):

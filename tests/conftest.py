@@ -19,6 +19,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+def pytest_collection_modifyitems(items):
+    """An empty /root/reference is as good as none: the test that imports a module of the reference's says so itself only where the folder is missing."""
+    if os.path.isdir("/root/reference") and not os.listdir("/root/reference"):
+        for item in items:
+            if item.name == "test_vendored_class_schedule_tables_and_helpers_match_the_reference":
+                item.add_marker(pytest.mark.skip(reason="reference not present"))
+
+
 sys.path.insert(0, GOLDEN)
 import compact  # noqa: E402  (tests/golden/compact.py: which arrays are stored whole, which as samples, the shared DeltaBlock weights)
 
