@@ -311,6 +311,23 @@ __device__ __forceinline__ typename Frag<T>::V pack8(const f32x16& s, int half) 
   return v;
 }
 
+// sums += A * dS for 16 rows of a tile.  dS is rounded to the operands' type, except in the tiles that the mask cuts or the sequence ends in: there it
+// goes in as two terms (its rounded value and the rest).  Under the causal mask those tiles hold the rows with few keys, whose dS is largest, and most
+// of what dq and dk would be off; all others are many to one of them.
+template <typename T, int DP>
+__device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const char* tile, int row0, const f32x16& ds, int half, bool two_terms, int lane) {
+  const typename Frag<T>::V hi = pack8<T>(ds, half);
+  if (two_terms) {
+    typename Frag<T>::V lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lo[j] = (T)(ds[8 * half + j] - (float)hi[j]);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(tile, row0, dt, lane), lo, acc[dt]);
+  }
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(tile, row0, dt, lane), hi, acc[dt]);
+}
+
 // What a wave of the forward carries from one half tile (32 keys) to the next
 template <typename T, int DP>
 struct FwdWave {
@@ -530,9 +547,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const typename Frag<T>::V pf = pack8<T>(s, b);
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(kt[buf], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
+        add_ds<T, DP>(acc, kt[buf], 32 * n + 16 * b, s, b, edge, lane);
       }
     }
   }
@@ -635,12 +650,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const typename Frag<T>::V pf = pack8<T>(s, b), zf = pack8<T>(g, b);
+        const typename Frag<T>::V pf = pack8<T>(s, b);
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) {
-          dv[dt] = Frag<T>::mma(read_cols<T, DP>(gt[buf], 32 * n + 16 * b, dt, lane), pf, dv[dt]);
-          dk[dt] = Frag<T>::mma(read_cols<T, DP>(qt[buf], 32 * n + 16 * b, dt, lane), zf, dk[dt]);
-        }
+        for (int dt = 0; dt < DP / 32; ++dt) dv[dt] = Frag<T>::mma(read_cols<T, DP>(gt[buf], 32 * n + 16 * b, dt, lane), pf, dv[dt]);
+        add_ds<T, DP>(dk, qt[buf], 32 * n + 16 * b, g, b, edge, lane);
       }
     }
   }
@@ -654,17 +667,38 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   }
 }
 
+// P in 16 bits on its way from one wave to another, finer than the operands' type, so that dS is rounded once in effect.  For bf16 operands f16 is; for f16
+// ones P, which is never negative nor over 1 (and a rounding), takes four bits of exponent and twelve of mantissa (2^-13 of its value, from 2^-15 on).
+template <typename T> struct Handed;
+template <> struct Handed<__bf16> {
+  typedef Frag<_Float16>::V V;
+  static __device__ __forceinline__ V pack(const f32x16& s, int half) { return pack8<_Float16>(s, half); }
+  static __device__ __forceinline__ float get(const V& v, int j) { return (float)v[j]; }
+};
+template <> struct Handed<_Float16> {
+  typedef unsigned V __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ unsigned bits(float p) { return __float_as_uint(p * 0x1p-112f) + 0x400u; }      // exponents 0 .. 15, eleven bits to go
+  static __device__ __forceinline__ V pack(const f32x16& s, int half) {
+    V v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = bits(s[8 * half + 2 * j]) >> 11 | (bits(s[8 * half + 2 * j + 1]) & ~0x7ffu) << 5;
+    return v;
+  }
+  static __device__ __forceinline__ float get(const V& v, int j) {
+    return __uint_as_float(j & 1 ? v[j / 2] >> 5 & ~0x7ffu : (v[j / 2] & 0xffffu) << 11) * 0x1p112f;
+  }
+};
+
 // The same for heads wider than 64, where one wave cannot hold both sums, its keys' and values' fragments and the scores in half a SIMD's registers, and a
 // wave alone on its SIMD waits out every exponential: eight waves, two on each SIMD, share the four products of 128 keys.  The first of a pair forms S and P
-// and sums dv; it hands P over through LDS (as f16 whatever the operands' type: P <= 1, and rounding it like the operands before it multiplies dP would
-// double what dk is off), and the second forms dP and dS and sums dk one tile behind, so that the only wait is the barrier that there is for the
+// and sums dv; it hands P over through LDS, and the second forms dP and dS and sums dk one tile behind, so that the only wait is the barrier that there is for the
 // tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, XXX us so.
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char qt[3][BN * DP * 2], gt[3][BN * DP * 2];
-  __shared__ __attribute__((aligned(16))) _Float16 pt[2][4][4][64][8];      // [tile's parity][pair][half of the tile x half of its rows][lane]
+  typedef Handed<T> Pass;
+  __shared__ typename Pass::V pt[2][4][4][64];          // [tile's parity][pair][half of the tile x half of its rows][lane]
   __shared__ __attribute__((aligned(16))) float ls[3][BN], ds[3][BN];
-  typedef typename Frag<_Float16>::V Half8;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, h = lane >> 5;
   const bool values = __builtin_amdgcn_readfirstlane(tid >> 8);          // this wave forms P and dv, its partner dk
   const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
@@ -755,7 +789,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          *reinterpret_cast<Half8*>(pt[i & 1][wave][2 * n + b][lane]) = pack8<_Float16>(s, b);
+          pt[i & 1][wave][2 * n + b][lane] = Pass::pack(s, b);
           const typename Frag<T>::V pf = pack8<T>(s, b);
 #pragma unroll
           for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(gt[cur], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
@@ -768,6 +802,8 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     begin(i0);
     end();
     for (int i = i0; i < i1; ++i) {
+      const int before = here;
+      const bool edge = before + BN > f.len || (p.causal && before < f.row0 + wave * 32 + 31);
       begin(i + 1);
 #pragma unroll
       for (int n = 0; n < BN / 32; ++n) {
@@ -778,16 +814,14 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
         for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[prev], 32 * n, ks, lane), kf[ks], g);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const Half8 pr = *reinterpret_cast<const Half8*>(pt[i & 1][wave][2 * n + b][lane]);
+          const typename Pass::V pr = pt[i & 1][wave][2 * n + b][lane];
 #pragma unroll
           for (int r4 = 2 * b; r4 < 2 * b + 2; ++r4) {
             const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[prev][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g[4 * r4 + j] = (float)pr[4 * (r4 - 2 * b) + j] * (g[4 * r4 + j] - dl[j]);
+            for (int j = 0; j < 4; ++j) g[4 * r4 + j] = Pass::get(pr, 4 * (r4 - 2 * b) + j) * (g[4 * r4 + j] - dl[j]);
           }
-          const typename Frag<T>::V zf = pack8<T>(g, b);
-#pragma unroll
-          for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(qt[prev], 32 * n + 16 * b, dt, lane), zf, acc[dt]);
+          add_ds<T, DP>(acc, qt[prev], 32 * n + 16 * b, g, b, edge, lane);
         }
       }
       end();

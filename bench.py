@@ -294,7 +294,7 @@ def engine_device_index(local_rank, backend, ndev):
 
 
 def _setup_ranks(a, need_gpu):
-    """Launcher contract: `python bench.py --gpus N` re-executes itself under torch.distributed.run (one rank per GPU); a rank reads
+    """Launcher contract: `python bench.py --gpus N` runs itself under torch.distributed.run (one rank per GPU); a rank reads
     RANK / LOCAL_RANK / WORLD_SIZE / MASTER_* from the environment and joins the process group (nccl = RCCL; gloo = dry run)."""
     if "WORLD_SIZE" not in os.environ and a.gpus > 1:
         _self_launch(a.gpus)            # does not return
@@ -539,7 +539,7 @@ def main():
                              "fp32-equivalent - see parity_check for its measured error)"}[a.conv_math], "data": "synthetic (seeded U[-1,1) images, seeded random-init weights)",
             "config": {"workload": workload, "baseline_config": baseline_cfg,
                        "batch_per_gpu": B, "parallelism": f"dp{world} (batch sharded, one all-gather of x_edit)",
-                       "launcher": "self (bench.py re-executed under torch.distributed.run)"
+                       "launcher": "self (bench.py started under torch.distributed.run)"
                        if os.environ.get("ASYRP_BENCH_SELF_LAUNCHED") else ("torch.distributed.run" if world > 1 else "single process"),
                        "collective_backend": (backend if world > 1 else None),
                        # proof that the collective library saw N ranks (a SCALE record is judged on this)
