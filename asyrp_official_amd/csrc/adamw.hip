@@ -15,7 +15,11 @@
 // power of two so that it moves a value's place only by whole exponents and values that did not change are not rounded anew when it
 // changes.  A second moment of a block that holds anything is never kept as zero (the smallest code is 1): the next first moment is at least
 // as coarse, so no quotient of the two can grow beyond its block's.  An exponent byte of 0 is a block of zeros; 255 one that held a value that is
-// not finite, and reads as NaN.  The random bits are a hash of the value's place, the step and the caller's seed.
+// not finite, and reads as NaN.
+//
+// 36.6 M fp32 values with 32-bit moments: 170 us (6.0 TB/s of its 1.03 GB).  146 M with 8-bit ones: 435 us (5.4 TB/s of 2.34 GB; 540 us while the codes were
+// taken apart in branches and the largest value found through LDS); their moments as fp32 240 us (6.1 TB/s); the norm 4.0 TB/s, what reading alone
+// reaches on this card.  The random bits are a hash of the value's place, the step and the caller's seed.
 #include "kernels.h"
 #include "../../include/asyrp.h"
 

