@@ -18,7 +18,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <string>
 
 namespace asyrp {
 
@@ -901,7 +900,7 @@ int dkv_parts(long long T, int nseq, int Hq, int Hkv) {
   return parts;
 }
 
-int refuse(const std::string& m) { return set_last_error(ASYRP_EINVAL, m.c_str()); }
+int refuse(const char* m) { return set_last_error(ASYRP_EINVAL, m); }
 
 // the checks that both directions share; 0 or the error
 int check(const PackedAttnArgs& a, int dtype, const long long* strides, int n) {

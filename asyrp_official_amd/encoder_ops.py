@@ -4,7 +4,8 @@ The reference's loss runs an image and a text encoder around the DeltaBlock step
 attention and the seams between their residual blocks are the work there that is not a plain matrix product:
   packed_attention      attention over sequences packed behind each other, causal or not, with grouped key / value heads
   gated_residual_norm   norm behind a block, gate, residual sum with its scale, norm in front of the next block
-Both run on the current stream of their tensors' device, keep nothing between calls, and may be captured into a graph.
+Both run on the current stream of their tensors' device, keep nothing between calls, and may be captured into a graph.  (As with any autograd function: while a
+backward pass is captured, no graph of the same leaves that was built outside the capture may be alive.)
 """
 import math
 

@@ -121,6 +121,8 @@ class AdamW(torch.optim.Optimizer):
         for p in g["params"]:
             if not p.is_contiguous():
                 raise ValueError("parameters must be contiguous")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the moments have to be there before a step is captured (every replay would start from new ones): step once or call prepare() first")
         mo = _Moments(g["params"], self.state_bits, device)
         for i, p in enumerate(mo.params):                 # moments that are there already: loaded ones, or those of an unpickled copy
             views, old = mo.views(i), self.state.get(p) or {}

@@ -326,6 +326,22 @@ def test_a_captured_step_counts_and_follows_a_rate_on_the_device():
 
 
 @pytest.mark.gpu
+def test_a_first_step_is_not_captured():
+    ps = params_of(tensors([(100,)]))
+    ps[0].grad = torch.ones_like(ps[0])
+    opt = AdamW(ps)
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)                       # a graph of nothing is a warning
+        with pytest.raises(RuntimeError):
+            opt.step()
+    assert torch.equal(ps[0].detach().cpu(), tensors([(100,)])[0])
+    opt.step()
+    assert int(opt.state[ps[0]]["step"]) == 1
+
+
+@pytest.mark.gpu
 def test_another_stream_and_two_optimisers_at_once():
     a, pa = trained(8)
     side = torch.cuda.Stream()
