@@ -402,8 +402,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   const T* qrow = (const T*)p.q + (f.start + (there ? row : 0)) * p.q_t + head * p.q_h;
   const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
   // keys that all of this wave's queries see, in whole tiles, and keys that it has to look at
-  const int open = (p.causal ? min(f.len, f.row0 + wave * 32 + 1) : f.len) / BN * BN;
-  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;
+  const bool empty = f.row0 + wave * 32 >= f.len;       // a wave behind the sequence's end only loads
+  const int open = empty ? 0 : (p.causal ? min(f.len, f.row0 + wave * 32 + 1) : f.len) / BN * BN;
+  const int wend = empty ? 0 : p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;
   Tile<T, DP> ks_, vs_;
   ks_.init(p.k_t, f.len, p.D, tid);
   vs_.init(p.v_t, f.len, p.D, tid);
@@ -452,11 +453,13 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
         if (8 * (r >> 2) + (r & 3) > last) s0[r] = -INFINITY;
       w.maximum(s0);
       w.half(s0, s1, kt[ka], 32, vt[vb], 0, lane);
+      if (k0 + 32 < wend) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (32 + 8 * (r >> 2) + (r & 3) > last) s1[r] = -INFINITY;
-      w.maximum(s1);
-      w.half(s1, s0, kt[kb], 0, vt[vb], 32, lane);
+        for (int r = 0; r < 16; ++r)
+          if (32 + 8 * (r >> 2) + (r & 3) > last) s1[r] = -INFINITY;
+        w.maximum(s1);
+        w.half(s1, s0, kt[kb], 0, vt[vb], 32, lane);
+      }
     }
     advance();
   }
@@ -516,7 +519,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
   const float sc = p.scale * LOG2E;
   const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
-  const int wend = p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
+  const int wend = f.row0 + wave * 32 >= f.len ? 0 : p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
   Tile<T, DP> ks_, vs_;
   ks_.init(p.k_t, f.len, p.D, tid);
   vs_.init(p.v_t, f.len, p.D, tid);
@@ -534,6 +537,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
     const bool edge = k0 + BN > f.len || f.row0 + wave * 32 + 32 > f.len || (p.causal && k0 + BN - 1 > f.row0 + wave * 32);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
+      if (n && k0 + 32 >= wend) break;
       f32x16 s, g;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
@@ -627,8 +631,11 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
     // queries that see this lane's key: from `first` on, `seen` of them
     const int first = (p.causal ? row : 0) - at0 - 4 * h, seen = f.len - (p.causal ? row : 0);
     const bool edge = at0 + BN > f.len || (p.causal && at0 < f.row0 + wave * 32 + 31);
+    if (f.row0 + wave * 32 >= f.len) continue;            // a wave behind the sequence's end only loads
 #pragma unroll
     for (int n = 0; n < BN / 32; ++n) {
+      // 32 queries behind the end, or all before this wave's keys
+      if (edge && (at0 + 32 * n >= f.len || (p.causal && at0 + 32 * n + 32 <= f.row0 + wave * 32))) continue;
       f32x16 s, g;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
