@@ -62,8 +62,8 @@ _SIGS = {
     "asyrp_train_backward": (C.c_int, [_P, C.c_int64, _P, _I, C.POINTER(C.c_char_p), C.POINTER(_P), _P]),
     "asyrp_train_discard": (None, [_P, C.c_int64]),
     "asyrp_sampler_update": (C.c_int, [_I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
-    "asyrp_packed_attention_forward": (C.c_int, [_I] + [_P] * 8 + [_I, _P]),
-    "asyrp_packed_attention_workspace": (C.c_int64, [_P]),
+    "asyrp_packed_attention_forward": (C.c_int, [_I] + [_P] * 9 + [_I, _P]),
+    "asyrp_packed_attention_workspace": (C.c_int64, [_P, _I]),
     "asyrp_packed_attention_backward": (C.c_int, [_I] + [_P] * 14),
     "asyrp_residual_norm_forward": (C.c_int, [_I] + [_P] * 12),
     "asyrp_residual_norm_workspace": (C.c_int64, [_P]),

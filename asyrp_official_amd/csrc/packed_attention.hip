@@ -54,7 +54,9 @@ struct PackedAttnArgs {
   long long T;
   int nseq, Hq, Hkv, D, causal, fill_tail;
   int parts;                 // workgroups that share the queries of one key tile (dk / dv)
-  float* partial;            // [parts][T][Hkv][dk, dv][D] where there are several
+  int splits;                // workgroups that share the keys of one query tile (forward, dq)
+  float* partial;            // where there are several, their sums: [parts][T][Hkv][dk, dv][D], [splits][T][Hq][D]
+  float2* stats;             // [splits][Hq][T] reference (times scale, base 2) and sum of each part of the forward
   int tiles;                 // row tiles launched per head: T / BM + nseq + 1, at least one more than the sequences have
   float scale;
   long long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h, do_t, do_h, dq_t, dq_h, dk_t, dk_h, dv_t, dv_h;
@@ -388,10 +390,10 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[3][BN * DP * 2], vt[2][BN * DP * 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int head = blockIdx.x % p.Hq, tile = blockIdx.x / p.Hq;
+  const int split = blockIdx.x % p.splits, head = blockIdx.x / p.splits % p.Hq, tile = blockIdx.x / p.splits / p.Hq;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT : IN_ORDER);
   if (f.idle) {
-    if (p.fill_tail) zero_tail((T*)p.out, p.o_t, p.o_h, head, p.D, f, p.T, tid);
+    if (p.fill_tail && split == 0) zero_tail((T*)p.out, p.o_t, p.o_h, head, p.D, f, p.T, tid);
     return;
   }
   const int hk = head / (p.Hq / p.Hkv);
@@ -400,17 +402,26 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   const int row = f.row0 + wave * 32 + (lane & 31);
   const bool there = row < f.len;
   const T* qrow = (const T*)p.q + (f.start + (there ? row : 0)) * p.q_t + head * p.q_h;
-  const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
+  int kend = p.causal ? min(f.len, f.row0 + BM) : f.len, k0 = 0;
+  if (p.splits > 1) {                                   // this part of the key tiles
+    const int n = (kend + BN - 1) / BN;
+    k0 = n * split / p.splits * BN;
+    kend = min(kend, n * (split + 1) / p.splits * BN);
+    if (k0 >= kend) {
+      if (there && h == 0) p.stats[((long long)split * p.Hq + head) * p.T + f.start + row] = make_float2(-INFINITY, 0.f);
+      return;
+    }
+  }
   // keys that all of this wave's queries see, in whole tiles, and keys that it has to look at
   const bool empty = f.row0 + wave * 32 >= f.len;       // a wave behind the sequence's end only loads
-  const int open = empty ? 0 : (p.causal ? min(f.len, f.row0 + wave * 32 + 1) : f.len) / BN * BN;
+  const int open = empty ? 0 : min(kend, p.causal ? min(f.len, f.row0 + wave * 32 + 1) / BN * BN : f.len / BN * BN);
   const int wend = empty ? 0 : p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;
   Tile<T, DP> ks_, vs_;
-  ks_.init(p.k_t, f.len, p.D, tid);
-  vs_.init(p.v_t, f.len, p.D, tid);
-  ks_.load(k, f.len, lds_offset(kt[0]), p.D, tid);
-  vs_.load(v, f.len, lds_offset(vt[0]), p.D, tid);
-  if (BN < kend) ks_.load(k + BN * p.k_t, f.len - BN, lds_offset(kt[1]), p.D, tid);
+  ks_.init(p.k_t, f.len - k0, p.D, tid);
+  vs_.init(p.v_t, f.len - k0, p.D, tid);
+  ks_.load(k + (long long)k0 * p.k_t, f.len - k0, lds_offset(kt[0]), p.D, tid);
+  vs_.load(v + (long long)k0 * p.v_t, f.len - k0, lds_offset(vt[0]), p.D, tid);
+  if (k0 + BN < kend) ks_.load(k + (long long)(k0 + BN) * p.k_t, f.len - k0 - BN, lds_offset(kt[1]), p.D, tid);
   FwdWave<T, DP> w;
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) w.qf[ks] = load_frag<T>(qrow, ks, h, p.D, there);
@@ -425,7 +436,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   tile_barrier();
   w.scores(s0, kt[0], 0, lane);
   w.maximum(s0);
-  int k0 = 0, ka = 0, kb = 1, kc = 2, vb = 0;           // key tiles of this, the next and the next but one; parity of the value tile
+  int ka = 0, kb = 1, kc = 2, vb = 0;           // key tiles of this, the next and the next but one; parity of the value tile
   // Loads of the tiles behind: the keys run one tile ahead of the values, since a tile's last scores are those of the next one's first half
   auto fetch = [&] {
     if (k0 + 2 * BN < kend) ks_.load(k + (long long)(k0 + 2 * BN) * p.k_t, f.len - k0 - 2 * BN, lds_offset(kt[kc]), p.D, tid);
@@ -464,6 +475,12 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
     advance();
   }
   const float l = both_halves_sum(w.l);
+  if (p.splits > 1) {
+    const long long at = f.start + row;
+    if (there) store_cols<DP>(p.partial + ((split * p.T + at) * p.Hq + head) * p.D, w.acc, 1.0f, h, p.D);
+    if (there && h == 0) p.stats[((long long)split * p.Hq + head) * p.T + at] = make_float2(w.m * w.sc, l);
+    return;
+  }
   store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, w.acc, 1.0f / l, h, p.D, there,
                     p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
   if (there && p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (w.m * w.sc + log2f(l)) * LN2;
@@ -475,10 +492,10 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int head = blockIdx.x % p.Hq, tile = blockIdx.x / p.Hq;
+  const int split = blockIdx.x % p.splits, head = blockIdx.x / p.splits % p.Hq, tile = blockIdx.x / p.splits / p.Hq;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT : IN_ORDER);
   if (f.idle) {
-    zero_tail((T*)p.dq, p.dq_t, p.dq_h, head, p.D, f, p.T, tid);
+    if (split == 0) zero_tail((T*)p.dq, p.dq_t, p.dq_h, head, p.D, f, p.T, tid);
     return;
   }
   const int hk = head / (p.Hq / p.Hkv);
@@ -510,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
   }
   delta = both_halves_sum(delta);
   const float lse2 = there ? p.lse[(long long)head * p.T + at] * LOG2E : 0.f;
-  if (there && h == 0) p.delta[(long long)head * p.T + at] = delta;
+  if (there && h == 0 && split == 0) p.delta[(long long)head * p.T + at] = delta;
 
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -518,15 +535,18 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
   const float sc = p.scale * LOG2E;
-  const int kend = p.causal ? min(f.len, f.row0 + BM) : f.len;
+  const int all = p.causal ? min(f.len, f.row0 + BM) : f.len, tiles = (all + BN - 1) / BN;
+  const int kbeg = tiles * split / p.splits * BN, kend = min(all, tiles * (split + 1) / p.splits * BN);      // this part of the key tiles
   const int wend = f.row0 + wave * 32 >= f.len ? 0 : p.causal ? min(f.len, f.row0 + wave * 32 + 32) : f.len;     // keys this wave has to look at
   Tile<T, DP> ks_, vs_;
-  ks_.init(p.k_t, f.len, p.D, tid);
-  vs_.init(p.v_t, f.len, p.D, tid);
-  ks_.load(k, f.len, lds_offset(kt[0]), p.D, tid);
-  vs_.load(v, f.len, lds_offset(vt[0]), p.D, tid);
+  if (kbeg < kend) {
+    ks_.init(p.k_t, f.len - kbeg, p.D, tid);
+    vs_.init(p.v_t, f.len - kbeg, p.D, tid);
+    ks_.load(k + (long long)kbeg * p.k_t, f.len - kbeg, lds_offset(kt[0]), p.D, tid);
+    vs_.load(v + (long long)kbeg * p.v_t, f.len - kbeg, lds_offset(vt[0]), p.D, tid);
+  }
   int buf = 0;
-  for (int k0 = 0; k0 < kend; k0 += BN, buf ^= 1) {
+  for (int k0 = kbeg; k0 < kend; k0 += BN, buf ^= 1) {
     tile_barrier();
     if (k0 + BN < kend) {
       ks_.load(k + (long long)(k0 + BN) * p.k_t, f.len - k0 - BN, lds_offset(kt[buf ^ 1]), p.D, tid);
@@ -559,6 +579,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
         add_ds<T, DP>(acc, kt[buf], 32 * n + 16 * b, s, b, edge, lane);
       }
     }
+  }
+  if (p.splits > 1) {
+    if (there) store_cols<DP>(p.partial + ((split * p.T + at) * p.Hq + head) * p.D, acc, p.scale, h, p.D);
+    return;
   }
   store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale, h, p.D, there);
 }
@@ -870,14 +894,66 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const PackedAttnA
   *reinterpret_cast<typename Frag<T>::V*>(to) = x;
 }
 
+// dq from the parts' sums, in the parts' order
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_join_dq_kernel(const PackedAttnArgs p) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8, wide = (long long)p.Hq * p.D;
+  const long long row = i / wide, begin = p.cu[0] < 0 ? 0 : p.cu[0], end = min(p.T, (long long)p.cu[p.nseq]);
+  if (row >= end || row < begin) return;                // rows of no sequence are zero already
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = p.partial[i + j];
+  for (int k = 1; k < p.splits; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += p.partial[k * p.T * wide + i + j];
+  typename Frag<T>::V x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = (T)s[j];
+  *reinterpret_cast<typename Frag<T>::V*>((T*)p.dq + i) = x;
+}
+// the forward from its parts: each part's sums are taken to the largest reference
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_join_fwd_kernel(const PackedAttnArgs p) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8, wide = (long long)p.Hq * p.D;
+  const long long row = i / wide, begin = p.cu[0] < 0 ? 0 : p.cu[0], end = min(p.T, (long long)p.cu[p.nseq]);
+  if (row >= end || row < begin) return;
+  const int head = (int)(i % wide / p.D), d = (int)(i % p.D);
+  float m = -INFINITY;
+  for (int k = 0; k < p.splits; ++k) m = fmaxf(m, p.stats[((long long)k * p.Hq + head) * p.T + row].x);
+  float s[8], l = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  for (int k = 0; k < p.splits; ++k) {
+    const float2 st = p.stats[((long long)k * p.Hq + head) * p.T + row];
+    if (st.y == 0.f) continue;                          // a part that saw no key
+    const float w = exp2_fast(st.x - m);
+    l = __builtin_fmaf(st.y, w, l);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = __builtin_fmaf(p.partial[k * p.T * wide + i + j], w, s[j]);
+  }
+  const float inv = 1.0f / l;
+  typename Frag<T>::V x, r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float o = s[j] * inv;
+    x[j] = (T)o;
+    r[j] = (T)(o - (float)x[j]);
+  }
+  *reinterpret_cast<typename Frag<T>::V*>((T*)p.out + row * p.o_t + head * p.o_h + d) = x;
+  if (p.rest) *reinterpret_cast<typename Frag<T>::V*>((T*)p.rest + i) = r;
+  if (p.lse && d == 0) p.lse[(long long)head * p.T + row] = (m + log2f(l)) * LN2;
+}
+
 template <typename T, int DP>
 hipError_t launch_forward(const PackedAttnArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq * a.splits), dim3(256), 0, s, a);
+  if (a.splits > 1) hipLaunchKernelGGL((packed_attn_join_fwd_kernel<T>), dim3((unsigned)((a.T * a.Hq * a.D / 8 + 255) / 256)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 template <typename T, int DP>
 hipError_t launch_backward(const PackedAttnArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP>), dim3((unsigned)a.tiles * a.Hq * a.splits), dim3(256), 0, s, a);
+  if (a.splits > 1) hipLaunchKernelGGL((packed_attn_join_dq_kernel<T>), dim3((unsigned)((a.T * a.Hq * a.D / 8 + 255) / 256)), dim3(256), 0, s, a);
   const dim3 g((unsigned)a.tiles * a.Hkv * a.parts);
   if constexpr (DP > 64) hipLaunchKernelGGL((packed_attn_dkv_pair_kernel<T, DP>), g, dim3(512), 0, s, a);
   else hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP>), g, dim3(256), 0, s, a);
@@ -896,21 +972,29 @@ hipError_t launch(const PackedAttnArgs& a, bool backward, hipStream_t s) {
   }
 }
 
-// Into how many parts the queries of a key tile are dealt: a kernel of few tiles (few rows, or few key / value heads with many query heads each) leaves CUs idle
-// and ends with its longest workgroup; the parts' fp32 sums cost a write and a read of 8 bytes per value and part.  Wanted are two workgroups per CU, and
-// a part is at least 1024 queries on average.  (16 heads on 4, 8192 rows: 1 part 1.41 ms, 2 parts 0.49 ms, 4 parts 0.46 ms with the first form of the kernel; now
-// 2 and 4 parts are within 1 %, and 2 take half the workspace.)
-int dkv_parts(long long T, int nseq, int Hq, int Hkv) {
-  const long long wgs = std::max<long long>(1, T / BM) * Hkv;       // full tiles; the ragged ones are light
+// Into how many parts a tile's other axis is dealt: the keys of a query tile (forward, dq: `heads` query heads, shared = 1) and the queries of a key tile (dk / dv:
+// `heads` key / value heads, each `shared` times the queries).  A launch of few tiles leaves CUs idle and ends with its longest workgroup; the
+// parts' fp32 sums cost a write and a read.  Wanted are more workgroups than CUs and eight tiles a part where all rows are one sequence (their
+// lengths are on the device); many short sequences are left whole.  Forward + backward in us, whole and in parts: causal sequences of 1829 / 379 / 312,
+// 8 heads on 2 of 64: 285 and 110; one of 6000, one head of 128: 511 and 142 (forward 107 and 41); one of 2000, 4 heads on 1 of 128: 363 and 130; 600 / 500, 4 heads
+// of 64: 61 and 52.  (16 heads on 4, 128 wide, 8192 rows: dk and dv in 1 part 1.41 ms, in 2 0.49 ms with their first form; 4 parts are within 1 % of 2.)
+int parts_of(long long T, int nseq, int heads, int shared) {
+  const long long wgs = std::max<long long>(1, T / BM) * heads;     // full tiles; the ragged ones are light
   int parts = 1;
-  while (parts < 8 && wgs * parts < 512 && T / nseq * (Hq / Hkv) >= 1024LL * parts) parts *= 2;
+  while (parts < 8 && wgs * parts <= 256 && T * shared >= 16LL * BN * parts && T / nseq * shared >= 3 * BN) parts *= 2;
   return parts;
+}
+// floats of workspace: forward {sums, statistics}; backward {delta, sums of dq and then of dk / dv}
+long long forward_floats(const PackedAttnArgs& a) { return a.splits > 1 ? a.splits * a.T * a.Hq * (a.D + 2LL) : 0; }
+long long delta_floats(const PackedAttnArgs& a) { return (a.T * a.Hq + 3) / 4 * 4; }
+long long backward_floats(const PackedAttnArgs& a) {
+  return delta_floats(a) + std::max(a.splits > 1 ? a.splits * a.T * a.Hq * a.D : 0LL, a.parts > 1 ? a.parts * a.T * a.Hkv * 2 * a.D : 0LL);
 }
 
 int refuse(const char* m) { return set_last_error(ASYRP_EINVAL, m); }
 
-// the checks that both directions share; 0 or the error
-int check(const PackedAttnArgs& a, int dtype, const long long* strides, int n) {
+// the checks that both directions share, and how their work is dealt out; 0 or the error
+int check(PackedAttnArgs& a, int dtype, const long long* strides, int n) {
   if (dtype != ASYRP_F16 && dtype != ASYRP_BF16) return refuse("packed attention takes f16 or bf16 operands");
   if (a.D < 8 || a.D > 128 || a.D % 8) return refuse("packed attention: the head width must be a multiple of 8 from 8 to 128");
   if (a.Hq < 1 || a.Hkv < 1 || a.Hq % a.Hkv) return refuse("packed attention: query heads must be a multiple of key/value heads");
@@ -919,6 +1003,9 @@ int check(const PackedAttnArgs& a, int dtype, const long long* strides, int n) {
   for (int i = 0; i < n; ++i)
     if (strides[i] < 0 || strides[i] % 8 || strides[i] > (i % 2 ? 1LL << 40 : 1LL << 23))
       return refuse("packed attention: strides must be multiples of 8 values, not negative, rows at most 2^23 values apart");
+  a.tiles = (int)std::min<long long>(a.T / BM + a.nseq + 1, 0x7fffffff);
+  a.splits = parts_of(a.T, a.nseq, a.Hq, 1);
+  a.parts = parts_of(a.T, a.nseq, a.Hkv, a.Hq / a.Hkv);
   const long long tiles = a.T / BM + a.nseq + 1;
   if (tiles * a.Hq * 8 > 0x7fffffffLL) return refuse("packed attention: too many rows x heads for one launch");
   return 0;
@@ -937,7 +1024,7 @@ using namespace asyrp;
 extern "C" {
 
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
-                                   float* lse, void* out_rest, int fill_tail, void* stream) {
+                                   float* lse, void* out_rest, float* workspace, int fill_tail, void* stream) {
   if (!p || !cu_seqlens) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.cu = cu_seqlens;
@@ -948,21 +1035,21 @@ int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, 
   const long long st[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.o_t, a.o_h};
   if (int rc = check(a, p->dtype, st, 8)) return rc;
   if (a.T == 0) return 0;
-  if (unaligned({q, k, v, out}) || ((uintptr_t)out_rest & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");
-  a.tiles = (int)(a.T / BM + a.nseq + 1);
+  a.partial = workspace;
+  a.stats = reinterpret_cast<float2*>(workspace + (a.splits > 1 ? a.splits * a.T * a.Hq * a.D : 0));
+  if (unaligned({q, k, v, out}) || ((uintptr_t)out_rest & 15) || ((uintptr_t)workspace & 15) || (a.splits > 1 && !workspace)) return refuse("packed attention: tensors must be given and 16-byte aligned");
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
   const hipError_t e = p->dtype == ASYRP_F16 ? launch<_Float16>(a, false, (hipStream_t)stream) : launch<__bf16>(a, false, (hipStream_t)stream);
   return e == hipSuccess ? 0 : set_last_error(ASYRP_EHIP, hipGetErrorString(e));
 }
 
-int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p) {
+int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p, int backward) {
   if (!p) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
   a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.scale = p->scale;
   if (int rc = check(a, p->dtype, nullptr, 0)) return rc;
-  const int parts = dkv_parts(a.T, a.nseq, a.Hq, a.Hkv);
-  return (a.T * a.Hq + 3) / 4 * 4 + (parts > 1 ? parts * a.T * a.Hkv * 2 * a.D : 0);
+  return backward ? backward_floats(a) : forward_floats(a);
 }
 
 int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
@@ -978,10 +1065,8 @@ int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p,
   const long long st[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.o_t, a.o_h, a.do_t, a.do_h};
   if (int rc = check(a, p->dtype, st, 10)) return rc;
   if (a.T == 0) return 0;
-  a.parts = dkv_parts(a.T, a.nseq, a.Hq, a.Hkv);
-  a.partial = workspace + (a.T * a.Hq + 3) / 4 * 4;
+  a.partial = workspace + delta_floats(a);
   if (unaligned({q, k, v, out, d_out, dq, dk, dv}) || ((uintptr_t)out_rest & 15) || !lse || !workspace || ((uintptr_t)workspace & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");
-  a.tiles = (int)(a.T / BM + a.nseq + 1);
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
   const hipError_t e = p->dtype == ASYRP_F16 ? launch<_Float16>(a, true, (hipStream_t)stream) : launch<__bf16>(a, true, (hipStream_t)stream);

@@ -71,9 +71,13 @@ def _attention_forward(q, k, v, cu, causal, scale, out, train):
     lse = q.new_empty((H, T), dtype=torch.float32) if train else None
     rest = q.new_empty(q.shape) if train else None
     spec = (T, cu.shape[0] - 1, H, k.shape[1], D, causal, _lib.DTYPES[q.dtype], scale, *sq, *sk, *sv, *_strides(out))
-    device = q.device.index
-    rc = _lib.load().asyrp_packed_attention_forward(device, _lib.PACKED_ATTENTION.pack(*spec, 0, 0), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(),
-                                                    out.data_ptr(), _ptr(lse), _ptr(rest), fill, _raw_stream(device))
+    lib, device, packed = _lib.load(), q.get_device(), _lib.PACKED_ATTENTION.pack(*spec, 0, 0)
+    words = lib.asyrp_packed_attention_workspace(packed, 0)
+    if words < 0:
+        _lib.check(words)
+    ws = q.new_empty((words,), dtype=torch.float32) if words else None
+    rc = lib.asyrp_packed_attention_forward(device, packed, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(),
+                                                    out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(ws), fill, _raw_stream(device))
     if rc:
         _lib.check(rc)
     return q, k, v, out, lse, rest, spec
@@ -92,8 +96,8 @@ class _PackedAttention(torch.autograd.Function):
         q, k, v, cu, out, lse, rest = ctx.saved_tensors
         d_out, sd = _readable(d_out)
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        lib, device, spec = _lib.load(), q.device.index, _lib.PACKED_ATTENTION.pack(*ctx.spec, *sd)
-        words = lib.asyrp_packed_attention_workspace(spec)
+        lib, device, spec = _lib.load(), q.get_device(), _lib.PACKED_ATTENTION.pack(*ctx.spec, *sd)
+        words = lib.asyrp_packed_attention_workspace(spec, 1)
         if words < 0:
             _lib.check(words)
         ws = q.new_empty((max(4, words),), dtype=torch.float32)

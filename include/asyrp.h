@@ -296,11 +296,11 @@ int asyrp_sampler_update(int device, const float* x, const float* model_out, int
  * ascending values from 0; values outside [0, tokens] or falling ones are held inside the tensors but give no defined result).
  * lse [heads][tokens] (nullable in the forward) = log sum exp of the scaled scores.  out_rest [tokens][heads][head_dim] contiguous (nullable in both) = what the
  * rounding of out took away, so that the backward's rowsum(d_out * out) is that of the unrounded output.  Rows behind the last sequence are set to zero in the gradients
- * and, where fill_tail is not 0, in out.  The gradients are contiguous; workspace: asyrp_packed_attention_workspace() floats (negative: an
- * error code). */
+ * and, where fill_tail is not 0, in out.  The gradients are contiguous; workspace: asyrp_packed_attention_workspace() floats of the
+ * direction (negative: an error code; 0: none, null will do), 16-byte aligned. */
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                   void* out, float* lse, void* out_rest, int fill_tail, void* stream);
-int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p);
+                                   void* out, float* lse, void* out_rest, float* workspace, int fill_tail, void* stream);
+int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p, int backward);
 int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
                                     const void* out, const float* lse, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream);
 

@@ -90,7 +90,7 @@ def test_forward_and_gradients(case, dtype):
 
 
 # ---- two parts of the queries per key tile, more than 64 sequences, other layouts -----------------------------------------------------------
-LONG = [([1500], 4, 1, 128, True), ([1100, 700], 8, 1, 96, False), ([3] * 80 + [90], 2, 1, 64, True), ([1, 0] * 50, 2, 2, 32, True), ([130] * 66, 1, 1, 128, True)]
+LONG = [([1500], 4, 1, 128, True), ([2600], 1, 1, 64, True), ([0, 2300, 31], 2, 1, 128, False), ([1100, 700], 8, 1, 96, False), ([3] * 80 + [90], 2, 1, 64, True), ([1, 0] * 50, 2, 2, 32, True), ([130] * 66, 1, 1, 128, True)]
 
 
 @pytest.mark.gpu
@@ -129,13 +129,15 @@ def test_rows_of_no_sequence_stay_zero_or_untouched():
     for t in (q, k, v, do):
         t[300:] = math.nan                                             # nothing of these rows may be seen
     got = run(q, k, v, do, offsets([100, 0, 200]), True)
-    want = run(q[:300], k[:300], v[:300], do[:300], offsets([100, 0, 200]), True)
+    # (how the work is dealt out goes by the number of rows, so the bits may differ from those of the 300 rows alone; the values' bounds do not)
+    want, tol = reference(q[:300], k[:300], v[:300], [100, 0, 200], True, 1 / 8, do[:300])
     for n in got:
-        assert torch.equal(got[n][:300], want[n]) and not got[n][300:].any()
+        check(n, got[n][:300], want[n], tol[n], HALF[torch.bfloat16])
+        assert not got[n][300:].any()
     out = torch.full_like(q, 7.0)
     with torch.no_grad():
         assert packed_attention(q, k, v, offsets([100, 0, 200]), causal=True, out=out) is out
-    assert torch.equal(out[:300], want["o"]) and (out[300:] == 7.0).all()
+    assert torch.equal(out[:300], got["o"][:300]) and (out[300:] == 7.0).all()
     none = run(q, k, v, do, offsets([0, 0]), False)                    # no rows in any sequence
     assert not any(t.any() for t in none.values())
     assert packed_attention(q[:0], k[:0], v[:0], offsets([0])).shape == (0, 2, 64)
@@ -238,7 +240,7 @@ def test_library_refuses_what_its_kernels_do_not_take():
 
     def call(T=4, n=1, H=2, K=1, D=64, dtype=_lib.F16, scale=1.0, sq=(128, 64), ptr=4096):
         spec = _lib.PACKED_ATTENTION.pack(T, n, H, K, D, 0, dtype, scale, *sq, 64, 64, 64, 64, 128, 64, 128, 64)
-        f = lib.asyrp_packed_attention_forward(0, spec, ptr, ptr, ptr, 4096, ptr, None, None, 1, None)
+        f = lib.asyrp_packed_attention_forward(0, spec, ptr, ptr, ptr, 4096, ptr, None, None, 4096, 1, None)
         b = lib.asyrp_packed_attention_backward(0, spec, ptr, ptr, ptr, 4096, ptr, 4096, None, ptr, 4096, ptr, ptr, ptr, None)
         assert f == b
         return f
@@ -248,8 +250,8 @@ def test_library_refuses_what_its_kernels_do_not_take():
         assert call(**bad) == -1, bad
         assert b"packed attention" in lib.asyrp_last_error()
     assert call(T=0) == 0                                              # nothing to do, nothing launched
-    assert lib.asyrp_packed_attention_forward(0, None, 4096, 4096, 4096, 4096, 4096, None, None, 1, None) == -1
-    assert lib.asyrp_packed_attention_workspace(None) == -1
+    assert lib.asyrp_packed_attention_forward(0, None, 4096, 4096, 4096, 4096, 4096, None, None, 4096, 1, None) == -1
+    assert lib.asyrp_packed_attention_workspace(None, 0) == -1
 
 
 @pytest.mark.gpu
