@@ -36,12 +36,13 @@ struct NormArgs {
   int C, after, before, rms; // which norms there are
   int chunks;                // workgroups per gate row (1 where a workgroup takes whole gate rows)
   long long gates_per_wg, chunk_rows, gates;
+  int row_gate;              // every row has its gate (and the walk takes them for one set of rows)
   int want_w1, want_b1, want_w2, want_b2, want_gate;
 };
 // partial vectors, in this order
 enum { V_W2, V_B2, V_W1, V_B1, V_GATE, VECTORS };
 
-// A thread's VPT values of a row: contiguous (VEC: whole 16-byte groups of the row), or TPR apart, so that neighbouring lanes still read
+// A thread's VPT values of a row: contiguous (VEC: whole groups of the row), or TPR (threads per row) apart, so that neighbouring lanes still read
 // neighbouring values of a row of any width and address.
 template <typename T, int VPT>
 struct Raw {
@@ -110,10 +111,28 @@ __device__ __forceinline__ float wave_sum(float v) {
 #undef ASYRP_DPP
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
+// sums over the 16 lanes of a row of lanes, in all of them
+__device__ __forceinline__ float sum16(float v) {
+#define ASYRP_DPP(CTRL) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false))
+  ASYRP_DPP(0x121);
+  ASYRP_DPP(0x122);
+  ASYRP_DPP(0x124);
+  ASYRP_DPP(0x128);
+#undef ASYRP_DPP
+  return v;
+}
 // sums of K values over the TPR threads of a row.  `buf` holds two sets of one row of K values per wave, used in turn, so that
 // one barrier per reduction is enough.
 template <int TPR, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float* buf, int& turn, int sub, int t) {
+  if (TPR == 16 || TPR == 32) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = sum16(v[k]);
+      if (TPR == 32) v[k] += __shfl_xor(v[k], 16);
+    }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
   if (TPR > 64) {
@@ -126,10 +145,14 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* buf, int& turn, in
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float s = 0.f;
+      if (W == 16) {                     // sixteen waves: one read and four steps (4000 x 5041 in fp32, both directions: 450 us, with sixteen reads 596)
+        v[k] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sum16(b[(t & 15) * 2 + k]))));
+      } else {
+        float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) s += b[w * 2 + k];
-      v[k] = s;
+        for (int w = 0; w < W; ++w) s += b[w * 2 + k];
+        v[k] = s;
+      }
     }
   }
 }
@@ -180,6 +203,7 @@ template <typename X, typename Y, bool VEC, int TPR, int VPT>
 __global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const NormArgs p) {
   __shared__ float buf[64];
   constexpr int SUB = threads<TPR>() / TPR;
+  const bool row_gate = SUB > 1 && p.row_gate;
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
   int turn = 0;
   float w1[VPT], w2[VPT], b1[VPT], b2[VPT];
@@ -192,7 +216,7 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const
   for (long long g = g0; g < g1; ++g) {
     const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
     float gate[VPT];
-    columns<VEC, TPR, VPT>(p.gate ? p.gate + g * C : nullptr, 1.f, t, C, gate);
+    if (!row_gate) columns<VEC, TPR, VPT>(p.gate ? p.gate + g * C : nullptr, 1.f, t, C, gate);
     Raw<X, VPT> xn{};
     Raw<Y, VPT> yn{};
     auto fetch = [&](long long r) {
@@ -208,6 +232,7 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const
       floats(xn, x);
       floats(yn, y);
       if (r0 + SUB < last) fetch(r0 + SUB);
+      if (row_gate) columns<VEC, TPR, VPT>(p.gate + row * C, 1.f, t, C, gate);
       float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
       if (p.after) {
         statistics<VEC, TPR, VPT>(y, p, buf, turn, sub, t, m1, r1);
@@ -233,14 +258,20 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_fwd_kernel(const
 template <typename X, typename Y, bool VEC, int TPR, int VPT>
 __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const NormArgs p) {
   constexpr int SUB = threads<TPR>() / TPR;
+  const bool row_gate = SUB > 1 && p.row_gate;
   __shared__ float buf[64];
   __shared__ float join[SUB > 1 ? SUB * TPR * VPT : 1];
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR, C = p.C;
   int turn = 0;
+  // eight or sixteen values a thread leave no registers for the weights beside the sums, nor for a row ahead: they are read again for every row, from the caches
+  // (8192 x 8192 in bf16, eight values, both directions: 501 us, with spilled registers 805)
+  constexpr bool LEAN = VPT > 4;
   float w1[VPT], w2[VPT], b1[VPT];
-  columns<VEC, TPR, VPT>(p.w1, 1.f, t, C, w1);
-  columns<VEC, TPR, VPT>(p.b1, 0.f, t, C, b1);
-  columns<VEC, TPR, VPT>(p.w2, 1.f, t, C, w2);
+  if (!LEAN) {
+    columns<VEC, TPR, VPT>(p.w1, 1.f, t, C, w1);
+    columns<VEC, TPR, VPT>(p.b1, 0.f, t, C, b1);
+    columns<VEC, TPR, VPT>(p.w2, 1.f, t, C, w2);
+  }
   float sw1[VPT], sb1[VPT], sw2[VPT], sb2[VPT], sg[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) sw1[j] = sb1[j] = sw2[j] = sb2[j] = 0.f;
@@ -266,7 +297,7 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
   for (long long g = g0; g < g1; ++g) {
     const long long first = g * p.per_gate + part * p.chunk_rows, last = min(p.rows, min((g + 1) * p.per_gate, first + p.chunk_rows));
     float gate[VPT];
-    columns<VEC, TPR, VPT>(p.gate ? p.gate + g * C : nullptr, 1.f, t, C, gate);
+    if (!LEAN && !row_gate) columns<VEC, TPR, VPT>(p.gate ? p.gate + g * C : nullptr, 1.f, t, C, gate);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) sg[j] = 0.f;
     Raw<X, VPT> xn{}, dhn{};
@@ -280,22 +311,29 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
       if (p.dh) load<X, VEC, TPR, VPT>((const X*)p.dh + row * C, t, C, dhn);
       stn = reinterpret_cast<const float4*>(p.stats)[row];
     };
-    if (first < last) fetch(first);
+    if (!LEAN && first < last) fetch(first);
     for (long long r0 = first; r0 < last; r0 += SUB) {
       const bool there = r0 + sub < last;
       const long long row = there ? r0 + sub : last - 1;
+      if (LEAN) {
+        fetch(r0);
+        columns<VEC, TPR, VPT>(p.w1, 1.f, t, C, w1);
+        columns<VEC, TPR, VPT>(p.b1, 0.f, t, C, b1);
+      }
       float x[VPT], y[VPT], dh[VPT], dn[VPT], u[VPT];
       floats(xn, x);
       floats(yn, y);
       floats(dhn, dh);
       floats(dnn, dn);
       const float4 st = stn;
-      if (r0 + SUB < last) fetch(r0 + SUB);
+      if (!LEAN && r0 + SUB < last) fetch(r0 + SUB);
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
         y[j] = (y[j] - st.x) * st.y;                          // without the norm behind the block: mean 0, rstd 1
         u[j] = __builtin_fmaf(y[j], w1[j], b1[j]);
       }
+      if (LEAN || row_gate) columns<VEC, TPR, VPT>(p.gate ? p.gate + (row_gate ? row : g) * C : nullptr, 1.f, t, C, gate);
+      if (LEAN) columns<VEC, TPR, VPT>(p.w2, 1.f, t, C, w2);
       // `keep`: false only for the copies of the last row that fill up a set of rows
       const bool keep = SUB == 1 || there;
       if (p.before && p.dn) {
@@ -322,7 +360,8 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
         x[j] = p.a * dh[j];                                   // dx
-        if (keep) sg[j] = __builtin_fmaf(dh[j], u[j], sg[j]);
+        u[j] *= dh[j];                                        // of the gate
+        if (keep) sg[j] += u[j];
         dh[j] *= gate[j];
       }
       if (p.after) {
@@ -344,14 +383,17 @@ __global__ __launch_bounds__(threads<TPR>()) void residual_norm_bwd_kernel(const
 #pragma unroll
         for (int j = 0; j < VPT; ++j) dh[j] = st.y * __builtin_fmaf(-y[j], c2, dh[j] - c1);
       }
-      landed(xn);
-      landed(yn);
-      landed(dhn);
-      landed(dnn);
+      if (!LEAN) {
+        landed(xn);
+        landed(yn);
+        landed(dhn);
+        landed(dnn);
+      }
+      if (there && row_gate && p.want_gate) store<float, VEC, TPR, VPT>(p.dgate + row * C, t, C, u);
       if (there && p.dx) store<X, VEC, TPR, VPT>((X*)p.dx + row * C, t, C, x);
       if (there && p.dy) store<Y, VEC, TPR, VPT>((Y*)p.dy + row * C, t, C, dh);
     }
-    if (p.want_gate) put(sg, p.chunks == 1 ? p.dgate + g * C : slot + V_GATE * C);
+    if (p.want_gate && !row_gate) put(sg, p.chunks == 1 ? p.dgate + g * C : slot + V_GATE * C);
   }
   if (p.want_w2) put(sw2, slot + V_W2 * C);
   if (p.want_b2) put(sb2, slot + V_B2 * C);
@@ -394,13 +436,20 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(const NormSumAr
   }
 }
 
-// four values per thread keep the backward's registers (five sums, four weights, two rows) under 128; widths over 4096 take eight
+// Four values per thread keep the backward's registers (five sums, four weights, two rows) under 128, so that 16 waves share a CU.  Rows of up to 128 share a
+// wave (63731 x 33 in fp32, both directions: 35 us, with a wave to each 56).  Rows over 4096 take sixteen values a thread (8192 x 8192 in bf16, both directions:
+// 450 us, with eight 501) or, where they are no multiple of sixteen, eight.
+constexpr int SHARED_WAVES = 512;        // up to this width a workgroup takes several rows at once
+int values_per_thread(int C) { return C <= 4096 ? 4 : C % 16 == 0 ? 16 : 8; }
 #define ASYRP_NORM(KERNEL) \
-  if (a.C <= 256) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 64, 4>), g, dim3(256), 0, s, a); \
-  else if (a.C <= 512) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 128, 4>), g, dim3(256), 0, s, a); \
+  if (a.C <= 64) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 16, 4>), g, dim3(256), 0, s, a); \
+  else if (a.C <= 128) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 32, 4>), g, dim3(256), 0, s, a); \
+  else if (a.C <= 256) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 64, 4>), g, dim3(256), 0, s, a); \
+  else if (a.C <= SHARED_WAVES) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 128, 4>), g, dim3(256), 0, s, a); \
   else if (a.C <= 1024) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 256, 4>), g, dim3(256), 0, s, a); \
   else if (a.C <= 2048) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 512, 4>), g, dim3(512), 0, s, a); \
   else if (a.C <= 4096) hipLaunchKernelGGL((KERNEL<X, Y, VEC, 1024, 4>), g, dim3(1024), 0, s, a); \
+  else if (VEC && values_per_thread(a.C) == 16) hipLaunchKernelGGL((KERNEL<X, Y, true, 512, 16>), g, dim3(512), 0, s, a); \
   else hipLaunchKernelGGL((KERNEL<X, Y, VEC, 1024, 8>), g, dim3(1024), 0, s, a)
 
 template <typename X, typename Y, bool VEC>
@@ -443,7 +492,8 @@ int check(const asyrp_residual_norm* p) {
 }
 // How the rows are dealt out: `want` workgroups where the rows allow, each with a part of one gate row or with several whole ones
 void deal(const asyrp_residual_norm* p, NormArgs& a, long long want, unsigned& wgs) {
-  a.gates = p->gates > 0 ? p->gates : 1;
+  a.row_gate = p->gates == p->rows && p->width <= SHARED_WAVES;
+  a.gates = p->gates > 0 && !a.row_gate ? p->gates : 1;
   a.per_gate = std::max<long long>(1, a.rows / a.gates);
   want = std::max<long long>(1, want);
   a.chunks = (int)std::max<long long>(1, std::min(want / a.gates, a.per_gate));
@@ -487,7 +537,7 @@ int asyrp_residual_norm_forward(int device, const asyrp_residual_norm* p, const 
   fill(p, a);
   a.x = x; a.y = y; a.gate = gate; a.w1 = after_weight; a.b1 = after_bias; a.w2 = before_weight; a.b2 = before_bias; a.h = h; a.n = n; a.stats = stats;
   if (!aligned({stats})) return refuse("residual norm: the statistics must be 16-byte aligned");
-  const bool vec = a.C % 8 == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, before_bias, h, n});
+  const bool vec = a.C % values_per_thread(a.C) == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, before_bias, h, n});
   unsigned wgs = 0;
   deal(p, a, std::min<long long>(4096, a.rows), wgs);
   DeviceGuard g(device);
@@ -525,7 +575,7 @@ int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const
   a.dh = dh; a.dn = dn; a.dx = dx; a.dy = dy; a.partial = workspace; a.dgate = dgate;
   a.want_w2 = d_before_weight != nullptr; a.want_b2 = d_before_bias != nullptr; a.want_w1 = d_after_weight != nullptr; a.want_b1 = d_after_bias != nullptr;
   a.want_gate = dgate != nullptr;
-  const bool vec = a.C % 8 == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, dh, dn, dx, dy, dgate, workspace});
+  const bool vec = a.C % values_per_thread(a.C) == 0 && aligned({x, y, gate, after_weight, after_bias, before_weight, dh, dn, dx, dy, dgate, workspace});
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
   hipError_t e = dispatch(p->stream_dtype, p->branch_dtype, a, vec, true, wgs, (hipStream_t)stream);
@@ -537,7 +587,7 @@ int asyrp_residual_norm_backward(int device, const asyrp_residual_norm* p, const
     sa.slots = (int)wgs;
     sa.chunks = a.chunks;
     sa.gates = a.gates;
-    if (a.chunks == 1) sa.out[V_GATE] = nullptr;     // whole gate rows were written by the kernel itself
+    if (a.chunks == 1 || a.row_gate) sa.out[V_GATE] = nullptr;     // whole gate rows were written by the kernel itself
     bool any = false;
     for (float* o : sa.out) any = any || o;
     if (any) {

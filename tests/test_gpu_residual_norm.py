@@ -122,6 +122,34 @@ def test_forward_and_gradients(name):
     compare(CASES[name], run(CASES[name]))
 
 
+# rows that share a wave, a gate to every row, groups of four, eight and sixteen values and rows that fall out of groups
+WIDTHS = {
+    "narrow": case(83, 33, "rms", gates=1), "narrow_16": case(129, 64, X=bf16, Y=bf16, gates=43), "narrow_full": case(35, 128, X=f32, Y=f16, gates=5), "narrow_odd": case(31, 127, "rms", X=f16, Y=f16),
+    "row_gate_17": case(45, 17, gates=45), "row_gate_64": case(51, 60, "rms", X=bf16, Y=bf16, gates=51), "row_gate_128": case(22, 100, X=f32, Y=bf16, gates=22, before=None, grads="h"),
+    "row_gate_512": case(37, 509, X=f16, Y=f16, gates=37, after=None), "row_gate_wide": case(9, 1100, gates=9), "row_gate_one": case(1, 80, gates=1),
+    "fours": case(40, 2300, "rms", X=bf16, Y=bf16, gates=1), "fours_mixed": case(23, 516, X=f32, Y=f16, gates=23), "sixteens": case(13, 4112, X=bf16, Y=bf16, gates=1), "sixteens_f32": case(7, 6144, "rms", gates=7),
+    "eights": case(9, 5000, X=f16, Y=f16, gates=3), "odd_wide": case(7, 5041, gates=1), "odd_fours_wide": case(6, 4100, X=bf16, Y=bf16),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", list(WIDTHS))
+def test_widths_and_gates_per_row(name):
+    compare(WIDTHS[name], run(WIDTHS[name]))
+
+
+@pytest.mark.gpu
+def test_gate_per_row_without_its_gradient():
+    c = WIDTHS["row_gate_64"]
+    x, y = (c[k].cuda().requires_grad_() for k in ("x", "y"))
+    both = []
+    for wants in (True, False):
+        h, n = gated_residual_norm(x, y, gate=c["gate"].cuda().requires_grad_(wants), residual_scale=c["a"], kind=c["kind"], after=tuple(w.cuda() for w in c["after"]), before=tuple(w.cuda() for w in c["before"]), eps=c["eps"])
+        both.append((h, n, *torch.autograd.grad((h, n), (x, y), (c["dh"].cuda(), c["dn"].cuda()))))
+    for a, b in zip(*both):
+        assert torch.equal(a, b)
+
+
 def test_oracle_formulas_against_autograd_and_differences():
     """The oracle itself, in fp64 on the CPU: its gradients are those of automatic differentiation, and of differences along a random direction."""
     c = case(12, 20, gates=3, seed=3)
