@@ -36,6 +36,9 @@ class _Moments:
             self.me, self.ve = (torch.zeros(n // BLOCK, device=device, dtype=torch.uint8) for _ in range(2))
         self.steps = torch.zeros(max(1, len(self.params)), device=device, dtype=torch.int32)
 
+    def of(self, params):
+        return len(self.params) == len(params) and all(map(operator.is_, self.params, params))
+
     def views(self, i):
         """What self.state holds of parameter i: views of the flat moments (8 bits: codes and exponent bytes)."""
         at, k, p = self.offsets[i], self.numels[i], self.params[i]
@@ -89,6 +92,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must lie in [0, 1), got {g['betas']}")
         if not 0.0 <= g["eps"] < float("inf") or not 0.0 <= g["weight_decay"] < float("inf"):
             raise ValueError("eps and weight_decay must be finite and not negative")
+        if len(set(map(id, g["params"]))) != len(g["params"]):
+            raise ValueError("a parameter stands in the group twice")
         for p in g["params"]:
             if p.dtype not in _lib.DTYPES:
                 raise ValueError(f"parameters must be float32, float16 or bfloat16, got {p.dtype}")
@@ -116,7 +121,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _group_moments(self, k, device):
         g, mo = self.param_groups[k], self._moments.get(k)
-        if mo is not None and mo.device == device and len(mo.params) == len(g["params"]) and all(map(operator.is_, mo.params, g["params"])):
+        if mo is not None and mo.device == device and mo.of(g["params"]):
             return mo
         for p in g["params"]:
             if not p.is_contiguous():
@@ -158,7 +163,8 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        """Takes what state_dict() of an optimiser with the same state_bits gave."""
+        """Takes what state_dict() of an optimiser with the same state_bits gave.  Moments, step counts and a learning rate on the device that are there
+        already take their values in place, so that a captured step goes on with what was loaded."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("loaded state dict has other parameter groups")
@@ -171,10 +177,25 @@ class AdamW(torch.optim.Optimizer):
             if set(st) != want or tuple(st["exp_avg"].shape) != tuple(p.shape) or tuple(st["exp_avg_sq"].shape) != tuple(p.shape) \
                     or (st["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
                 raise ValueError(f"loaded state of parameter {i} is not one of AdamW with {self.state_bits}-bit moments and shape {tuple(p.shape)}")
+        moments, norm, rates = self._moments, self.grad_norm, [g["lr"] for g in self.param_groups]
         super().load_state_dict({"state": {}, "param_groups": groups})
-        self._moments = {}
+        self._moments, self.grad_norm = moments, norm
+        with torch.no_grad():
+            for g, lr in zip(self.param_groups, rates):
+                if isinstance(lr, torch.Tensor) and lr.is_cuda:
+                    lr.fill_(float(g["lr"]))
+                    g["lr"] = lr
+            for k, mo in list(moments.items()):
+                if not mo.of(self.param_groups[k]["params"]):
+                    del moments[k]
+                    continue
+                for i, p in enumerate(mo.params):
+                    views, st = mo.views(i), saved.get(groups[k]["params"][i]) or {}
+                    for key, view in views.items():
+                        view.copy_(torch.as_tensor(st[key]).reshape(view.shape)) if key in st else view.zero_()
+                    self.state[p] = views
         for i, p in pairs:
-            if saved.get(i):
+            if saved.get(i) and p not in self.state:
                 self.state[p] = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in saved[i].items()}
 
     # ---- the step --------------------------------------------------------------------------------------

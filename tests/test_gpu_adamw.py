@@ -6,6 +6,7 @@ bounds add: v, m: 3 n u of their terms' sums; p: n (3 u |p| + 10 u |update| + wh
 import copy
 import io
 import math
+import warnings
 
 import pytest
 import torch
@@ -323,6 +324,52 @@ def test_a_captured_step_counts_and_follows_a_rate_on_the_device():
             assert all(torch.equal(p, q) for p, q in zip(ps, qs)), (bits, k)
             assert float(opt.grad_norm) == float(eager.grad_norm)
         assert int(opt.state[ps[0]]["step"]) == 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_goes_on_with_loaded_moments(bits):
+    shapes = [(1000,), (33, 5)]
+    init, grads = tensors(shapes), [tensors(shapes, seed=20 + k) for k in range(5)]
+    lr = torch.tensor(1e-2, device="cuda")
+    ps, qs = params_of(init), params_of(init)
+    opt, eager = AdamW(ps, lr=lr, state_bits=bits, max_norm=2.0, seed=3), AdamW(qs, lr=2.0 ** -9, state_bits=bits, max_norm=2.0, seed=3)
+    for p, g in zip(ps, grads[0]):
+        p.grad = g.cuda()
+    opt.prepare()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    for k in (1, 2):                            # the eager one's steps, which the captured one takes over
+        for q, g in zip(qs, grads[k]):
+            q.grad = g.cuda()
+        eager.step()
+    opt.load_state_dict(copy.deepcopy(eager.state_dict()))
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 2.0 ** -9
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            p.copy_(q)
+    for k in (3, 4):
+        for p, q, g in zip(ps, qs, grads[k]):
+            p.grad.copy_(g)
+            q.grad = g.cuda()
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), k
+        assert float(opt.grad_norm) == float(eager.grad_norm)
+    assert int(opt.state[ps[1]]["step"]) == 4
+    opt.load_state_dict(AdamW(params_of(init), state_bits=bits).state_dict())        # of one that has not stepped
+    assert not any(m.any() or v.any() for m, v in opt.moments()) and int(opt.state[ps[0]]["step"]) == 0
+
+
+def test_a_parameter_twice_is_refused():
+    p = torch.zeros(8, requires_grad=True)
+    with pytest.raises(ValueError), warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        AdamW([p, p])
 
 
 @pytest.mark.gpu
