@@ -229,7 +229,7 @@ __device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T
       found = true;
       break;
     }
-    before += uniform(sum, 63);
+    before = min(before + uniform(sum, 63), (1 << 30) - 1);     // (more tiles than any launch has: only offsets that fall lead there)
     high = uniform((int)e, nseq - 1 - b0 < 63 ? nseq - 1 - b0 : 63);
     if (b0 == 0) low = uniform((int)s, 0);
   }
@@ -1006,8 +1006,8 @@ int check(PackedAttnArgs& a, int dtype, const long long* strides, int n) {
   a.tiles = (int)std::min<long long>(a.T / BM + a.nseq + 1, 0x7fffffff);
   a.splits = parts_of(a.T, a.nseq, a.Hq, 1);
   a.parts = parts_of(a.T, a.nseq, a.Hkv, a.Hq / a.Hkv);
-  const long long tiles = a.T / BM + a.nseq + 1;
-  if (tiles * a.Hq * 8 > 0x7fffffffLL) return refuse("packed attention: too many rows x heads for one launch");
+  const long long tiles = a.T / BM + a.nseq + 1, threads = std::max(tiles * a.Hq * a.splits * 256, tiles * a.Hkv * a.parts * 512);
+  if (threads > 0xffffffffLL) return refuse("packed attention: (rows / 128 + sequences) x heads are too many for one launch (2^24 / heads at most, half that for the gradients)");
   return 0;
 }
 bool unaligned(std::initializer_list<const void*> ps) {

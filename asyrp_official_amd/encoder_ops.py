@@ -52,6 +52,19 @@ def _strides(t):
     return (a, b) if c == 1 and a > 0 and b > 0 and not (a | b) & 7 and a <= 1 << 23 and not t.data_ptr() & 15 else None
 
 
+def _apart(out, so, t):
+    """No value of `t` lies where `out` is written: their spans do not meet, or they take different columns of the same rows (or of the same heads' blocks).  What is
+    not read in place is copied before."""
+    st = _strides(t)
+    if st is None:
+        return True
+    extent = lambda t, s, axes: sum((t.shape[i] - 1) * s[i] for i in axes) + t.shape[2]  # noqa: E731
+    gap = (out.data_ptr() - t.data_ptr()) // t.element_size()
+    if gap >= extent(t, st, (0, 1)) or -gap >= extent(out, so, (0, 1)):
+        return True
+    return any(so[i] == st[i] and extent(t, st, (1 - i,)) <= gap % so[i] <= so[i] - extent(out, so, (1 - i,)) for i in (0, 1))
+
+
 def _readable(t):
     st = _strides(t)
     if st is not None:
@@ -118,7 +131,7 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
     there: others than these give no defined result, but nothing outside the tensors is touched.)  scale: 1 / sqrt(head_dim) by default.
 
     Returns [tokens, heads, head_dim].  Rows behind the last sequence are zero there and in the gradients.  `out` (without gradients only;
-    the result's type and shape, laid out as q may be) takes the result and keeps what it holds in those rows.  Sums and softmax statistics are float32;
+    the result's type and shape, laid out as q may be, beside q, k and v and not over them) takes the result and keeps what it holds in those rows.  Sums and softmax statistics are float32;
     probabilities are rounded to the inputs' type before they multiply v.  A value that is not finite may reach every row of its own sequence, the
     rows before it included, and no other sequence.  Results do not depend on the order in which the card works."""
     device = _tensor(q, "q", None, _HALF)
@@ -146,8 +159,11 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
         _tensor(out, "out", device, same)
         if grad:
             raise ValueError("out= takes part in no graph: call without it, or under torch.no_grad()")
-        if out.shape != q.shape or _strides(out) is None:
+        so = _strides(out)
+        if out.shape != q.shape or so is None:
             raise ValueError(f"out must be {tuple(q.shape)} with its last axis contiguous, other strides multiples of 8 values and a 16-byte address")
+        if T and not ((so[0] >= (H - 1) * so[1] + D or so[1] >= (T - 1) * so[0] + D) and _apart(out, so, q) and _apart(out, so, k) and _apart(out, so, v)):
+            raise ValueError("out must not overlap itself, q, k or v")
     if grad:
         return _PackedAttention.apply(q, k, v, cu, causal, scale)
     return _attention_forward(q, k, v, cu, causal, scale, out, False)[3]

@@ -249,6 +249,7 @@ def test_library_refuses_what_its_kernels_do_not_take():
                 dict(scale=math.nan), dict(scale=math.inf), dict(sq=(100, 64)), dict(sq=(2 ** 24, 64)), dict(sq=(-128, 64)), dict(ptr=4098), dict(ptr=None)):
         assert call(**bad) == -1, bad
         assert b"packed attention" in lib.asyrp_last_error()
+    assert call(n=2 ** 23, H=2) == -1 and call(n=2 ** 22, H=8, K=2) == -1       # more workgroups than a launch takes
     assert call(T=0) == 0                                              # nothing to do, nothing launched
     assert lib.asyrp_packed_attention_forward(0, None, 4096, 4096, 4096, 4096, 4096, None, None, 4096, 1, None) == -1
     assert lib.asyrp_packed_attention_workspace(None, 0) == -1
@@ -269,6 +270,27 @@ def test_refusals():
     for kw in (dict(q=q.cpu()), dict(cu_seqlens=cu.cpu()), dict(out=q.cpu())):
         with pytest.raises(AsyrpDeviceError):
             ok(**kw)
+
+
+@pytest.mark.gpu
+def test_out_beside_and_over_its_inputs():
+    T, H, D = 70, 4, 16
+    q, k, v, _ = make(T, H, 2, D, torch.float16)
+    cu = offsets([30, 40])
+    want = packed_attention(q, k, v, cu, causal=True)
+    fused = torch.cat([q, k, v, torch.zeros_like(q)], 1)                  # [T, 4 + 2 + 2 + 4, D]
+    qf, kf, vf, of = fused.split([4, 2, 2, 4], 1)
+    assert packed_attention(qf, kf, vf, cu, causal=True, out=of) is of and torch.equal(of, want)
+    planes = torch.stack([q, q]).transpose(1, 2).contiguous().transpose(1, 2)        # heads in front of rows, q behind out
+    assert torch.equal(packed_attention(planes[1], kf, vf, cu, causal=True, out=planes[0]), want)
+    blocks = torch.cat([q, q]).transpose(0, 1).contiguous().transpose(0, 1)          # a head's block holds the rows of q, then of out
+    assert torch.equal(packed_attention(blocks[:T], kf, vf, cu, causal=True, out=blocks[T:]), want)
+    long = torch.cat([q, q])
+    twice = torch.empty(T * H * D, device="cuda", dtype=q.dtype).as_strided((T, H, D), (D, D, 1))
+    for kw in (dict(q=qf, out=qf), dict(q=long[:T], out=long[1:T + 1]), dict(q=long[1:T + 1], out=long[:T]), dict(q=q, k=fused[:, :2], out=fused[:, 1:5]),
+               dict(q=q, k=fused[:, 4:6], out=fused[:, 1:5]), dict(q=q, out=twice), dict(q=q, v=of[:, 2:], out=of)):
+        with pytest.raises(ValueError, match="overlap"):
+            packed_attention(**{**dict(k=k, v=v, cu_seqlens=cu), **kw})
 
 
 def test_reference_gradients_against_differences():
