@@ -974,15 +974,23 @@ hipError_t launch(const PackedAttnArgs& a, bool backward, hipStream_t s) {
 
 // Into how many parts a tile's other axis is dealt: the keys of a query tile (forward, dq: `heads` query heads, shared = 1) and the queries of a key tile (dk / dv:
 // `heads` key / value heads, each `shared` times the queries).  A launch of few tiles leaves CUs idle and ends with its longest workgroup; the
-// parts' fp32 sums cost a write and a read.  Wanted are more workgroups than CUs and eight tiles a part where all rows are one sequence (their
+// parts' fp32 sums cost a write and a read.  Wanted are `want` workgroups and eight tiles a part where all rows are one sequence (their
 // lengths are on the device); many short sequences are left whole.  Forward + backward in us, whole and in parts: causal sequences of 1829 / 379 / 312,
 // 8 heads on 2 of 64: 285 and 110; one of 6000, one head of 128: 511 and 142 (forward 107 and 41); one of 2000, 4 heads on 1 of 128: 363 and 130; 600 / 500, 4 heads
 // of 64: 61 and 52.  (16 heads on 4, 128 wide, 8192 rows: dk and dv in 1 part 1.41 ms, in 2 0.49 ms with their first form; 4 parts are within 1 % of 2.)
-int parts_of(long long T, int nseq, int heads, int shared) {
+int parts_of(long long T, int nseq, int heads, int shared, int want) {
   const long long wgs = std::max<long long>(1, T / BM) * heads;     // full tiles; the ragged ones are light
   int parts = 1;
-  while (parts < 8 && wgs * parts <= 256 && T * shared >= 16LL * BN * parts && T / nseq * shared >= 3 * BN) parts *= 2;
+  while (parts < 8 && wgs * parts < want && T * shared >= 16LL * BN * parts && T / nseq * shared >= 3 * BN) parts *= 2;
   return parts;
+}
+// More workgroups than CUs; under the causal mask, where the longest workgroup has twice the mean's work, as many as the CUs hold (two each) once the sequences are
+// long enough for what the parts cost, and more for the longest.  Forward / both directions in us at 257 and so: one sequence of 16384, 4 heads of 64: 223 / 965 and
+// 187 / 775; 5000, 10 heads of 96: 87 / 407 and 87 / 351; 4000, 9 heads of 128: 78 / 336 and 69 / 299; shorter: three of 1024, 16 heads of 64: 25 / 89 and, were
+// they dealt out so, 33 / 114.  (The kernel of wide heads' dk and dv fills a CU by itself: 257.)
+int wanted(const PackedAttnArgs& a, bool backward) {
+  const long long mean = a.T / a.nseq;
+  return !a.causal || mean < (backward ? 1280 : 2560) ? 257 : mean < 8192 ? 512 : 513;
 }
 // floats of workspace: forward {sums, statistics}; backward {delta, sums of dq and then of dk / dv}
 long long forward_floats(const PackedAttnArgs& a) { return a.splits > 1 ? a.splits * a.T * a.Hq * (a.D + 2LL) : 0; }
@@ -994,7 +1002,7 @@ long long backward_floats(const PackedAttnArgs& a) {
 int refuse(const char* m) { return set_last_error(ASYRP_EINVAL, m); }
 
 // the checks that both directions share, and how their work is dealt out; 0 or the error
-int check(PackedAttnArgs& a, int dtype, const long long* strides, int n) {
+int check(PackedAttnArgs& a, int dtype, const long long* strides, int n, bool backward) {
   if (dtype != ASYRP_F16 && dtype != ASYRP_BF16) return refuse("packed attention takes f16 or bf16 operands");
   if (a.D < 8 || a.D > 128 || a.D % 8) return refuse("packed attention: the head width must be a multiple of 8 from 8 to 128");
   if (a.Hq < 1 || a.Hkv < 1 || a.Hq % a.Hkv) return refuse("packed attention: query heads must be a multiple of key/value heads");
@@ -1004,8 +1012,8 @@ int check(PackedAttnArgs& a, int dtype, const long long* strides, int n) {
     if (strides[i] < 0 || strides[i] % 8 || strides[i] > (i % 2 ? 1LL << 40 : 1LL << 23))
       return refuse("packed attention: strides must be multiples of 8 values, not negative, rows at most 2^23 values apart");
   a.tiles = (int)std::min<long long>(a.T / BM + a.nseq + 1, 0x7fffffff);
-  a.splits = parts_of(a.T, a.nseq, a.Hq, 1);
-  a.parts = parts_of(a.T, a.nseq, a.Hkv, a.Hq / a.Hkv);
+  a.splits = parts_of(a.T, a.nseq, a.Hq, 1, wanted(a, backward));
+  a.parts = parts_of(a.T, a.nseq, a.Hkv, a.Hq / a.Hkv, a.D > 64 ? 257 : wanted(a, backward));
   const long long tiles = a.T / BM + a.nseq + 1, threads = std::max(tiles * a.Hq * a.splits * 256, tiles * a.Hkv * a.parts * 512);
   if (threads > 0xffffffffLL) return refuse("packed attention: (rows / 128 + sequences) x heads are too many for one launch (2^24 / heads at most, half that for the gradients)");
   return 0;
@@ -1033,7 +1041,7 @@ int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, 
   a.o_t = p->out_stride[0]; a.o_h = p->out_stride[1];
   a.fill_tail = fill_tail; a.rest = out_rest;
   const long long st[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.o_t, a.o_h};
-  if (int rc = check(a, p->dtype, st, 8)) return rc;
+  if (int rc = check(a, p->dtype, st, 8, false)) return rc;
   if (a.T == 0) return 0;
   a.partial = workspace;
   a.stats = reinterpret_cast<float2*>(workspace + (a.splits > 1 ? a.splits * a.T * a.Hq * a.D : 0));
@@ -1047,8 +1055,8 @@ int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, 
 int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p, int backward) {
   if (!p) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
-  a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.scale = p->scale;
-  if (int rc = check(a, p->dtype, nullptr, 0)) return rc;
+  a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.causal = p->causal != 0; a.scale = p->scale;
+  if (int rc = check(a, p->dtype, nullptr, 0, backward != 0)) return rc;
   return backward ? backward_floats(a) : forward_floats(a);
 }
 
@@ -1063,7 +1071,7 @@ int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p,
   a.dq_t = (long long)a.Hq * a.D; a.dk_t = a.dv_t = (long long)a.Hkv * a.D;         // the gradients are contiguous
   a.dq_h = a.dk_h = a.dv_h = a.D;
   const long long st[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, a.o_t, a.o_h, a.do_t, a.do_h};
-  if (int rc = check(a, p->dtype, st, 10)) return rc;
+  if (int rc = check(a, p->dtype, st, 10, true)) return rc;
   if (a.T == 0) return 0;
   a.partial = workspace + delta_floats(a);
   if (unaligned({q, k, v, out, d_out, dq, dk, dv}) || ((uintptr_t)out_rest & 15) || !lse || !workspace || ((uintptr_t)workspace & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");

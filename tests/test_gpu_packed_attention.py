@@ -105,6 +105,17 @@ def test_long_and_many(case):
 
 
 @pytest.mark.gpu
+def test_long_causal_sequences_dealt_out_beyond_the_cus():
+    """Over 256 workgroups of 128 rows in sequences of a mean length over 2560: the keys of a query tile go to two of them."""
+    lens = [2700, 2500]
+    q, k, v, do = make(sum(lens), 7, 1, 32, torch.float16, seed=2)
+    got = run(q, k, v, do, offsets(lens), True)
+    want, tol = reference(q, k, v, lens, True, 1 / math.sqrt(32), do)
+    for n in got:
+        check(n, got[n], want[n], tol[n], HALF[torch.float16])
+
+
+@pytest.mark.gpu
 def test_views_of_a_fused_projection_and_odd_layouts_read_the_same():
     lens, H, K, D = [60, 1, 131], 4, 2, 64
     T = sum(lens)
