@@ -588,7 +588,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
 }
 
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them.  A wave's 32 keys and values and both sums stay in its
-// registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 30 us, bound by
+// registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 28 us, bound by
 // latency (four tiles a workgroup).
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAttnArgs p) {
