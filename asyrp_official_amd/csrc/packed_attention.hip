@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 namespace asyrp {
 
@@ -148,6 +149,15 @@ __device__ __forceinline__ void tile_barrier() {
   __syncthreads();
 }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // one instruction; results under 2^-126 are zero
+
+// Calls step(i, place) for i0 <= i < i1 with place = (i - i0) % N as a constant: which of several LDS tiles a step works on is then part of its instructions, not an
+// address to be computed for every read (forward 2 %, dq and dk / dv of 128-wide heads 4 %, at 8192 rows).
+template <int N, typename F, int... P>
+__device__ __forceinline__ void turns(int i0, int i1, F& step, std::integer_sequence<int, P...>) {
+  for (int i = i0; i < i1; i += N) ((i + P < i1 ? step(i + P, std::integral_constant<int, P>()) : void()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void turns(int i0, int i1, F& step) { turns<N>(i0, i1, step, std::make_integer_sequence<int, N>()); }
 
 // a wave's sum, the same in all lanes: within rows of 16 by shifts, then from row to row
 __device__ __forceinline__ int wave_sum(int v) {
@@ -436,27 +446,25 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   tile_barrier();
   w.scores(s0, kt[0], 0, lane);
   w.maximum(s0);
-  int ka = 0, kb = 1, kc = 2, vb = 0;           // key tiles of this, the next and the next but one; parity of the value tile
   // Loads of the tiles behind: the keys run one tile ahead of the values, since a tile's last scores are those of the next one's first half
-  auto fetch = [&] {
-    if (k0 + 2 * BN < kend) ks_.load(k + (long long)(k0 + 2 * BN) * p.k_t, f.len - k0 - 2 * BN, lds_offset(kt[kc]), p.D, tid);
-    if (k0 + BN < kend) vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(vt[vb ^ 1]), p.D, tid);
+  auto fetch = [&](char* keys, char* values) {
+    if (k0 + 2 * BN < kend) ks_.load(k + (long long)(k0 + 2 * BN) * p.k_t, f.len - k0 - 2 * BN, lds_offset(keys), p.D, tid);
+    if (k0 + BN < kend) vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(values), p.D, tid);
   };
-  auto advance = [&] {
-    const int t = ka;
-    ka = kb; kb = kc; kc = t;
-    vb ^= 1;
+  const int whole = open > k0 ? (open - k0) / BN : 0;    // tiles without a mask
+  auto step = [&](int, auto place) {
+    constexpr int a = decltype(place)::value % 3, b = (a + 1) % 3, c = (a + 2) % 3, u = decltype(place)::value & 1;
+    fetch(kt[c], vt[u ^ 1]);
+    w.half(s0, s1, kt[a], 32, vt[u], 0, lane);
+    w.half(s1, s0, kt[b], 0, vt[u], 32, lane);          // (behind the last tile: scores of nothing, which nobody reads)
     k0 += BN;
     tile_barrier();
   };
-  while (k0 < open) {
-    fetch();
-    w.half(s0, s1, kt[ka], 32, vt[vb], 0, lane);
-    w.half(s1, s0, kt[kb], 0, vt[vb], 32, lane);        // (behind the last tile: scores of nothing, which nobody reads)
-    advance();
-  }
+  turns<6>(0, whole, step);
+  // key tiles of this, the next and the next but one; parity of the value tile
+  int ka = whole % 3, kb = (whole + 1) % 3, kc = (whole + 2) % 3, vb = whole & 1;
   while (k0 < kend) {                                   // tiles that end or are cut by the mask
-    fetch();
+    fetch(kt[kc], vt[vb ^ 1]);
     if (k0 < wend) {
       const int last = (p.causal ? min(row, f.len - 1) : f.len - 1) - k0 - 4 * h;    // the last key this column sees
 #pragma unroll
@@ -472,7 +480,11 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
         w.half(s1, s0, kt[kb], 0, vt[vb], 32, lane);
       }
     }
-    advance();
+    const int t = ka;
+    ka = kb; kb = kc; kc = t;
+    vb ^= 1;
+    k0 += BN;
+    tile_barrier();
   }
   const float l = both_halves_sum(w.l);
   if (p.splits > 1) {
@@ -545,14 +557,15 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
     ks_.load(k + (long long)kbeg * p.k_t, f.len - kbeg, lds_offset(kt[0]), p.D, tid);
     vs_.load(v + (long long)kbeg * p.v_t, f.len - kbeg, lds_offset(vt[0]), p.D, tid);
   }
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += BN, buf ^= 1) {
+  auto step = [&](const int i, auto place) {
+    constexpr int buf = decltype(place)::value;
+    const int k0 = kbeg + i * BN;
     tile_barrier();
     if (k0 + BN < kend) {
       ks_.load(k + (long long)(k0 + BN) * p.k_t, f.len - k0 - BN, lds_offset(kt[buf ^ 1]), p.D, tid);
       vs_.load(v + (long long)(k0 + BN) * p.v_t, f.len - k0 - BN, lds_offset(vt[buf ^ 1]), p.D, tid);
     }
-    if (k0 >= wend) continue;
+    if (k0 >= wend) return;
     const int last = (there ? (p.causal ? row : f.len - 1) : -1) - k0 - 4 * h;
     const bool edge = k0 + BN > f.len || f.row0 + wave * 32 + 32 > f.len || (p.causal && k0 + BN - 1 > f.row0 + wave * 32);
 #pragma unroll
@@ -579,7 +592,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
         add_ds<T, DP>(acc, kt[buf], 32 * n + 16 * b, s, b, edge, lane);
       }
     }
-  }
+  };
+  turns<2>(0, (kend - kbeg + BN - 1) / BN, step);
   if (p.splits > 1) {
     if (there) store_cols<DP>(p.partial + ((split * p.T + at) * p.Hq + head) * p.D, acc, p.scale, h, p.D);
     return;
@@ -638,8 +652,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
     }
   };
   if (i0 < i1) fetch(0);
-  int buf = 0;
-  for (int i = i0; i < i1; ++i, buf ^= 1) {
+  auto step = [&](const int i, auto place) {
+    constexpr int buf = decltype(place)::value;
     const int at0 = q0;                                 // first query of this tile
     if (tid < BN) {
       ls[buf][tid] = lv_;
@@ -655,7 +669,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
     // queries that see this lane's key: from `first` on, `seen` of them
     const int first = (p.causal ? row : 0) - at0 - 4 * h, seen = f.len - (p.causal ? row : 0);
     const bool edge = at0 + BN > f.len || (p.causal && at0 < f.row0 + wave * 32 + 31);
-    if (f.row0 + wave * 32 >= f.len) continue;            // a wave behind the sequence's end only loads
+    if (f.row0 + wave * 32 >= f.len) return;            // a wave behind the sequence's end only loads
 #pragma unroll
     for (int n = 0; n < BN / 32; ++n) {
       // 32 queries behind the end, or all before this wave's keys
@@ -694,7 +708,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
         add_ds<T, DP>(dk, qt[buf], 32 * n + 16 * b, g, b, edge, lane);
       }
     }
-  }
+  };
+  turns<2>(i0, i1, step);
   if (p.parts > 1) {
     float* to = p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D;
     if (there) store_cols<DP>(to, dk, p.scale, h, p.D);
@@ -778,10 +793,10 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     }
   };
   if (i0 < i1) fetch(0);
-  int prev = 2, cur = 0, next = 1;                      // slots of the tile before, of this one and of the next
   int here = q0;                                        // first query of this one
-  // the barrier of tile i, and behind it the loads of the next one
-  auto begin = [&](int i) {
+  // The barrier of tile i, and behind it the loads of the next one.  (Slots turn by 3, P's by 2.)
+  auto begin = [&](int i, auto place) {
+    constexpr int cur = decltype(place)::value % 3, next = (cur + 1) % 3;
     if (tid < BN && i < i1) {
       ls[cur][tid] = lv_;
       ds[cur][tid] = dl_;
@@ -795,14 +810,11 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     }
     if (i + 1 < i1) fetch(next);
   };
-  auto end = [&] {
-    const int free = prev;
-    prev = cur; cur = next; next = free;
-  };
   // (each kind of wave has its loop, so that its sums stay where they are; both pass the barriers of i0 .. i1)
   if (i0 < i1 && values) {
-    for (int i = i0; i < i1; ++i) {
-      begin(i);
+    auto step = [&](const int i, auto place) {
+      constexpr int cur = decltype(place)::value % 3, turn = decltype(place)::value & 1;
+      begin(i, place);
       // queries that see this lane's key: from `first` on, `seen` of them
       const int first = (p.causal ? row : 0) - here - 4 * h, seen = f.len - (p.causal ? row : 0);
       const bool edge = here + BN > f.len || (p.causal && here < f.row0 + wave * 32 + 31);
@@ -827,22 +839,22 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          pt[i & 1][wave][2 * n + b][lane] = Pass::pack(s, b);
+          pt[turn][wave][2 * n + b][lane] = Pass::pack(s, b);
           const typename Frag<T>::V pf = pack8<T>(s, b);
 #pragma unroll
           for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(gt[cur], 32 * n + 16 * b, dt, lane), pf, acc[dt]);
         }
       }
-      end();
-    }
-    begin(i1);
+    };
+    turns<6>(i0, i1, step);
+    begin(i1, std::integral_constant<int, 0>());          // (no tile's: its barrier only)
   } else if (i0 < i1) {
-    begin(i0);
-    end();
-    for (int i = i0; i < i1; ++i) {
+    begin(i0, std::integral_constant<int, 0>());
+    auto step = [&](const int i, auto place) {
+      constexpr int prev = decltype(place)::value % 3, turn = decltype(place)::value & 1;
       const int before = here;
       const bool edge = before + BN > f.len || (p.causal && before < f.row0 + wave * 32 + 31);
-      begin(i + 1);
+      begin(i + 1, std::integral_constant<int, (decltype(place)::value + 1) % 6>());
 #pragma unroll
       for (int n = 0; n < BN / 32; ++n) {
         f32x16 g;
@@ -852,7 +864,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
         for (int ks = 0; ks < DP / 16; ++ks) g = Frag<T>::mma(read_rows<T, DP>(gt[prev], 32 * n, ks, lane), kf[ks], g);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const typename Pass::V pr = pt[i & 1][wave][2 * n + b][lane];
+          const typename Pass::V pr = pt[turn][wave][2 * n + b][lane];
 #pragma unroll
           for (int r4 = 2 * b; r4 < 2 * b + 2; ++r4) {
             const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[prev][32 * n + 8 * r4 + 4 * h]);
@@ -862,8 +874,8 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
           add_ds<T, DP>(acc, qt[prev], 32 * n + 16 * b, g, b, edge, lane);
         }
       }
-      end();
-    }
+    };
+    turns<6>(i0, i1, step);
   }
   if (p.parts > 1) {
     if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
