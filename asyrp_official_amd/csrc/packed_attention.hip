@@ -745,7 +745,8 @@ template <> struct Handed<_Float16> {
 // The same for heads wider than 64, where one wave cannot hold both sums, its keys' and values' fragments and the scores in half a SIMD's registers, and a
 // wave alone on its SIMD waits out every exponential: eight waves, two on each SIMD, share the four products of 128 keys.  The first of a pair forms S and P
 // and sums dv; it hands P over through LDS, and the second forms dP and dS and sums dk one tile behind, so that the only wait is the barrier that there is for the
-// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, 277 us so (0.69 PFLOP/s).
+// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, 277 us so (0.69 PFLOP/s), and
+// 3 % less with constant places of its tiles.
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char qt[3][BN * DP * 2], gt[3][BN * DP * 2];
