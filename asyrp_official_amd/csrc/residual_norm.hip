@@ -12,7 +12,7 @@
 // mean and variance are taken in two passes over the registers, so no large sum of squares cancels.  Parameter gradients go
 // through per-workgroup partial sums and a second kernel that adds them in a fixed order: no atomics.
 //
-// 65536 x 2048 in bf16, rms on both sides and a gate: forward 204 us (5.2 TB/s of its 1.07 GB), backward 345 us (4.7 TB/s of 1.61 GB) and 11 us for the partial
+// 65536 x 2048 in bf16, rms on both sides and a gate: forward 204 us (5.2 TB/s of its 1.07 GB), backward 345 us (4.7 TB/s of 1.61 GB) and 9 us for the partial
 // sums; a large copy runs at 4.7 TB/s.  What carried it: sums over a wave by DPP instead of LDS exchanges and arithmetic without cases for absent parts
 // (backward 462 -> 321 us: it had been bound by its instructions), four values a thread, and the next row's loads ahead of the current row.
 #include "kernels.h"
@@ -421,6 +421,13 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(const NormSumAr
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < p.C) {
     long long i = wave;
+    for (; i + 240 < n; i += 256) {                     // sixteen loads on their way
+      float x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k] = from[(i + 16 * k) * step];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s[k & 3] += x[k];
+    }
     for (; i + 48 < n; i += 64)
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[k] += from[(i + 16 * k) * step];
