@@ -124,7 +124,7 @@ typedef struct asyrp_adamw_tensor {
   const void* grad;
   int64_t numel;
   int64_t offset;                 /* of its first value in the flat state arrays: a multiple of 256, spans of 256 do not overlap */
-  int64_t index;                  /* of its step count in `steps` */
+  int64_t index;                  /* of its step count in `steps`; no two tensors share one */
 } asyrp_adamw_tensor;
 #define ASYRP_ADAMW_PARTIALS 1024 /* partial sums per 100 tensors (or part of 100) that asyrp_grad_sumsq writes */
 typedef struct asyrp_adamw {
