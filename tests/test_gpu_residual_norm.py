@@ -296,3 +296,35 @@ def test_refusals():
     for args, kw in (((x, x.cpu()), {}), ((x, x), dict(gate=w.cpu())), ((x, x), dict(before=(w.cpu(), None)))):
         with pytest.raises(AsyrpDeviceError):
             gated_residual_norm(*args, **kw)
+
+
+def test_library_refuses_backward_calls_of_a_forward_that_is_there():
+    """What only the backward refuses, each argument by itself.  (Nothing else is called: the forward would take these addresses for real ones.)"""
+    from asyrp_official_amd import _lib
+    lib = _lib.load()
+
+    def backward(before=1, after=0, gate=None, gates=0, dh=None, dn=4096, dgate=None, dw1=None, db1=None, dw2=None, db2=None, stats=4096, ws=4096):
+        spec = _lib.RESIDUAL_NORM.pack(4, gates, 64, 0, after, before, 0, 0, 1.0, 1e-5)
+        return lib.asyrp_residual_norm_backward(0, spec, 4096, 4096, gate, None, None, None, stats, dh, dn, 4096, 4096, dgate, dw1, db1, dw2, db2, ws, None)
+
+    for bad in (dict(dn=None), dict(before=0), dict(dw1=4096), dict(db1=4096), dict(before=0, dn=None, dh=4096, dw2=4096), dict(before=0, dn=None, dh=4096, db2=4096),
+                dict(dgate=4096), dict(gate=4096), dict(gates=2), dict(ws=None), dict(stats=None), dict(stats=4100)):
+        assert backward(**bad) == -1, bad
+        assert b"residual norm" in lib.asyrp_last_error()
+
+
+def test_made_up_addresses_are_called_only_where_no_gpu_is(monkeypatch):
+    """test_library_refuses_what_its_kernels_do_not_take also calls the forward with arguments that only the backward refuses: harmless without a GPU, a memory
+    fault with one.  It is skipped there."""
+    import conftest
+
+    class Item:
+        def __init__(self, name):
+            self.name, self.nodeid, self.marks = name, "tests/test_gpu_residual_norm.py::" + name, []
+        add_marker = lambda self, m: self.marks.append(m.name)  # noqa: E731
+
+    for count in (0, 1):
+        monkeypatch.setattr(torch.cuda, "device_count", lambda: count)
+        items = [Item("test_library_refuses_what_its_kernels_do_not_take"), Item("test_refusals")]
+        conftest.pytest_collection_modifyitems(items)
+        assert [i.marks for i in items] == [["skip"] if count else [], []]
