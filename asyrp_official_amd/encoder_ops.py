@@ -157,7 +157,7 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:
         _tensor(out, "out", device, same)
-        if grad:
+        if grad or (out.requires_grad and torch.is_grad_enabled()):
             raise ValueError("out= takes part in no graph: call without it, or under torch.no_grad()")
         so = _strides(out)
         if out.shape != q.shape or so is None:
@@ -166,7 +166,10 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
             raise ValueError("out must not overlap itself, q, k or v")
     if grad:
         return _PackedAttention.apply(q, k, v, cu, causal, scale)
-    return _attention_forward(q, k, v, cu, causal, scale, out, False)[3]
+    result = _attention_forward(q, k, v, cu, causal, scale, out, False)[3]
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)          # what an earlier operation keeps of it for its backward is no longer there
+    return result
 
 
 # ---- the seam between two residual blocks ------------------------------------------------------------------------------------------------

@@ -317,3 +317,30 @@ def test_reference_gradients_against_differences():
             up, down = ([t + s * 1e-6 * d if j == i else t for j, t in enumerate((q, k, v))] for s in (1, -1))
             slope = (f(*up) - f(*down)) / 2e-6
             assert abs(slope - float((got[n] * d).sum())) <= 1e-7 * (1 + abs(slope))
+
+
+@pytest.mark.gpu
+def test_autograd_sees_that_out_was_written():
+    q, k, v, _ = make(40, 2, 1, 16, torch.float16)
+    cu, w = offsets([40]), torch.ones(40, 2, 16, device="cuda", dtype=torch.float16, requires_grad=True)
+    base = torch.zeros(40, 4, 16, device="cuda", dtype=torch.float16)
+    for buf in (torch.zeros_like(q), base[:, 1:3]):                    # a buffer, and a part of one
+        packed_attention(q, k, v, cu, out=buf)
+        loss, before = (buf * w).sum(), buf._version                   # keeps buf for its backward
+        with torch.no_grad():
+            packed_attention(q, k, v, cu, causal=True, out=buf)
+        assert buf._version == before + 1
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    leaf = torch.zeros_like(q).requires_grad_()
+    with pytest.raises(ValueError, match="graph"):
+        packed_attention(q, k, v, cu, out=leaf)
+    with pytest.raises(ValueError, match="graph"):
+        packed_attention(q, k, v, cu, out=leaf * 1)
+    want = packed_attention(q, k, v, cu)
+    with torch.no_grad():                                              # as other operations may write to a leaf there
+        before = leaf._version
+        assert torch.equal(packed_attention(q, k, v, cu, out=leaf), want) and leaf._version == before + 1
+    with torch.inference_mode():                                       # tensors made here have no version
+        buf = torch.empty_like(q)
+        assert torch.equal(packed_attention(q, k, v, cu, out=buf), want)
