@@ -4,12 +4,14 @@ The reference's loss runs an image and a text encoder around the DeltaBlock step
 attention and the seams between their residual blocks are the work there that is not a plain matrix product:
   packed_attention      attention over sequences packed behind each other, causal or not, with grouped key / value heads
   gated_residual_norm   norm behind a block, gate, residual sum with its scale, norm in front of the next block
-Both run on the current stream of their tensors' device, keep nothing between calls, and may be captured into a graph.  (As with any autograd function: while a
+Both run on the current stream of their tensors' device, keep nothing between calls, and may be captured into a graph.  Their gradients are those of one backward pass
+(no forward mode, no second derivative), and they cannot be traced.  (As with any autograd function: while a
 backward pass is captured, no graph of the same leaves that was built outside the capture may be alive.)
 """
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .engine import AsyrpDeviceError
@@ -34,6 +36,14 @@ def _tensor(t, name, device, dtypes):
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be one of {[str(v) for v in dtypes]}, got {t.dtype}")
     return d
+
+
+def _refuse_transforms(name, tensors):
+    """The kernels work through addresses: a tangent of an argument would be dropped, and a trace would hold the empty result alone."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{name} cannot be traced")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def _ptr(t):
@@ -153,6 +163,7 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
+    _refuse_transforms("packed_attention", (q, k, v, out))
     cu, causal = cu_seqlens.contiguous(), bool(causal)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if out is not None:
@@ -269,6 +280,7 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, kind="layer", af
     w2, b2 = (None, None) if before is None else (_vector(before[0], "before[0]", width, device), _vector(before[1], "before[1]", width, device))
     if len(shape) != 2:
         x, y = x.reshape(rows, width), y.reshape(rows, width)
+    _refuse_transforms("gated_residual_norm", (x, y, gate, w1, b1, w2, b2))
     args = (x.contiguous(), y.contiguous(), gate, w1, b1, w2, b2)
     spec = _lib.RESIDUAL_NORM.pack(rows, 0 if gate is None else gate.shape[0], width, _KINDS[kind], after is not None, before is not None, _lib.DTYPES[x.dtype],
                                    _lib.DTYPES[y.dtype], residual_scale, eps)

@@ -344,3 +344,20 @@ def test_autograd_sees_that_out_was_written():
     with torch.inference_mode():                                       # tensors made here have no version
         buf = torch.empty_like(q)
         assert torch.equal(packed_attention(q, k, v, cu, out=buf), want)
+
+
+@pytest.mark.gpu
+def test_tangents_and_traces_are_refused():
+    from torch.autograd import forward_ad
+    q, k, v, _ = make(12, 2, 2, 16, torch.float16)
+    cu = offsets([12])
+    for i in range(3):
+        with forward_ad.dual_level():
+            args = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((q, k, v))]
+            with pytest.raises(RuntimeError):
+                packed_attention(*args, cu)
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                packed_attention(*args, cu, out=torch.empty_like(q))
+            assert torch.equal(packed_attention(*(forward_ad.unpack_dual(t).primal for t in args), cu), packed_attention(q, k, v, cu))
+    with pytest.raises(RuntimeError):
+        torch.jit.trace(lambda a: packed_attention(a, k, v, cu), (q,), check_trace=False)

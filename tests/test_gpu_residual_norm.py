@@ -328,3 +328,22 @@ def test_made_up_addresses_are_called_only_where_no_gpu_is(monkeypatch):
         items = [Item("test_library_refuses_what_its_kernels_do_not_take"), Item("test_refusals")]
         conftest.pytest_collection_modifyitems(items)
         assert [i.marks for i in items] == [["skip"] if count else [], []]
+
+
+@pytest.mark.gpu
+def test_tangents_and_traces_are_refused():
+    """Neither passes a derivative or a call on in silence."""
+    from torch.autograd import forward_ad
+    x, y, w = (torch.randn(s, device="cuda") for s in ((5, 16), (5, 16), (16,)))
+    call = lambda x, y, gate, w1, b1, w2, b2: gated_residual_norm(x, y, gate=gate, after=(w1, b1), before=(w2, b2))  # noqa: E731
+    args = [x, y, w, w, w, w, w]
+    want = call(*args)
+    for i in range(7):
+        with forward_ad.dual_level():
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+            with pytest.raises(RuntimeError):
+                call(*dual)
+            got = call(*(forward_ad.unpack_dual(t).primal for t in dual))
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(RuntimeError):
+        torch.jit.trace(lambda a: gated_residual_norm(a, y)[0], (x,), check_trace=False)
