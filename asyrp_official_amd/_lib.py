@@ -40,7 +40,7 @@ ADAMW = struct.Struct("@dddddPPPdPPPPPiiI4x")
 
 
 _P, _F, _I = C.c_void_p, C.c_float, C.c_int
-ABI_VERSION = 9   # include/asyrp.h ASYRP_ABI_VERSION
+ABI_VERSION = 10   # include/asyrp.h ASYRP_ABI_VERSION
 
 _SIGS = {
     "asyrp_abi_version": (C.c_int, []),

@@ -1,6 +1,7 @@
 // packed_attention.hip -- attention over sequences packed behind each other, forward and backward (f16 / bf16 operands, fp32 sums).
 //
-//   S = scale * q k^T (causal: keys <= the query), P = softmax(S), o = P v, lse = log sum exp S
+//   S = scale * q k^T (causal: keys <= the query), P = softmax(S), o = P v
+//   (kept per row for the backward: a reference r of S, in powers of two, and log2 of the sum of 2^(S - r))
 //   dv = P^T do,  dS = P * (do v^T - delta) * scale with delta = rowsum(do * o),  dq = dS k,  dk = dS^T q
 //
 // All three kernels work on v_mfma_f32_32x32x16_{f16,bf16}.  A wave owns 32 queries (forward, dq) or 32 keys (dk/dv) as the COLUMNS of
@@ -43,13 +44,15 @@ template <> struct Frag<__bf16> {
 
 constexpr int BM = 128;      // rows of a workgroup: four waves of 32
 constexpr int BN = 64;       // rows of a tile in LDS
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct PackedAttnArgs {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
   void* rest;                // [T][Hq][D]: what rounding took from o (delta of the unrounded o halves what dq and dk are off); null: not kept
-  float* lse;                // [Hq][T]
+  // [Hq][T] reference and log2 of the sum.  Apart, since a large score less a reference close to it is exact, and their own sum is not: as one float, P was off by
+  // 0.5 % at scores of 1e5 and of any size at 2e7.
+  float2* sums;
   float* delta;              // [Hq][T]
   const int* cu;
   long long T;
@@ -495,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   }
   store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, w.acc, 1.0f / l, h, p.D, there,
                     p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
-  if (there && p.lse && h == 0) p.lse[(long long)head * p.T + f.start + row] = (w.m * w.sc + log2f(l)) * LN2;
+  if (there && p.sums && h == 0) p.sums[(long long)head * p.T + f.start + row] = make_float2(w.m > -INFINITY ? w.m * w.sc : 0.f, log2f(l));
 }
 
 // dq, and delta = rowsum(do * o) for the other kernel.  As the forward, with dP beside S; three products a tile and no running maximum.  172 us for the
@@ -538,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
       for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[ks][j], (float)of[ks][j] + (float)rf[ks][j], delta);
   }
   delta = both_halves_sum(delta);
-  const float lse2 = there ? p.lse[(long long)head * p.T + at] * LOG2E : 0.f;
+  const float2 sum = there ? p.sums[(long long)head * p.T + at] : make_float2(0.f, 0.f);
   if (there && h == 0 && split == 0) p.delta[(long long)head * p.T + at] = delta;
 
   f32x16 acc[DP / 32];
@@ -580,7 +583,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
         g = Frag<T>::mma(read_rows<T, DP>(vt[buf], 32 * n, ks, lane), gf[ks], g);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], sc, -lse2)) * (g[r] - delta);
+      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], sc, -sum.x) - sum.y) * (g[r] - delta);
       if (edge) {
         stay_a_branch();
 #pragma unroll
@@ -607,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char qt[2][BN * DP * 2], gt[2][BN * DP * 2];
-  __shared__ __attribute__((aligned(16))) float ls[2][BN], ds[2][BN];
+  __shared__ __attribute__((aligned(16))) float rs[2][BN], ls[2][BN], ds[2][BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
   const TileAt f = find_tile(p.cu, p.nseq, p.T, tile, p.tiles, lane, p.causal ? BY_WEIGHT_FROM_END : IN_ORDER);
@@ -640,14 +643,15 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   Tile<T, DP> qs, gs;
   qs.init(p.q_t, f.len - qbeg, p.D, tid);
   gs.init(p.do_t, f.len - qbeg, p.D, tid);
-  float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
+  float2 lv_ = make_float2(0.f, 0.f);                   // the next tile's statistics, one row per thread of the first wave
+  float dl_ = 0.f;
   int head = hk * G + i0 / per, q0 = qbeg + i0 % per * BN;      // of the tile that is fetched next
   auto fetch = [&](int buf) {
     qs.load((const T*)p.q + (f.start + q0) * p.q_t + head * p.q_h, f.len - q0, lds_offset(qt[buf]), p.D, tid);
     gs.load((const T*)p.dout + (f.start + q0) * p.do_t + head * p.do_h, f.len - q0, lds_offset(gt[buf]), p.D, tid);
     if (tid < BN) {
       const long long a = (long long)head * p.T + f.start + min(q0 + tid, f.len - 1);
-      lv_ = p.lse[a] * LOG2E;
+      lv_ = p.sums[a];
       dl_ = p.delta[a];
     }
   };
@@ -656,7 +660,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
     constexpr int buf = decltype(place)::value;
     const int at0 = q0;                                 // first query of this tile
     if (tid < BN) {
-      ls[buf][tid] = lv_;
+      rs[buf][tid] = lv_.x;
+      ls[buf][tid] = lv_.y;
       ds[buf][tid] = dl_;
     }
     tile_barrier();
@@ -684,9 +689,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
       }
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * n + 8 * r4 + 4 * h]);
+        const f32x4 ref = *reinterpret_cast<const f32x4*>(&rs[buf][32 * n + 8 * r4 + 4 * h]), lv = *reinterpret_cast<const f32x4*>(&ls[buf][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
+        for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -ref[j]) - lv[j]);
       }
       if (edge) {
         stay_a_branch();
@@ -752,7 +757,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   __shared__ __attribute__((aligned(16))) char qt[3][BN * DP * 2], gt[3][BN * DP * 2];
   typedef Handed<T> Pass;
   __shared__ typename Pass::V pt[2][4][4][64];          // [tile's parity][pair][half of the tile x half of its rows][lane]
-  __shared__ __attribute__((aligned(16))) float ls[3][BN], ds[3][BN];
+  __shared__ __attribute__((aligned(16))) float rs[3][BN], ls[3][BN], ds[3][BN];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, h = lane >> 5;
   const bool values = __builtin_amdgcn_readfirstlane(tid >> 8);          // this wave forms P and dv, its partner dk
   const int part = blockIdx.x % p.parts, hk = blockIdx.x / p.parts % p.Hkv, tile = blockIdx.x / p.parts / p.Hkv, G = p.Hq / p.Hkv;
@@ -783,13 +788,14 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   ts.init(values ? p.do_t : p.q_t, f.len - qbeg, p.D, tid & 255);
   const T* base = values ? (const T*)p.dout + f.start * p.do_t : (const T*)p.q + f.start * p.q_t;
   const long long st = values ? p.do_t : p.q_t, sh = values ? p.do_h : p.q_h;
-  float lv_ = 0.f, dl_ = 0.f;                           // the next tile's statistics, one row per thread of the first wave
+  float2 lv_ = make_float2(0.f, 0.f);                   // the next tile's statistics, one row per thread of the first wave
+  float dl_ = 0.f;
   int head = hk * G + i0 / per, q0 = qbeg + i0 % per * BN;      // of the tile that is fetched next
   auto fetch = [&](int slot) {
     ts.load(base + q0 * st + head * sh, f.len - q0, values ? lds_offset(gt[slot]) : lds_offset(qt[slot]), p.D, tid & 255);
     if (tid < BN) {
       const long long a = (long long)head * p.T + f.start + min(q0 + tid, f.len - 1);
-      lv_ = p.lse[a] * LOG2E;
+      lv_ = p.sums[a];
       dl_ = p.delta[a];
     }
   };
@@ -799,7 +805,8 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   auto begin = [&](int i, auto place) {
     constexpr int cur = decltype(place)::value % 3, next = (cur + 1) % 3;
     if (tid < BN && i < i1) {
-      ls[cur][tid] = lv_;
+      rs[cur][tid] = lv_.x;
+      ls[cur][tid] = lv_.y;
       ds[cur][tid] = dl_;
     }
     tile_barrier();
@@ -828,9 +835,9 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
         for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(qt[cur], 32 * n, ks, lane), kf[ks], s);
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 lv = *reinterpret_cast<const f32x4*>(&ls[cur][32 * n + 8 * r4 + 4 * h]);
+          const f32x4 ref = *reinterpret_cast<const f32x4*>(&rs[cur][32 * n + 8 * r4 + 4 * h]), lv = *reinterpret_cast<const f32x4*>(&ls[cur][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -lv[j]));
+          for (int j = 0; j < 4; ++j) s[4 * r4 + j] = exp2_fast(__builtin_fmaf(s[4 * r4 + j], sc, -ref[j]) - lv[j]);
         }
         if (edge) {
           stay_a_branch();
@@ -954,7 +961,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_fwd_kernel(const PackedA
   }
   *reinterpret_cast<typename Frag<T>::V*>((T*)p.out + row * p.o_t + head * p.o_h + d) = x;
   if (p.rest) *reinterpret_cast<typename Frag<T>::V*>((T*)p.rest + i) = r;
-  if (p.lse && d == 0) p.lse[(long long)head * p.T + row] = (m + log2f(l)) * LN2;
+  if (p.sums && d == 0) p.sums[(long long)head * p.T + row] = make_float2(m > -INFINITY ? m : 0.f, log2f(l));
 }
 
 template <typename T, int DP>
@@ -1045,10 +1052,10 @@ using namespace asyrp;
 extern "C" {
 
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens, void* out,
-                                   float* lse, void* out_rest, float* workspace, int fill_tail, void* stream) {
+                                   float* sums, void* out_rest, float* workspace, int fill_tail, void* stream) {
   if (!p || !cu_seqlens) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
-  a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.cu = cu_seqlens;
+  a.q = q; a.k = k; a.v = v; a.out = out; a.sums = (float2*)sums; a.cu = cu_seqlens;
   a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.causal = p->causal != 0; a.scale = p->scale;
   a.q_t = p->q_stride[0]; a.q_h = p->q_stride[1]; a.k_t = p->k_stride[0]; a.k_h = p->k_stride[1]; a.v_t = p->v_stride[0]; a.v_h = p->v_stride[1];
   a.o_t = p->out_stride[0]; a.o_h = p->out_stride[1];
@@ -1058,7 +1065,7 @@ int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, 
   if (a.T == 0) return 0;
   a.partial = workspace;
   a.stats = reinterpret_cast<float2*>(workspace + (a.splits > 1 ? a.splits * a.T * a.Hq * a.D : 0));
-  if (unaligned({q, k, v, out}) || ((uintptr_t)out_rest & 15) || ((uintptr_t)workspace & 15) || (a.splits > 1 && !workspace)) return refuse("packed attention: tensors must be given and 16-byte aligned");
+  if (unaligned({q, k, v, out}) || ((uintptr_t)out_rest & 15) || ((uintptr_t)sums & 7) || ((uintptr_t)workspace & 15) || (a.splits > 1 && !workspace)) return refuse("packed attention: tensors must be given and 16-byte aligned");
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
   const hipError_t e = p->dtype == ASYRP_F16 ? launch<_Float16>(a, false, (hipStream_t)stream) : launch<__bf16>(a, false, (hipStream_t)stream);
@@ -1074,10 +1081,10 @@ int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p, int ba
 }
 
 int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                    const void* out, const float* lse, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream) {
+                                    const void* out, const float* sums, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream) {
   if (!p || !cu_seqlens) return refuse("packed attention: null argument");
   PackedAttnArgs a{};
-  a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<float*>(lse); a.rest = const_cast<void*>(out_rest); a.dout = d_out; a.delta = workspace; a.dq = dq; a.dk = dk; a.dv = dv; a.cu = cu_seqlens;
+  a.q = q; a.k = k; a.v = v; a.o = out; a.sums = (float2*)sums; a.rest = const_cast<void*>(out_rest); a.dout = d_out; a.delta = workspace; a.dq = dq; a.dk = dk; a.dv = dv; a.cu = cu_seqlens;
   a.T = p->tokens; a.nseq = p->sequences; a.Hq = p->heads; a.Hkv = p->kv_heads; a.D = p->head_dim; a.causal = p->causal != 0; a.scale = p->scale;
   a.q_t = p->q_stride[0]; a.q_h = p->q_stride[1]; a.k_t = p->k_stride[0]; a.k_h = p->k_stride[1]; a.v_t = p->v_stride[0]; a.v_h = p->v_stride[1];
   a.o_t = p->out_stride[0]; a.o_h = p->out_stride[1]; a.do_t = p->dout_stride[0]; a.do_h = p->dout_stride[1];
@@ -1087,7 +1094,7 @@ int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p,
   if (int rc = check(a, p->dtype, st, 10, true)) return rc;
   if (a.T == 0) return 0;
   a.partial = workspace + delta_floats(a);
-  if (unaligned({q, k, v, out, d_out, dq, dk, dv}) || ((uintptr_t)out_rest & 15) || !lse || !workspace || ((uintptr_t)workspace & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");
+  if (unaligned({q, k, v, out, d_out, dq, dk, dv}) || ((uintptr_t)out_rest & 15) || !sums || ((uintptr_t)sums & 7) || !workspace || ((uintptr_t)workspace & 15)) return refuse("packed attention: tensors must be given and 16-byte aligned");
   DeviceGuard g(device);
   if (g.error != hipSuccess) return set_last_error(ASYRP_EHIP, hipGetErrorString(g.error));
   const hipError_t e = p->dtype == ASYRP_F16 ? launch<_Float16>(a, true, (hipStream_t)stream) : launch<__bf16>(a, true, (hipStream_t)stream);

@@ -91,7 +91,7 @@ def _attention_forward(q, k, v, cu, causal, scale, out, train):
     if fill:
         out = q.new_empty(q.shape)
     T, H, D = q.shape
-    lse = q.new_empty((H, T), dtype=torch.float32) if train else None
+    sums = q.new_empty((H, T, 2), dtype=torch.float32) if train else None
     rest = q.new_empty(q.shape) if train else None
     spec = (T, cu.shape[0] - 1, H, k.shape[1], D, causal, _lib.DTYPES[q.dtype], scale, *sq, *sk, *sv, *_strides(out))
     lib, device, packed = _lib.load(), q.get_device(), _lib.PACKED_ATTENTION.pack(*spec, 0, 0)
@@ -100,23 +100,23 @@ def _attention_forward(q, k, v, cu, causal, scale, out, train):
         _lib.check(words)
     ws = q.new_empty((words,), dtype=torch.float32) if words else None
     rc = lib.asyrp_packed_attention_forward(device, packed, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(),
-                                                    out.data_ptr(), _ptr(lse), _ptr(rest), _ptr(ws), fill, _raw_stream(device))
+                                                    out.data_ptr(), _ptr(sums), _ptr(rest), _ptr(ws), fill, _raw_stream(device))
     if rc:
         _lib.check(rc)
-    return q, k, v, out, lse, rest, spec
+    return q, k, v, out, sums, rest, spec
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, causal, scale):
-        q, k, v, out, lse, rest, ctx.spec = _attention_forward(q, k, v, cu, causal, scale, None, True)
-        ctx.save_for_backward(q, k, v, cu, out, lse, rest)
+        q, k, v, out, sums, rest, ctx.spec = _attention_forward(q, k, v, cu, causal, scale, None, True)
+        ctx.save_for_backward(q, k, v, cu, out, sums, rest)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, cu, out, lse, rest = ctx.saved_tensors
+        q, k, v, cu, out, sums, rest = ctx.saved_tensors
         d_out, sd = _readable(d_out)
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
         lib, device, spec = _lib.load(), q.get_device(), _lib.PACKED_ATTENTION.pack(*ctx.spec, *sd)
@@ -124,7 +124,7 @@ class _PackedAttention(torch.autograd.Function):
         if words < 0:
             _lib.check(words)
         ws = q.new_empty((max(4, words),), dtype=torch.float32)
-        rc = lib.asyrp_packed_attention_backward(device, spec, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(), out.data_ptr(), lse.data_ptr(),
+        rc = lib.asyrp_packed_attention_backward(device, spec, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(), out.data_ptr(), sums.data_ptr(),
                                                  rest.data_ptr(), d_out.data_ptr(), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _raw_stream(device))
         if rc:
             _lib.check(rc)

@@ -152,8 +152,9 @@ typedef struct asyrp_adamw {
  *   v8 (round 5): asyrp_config.nominal_batch (was reserved[0]) is validated (0, 1, 2, 32), the reserved words must be zero;
  *                 asyrp_run_edit accepts one hs_coeff tuple per image (n_coeff < 0).  The product library reads no environment variable.
  *   v9: the operators of a training step outside the UNet (asyrp_packed_attention_*, asyrp_residual_norm_*, asyrp_adamw_* and
- *                 asyrp_grad_*); nothing that was there has changed. */
-#define ASYRP_ABI_VERSION 9
+ *                 asyrp_grad_*); nothing that was there has changed.
+ *   v10: asyrp_packed_attention_* keep two floats per row and head (sums) where one was (lse). */
+#define ASYRP_ABI_VERSION 10
 int asyrp_abi_version(void);
 
 /* Last error text of the calling thread ("" if none). */
@@ -294,15 +295,16 @@ int asyrp_sampler_update(int device, const float* x, const float* model_out, int
  *
  * Attention over sequences packed behind each other: sequence i = rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (device, sequences + 1
  * ascending values from 0; values outside [0, tokens] or falling ones are held inside the tensors but give no defined result).
- * lse [heads][tokens] (nullable in the forward) = log sum exp of the scaled scores.  out_rest [tokens][heads][head_dim] contiguous (nullable in both) = what the
+ * sums [heads][tokens][2] (nullable in the forward, 8-byte aligned) = a reference r of the row's scaled scores times log2 e, and log2 of the sum of 2^(score log2 e - r): their
+ * sum times log 2 is the log sum exp of the scaled scores.  out_rest [tokens][heads][head_dim] contiguous (nullable in both) = what the
  * rounding of out took away, so that the backward's rowsum(d_out * out) is that of the unrounded output.  Rows behind the last sequence are set to zero in the gradients
  * and, where fill_tail is not 0, in out.  The gradients are contiguous; workspace: asyrp_packed_attention_workspace() floats of the
  * direction (negative: an error code; 0: none, null will do), 16-byte aligned. */
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                   void* out, float* lse, void* out_rest, float* workspace, int fill_tail, void* stream);
+                                   void* out, float* sums, void* out_rest, float* workspace, int fill_tail, void* stream);
 int64_t asyrp_packed_attention_workspace(const asyrp_packed_attention* p, int backward);
 int asyrp_packed_attention_backward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,
-                                    const void* out, const float* lse, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream);
+                                    const void* out, const float* sums, const void* out_rest, const void* d_out, float* workspace, void* dq, void* dk, void* dv, void* stream);
 
 /* h = residual_scale * x + gate * N1(y), n = N2(h): the norm behind a block, its gate, the residual sum and the norm in front of the next block.
  * gate [gates][width], row r takes gate row r / (rows / gates); weights and biases [width] f32, nullable each; n only where `before`.

@@ -361,3 +361,24 @@ def test_tangents_and_traces_are_refused():
             assert torch.equal(packed_attention(*(forward_ad.unpack_dual(t).primal for t in args), cu), packed_attention(q, k, v, cu))
     with pytest.raises(RuntimeError):
         torch.jit.trace(lambda a: packed_attention(a, k, v, cu), (q,), check_trace=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("size", [1e4, 1e5, 1e6, 2e7])
+def test_large_scores_of_equal_keys(size, dtype, D):
+    """Rows that see one key, or several equal ones: probabilities are 1 / n whatever the scores, in the backward pass too.  (Score sums of the same numbers in the same order are equal to the bit.)"""
+    lens = [1] * 20 + [2, 4] * 6 + [130]
+    q, k, v, do = make(sum(lens), 2, 1, D, dtype, seed=3)
+    c = (size / math.log2(math.e) / math.sqrt(D)) ** 0.5
+    at = 0
+    for n in lens:
+        k[at:at + n] = k[at:at + 1].sign() * (c * (1 + k[at:at + 1].abs() / 8)).to(dtype)
+        q[at:at + n] = (k[at:at + n].expand(n, 2, D).float() * (1 + torch.arange(n, device="cuda")[:, None, None] / 256)).to(dtype)
+        at += n
+    for causal in (True, False):
+        got = run(q, k, v, do, offsets(lens), causal)
+        want, tol = reference(q, k, v, lens, causal, 1 / math.sqrt(D), do)
+        for m in got:
+            check(m, got[m], want[m], tol[m], HALF[dtype])
