@@ -725,25 +725,30 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   }
 }
 
-// P in 16 bits on its way from one wave to another, finer than the operands' type, so that dS is rounded once in effect.  For bf16 operands f16 is; for f16
-// ones P, which is never negative nor over 1 (and a rounding), takes four bits of exponent and twelve of mantissa (2^-13 of its value, from 2^-15 on).
+// P in 16 bits on its way from one wave to another, finer than the operands' type, so that dS is nearly rounded once in effect.  It comes 2^14 times as large, so that what
+// is small has all its bits too: for bf16 operands f16 holds 11 of them from P = 2^-28 on (and under it steps of 2^-38); for f16 ones P, which is never negative, takes five bits of
+// exponent and eleven of mantissa: 12 bits from P = 2^-30 on, steps of 2^-41 under it.  (As f16 without the factor, the dk of keys that few queries see lost its bits: 26 half steps
+// of bf16 where P is 1e-7.)  The clamp is for P that does not belong to its sum: its bits would reach into the neighbour's.
+constexpr float LIFT = 14.f;
 template <typename T> struct Handed;
 template <> struct Handed<__bf16> {
   typedef Frag<_Float16>::V V;
+  static constexpr float LEFT = 0x1p14f;                // get() returns this times P
   static __device__ __forceinline__ V pack(const f32x16& s, int half) { return pack8<_Float16>(s, half); }
   static __device__ __forceinline__ float get(const V& v, int j) { return (float)v[j]; }
 };
 template <> struct Handed<_Float16> {
   typedef unsigned V __attribute__((ext_vector_type(4)));
-  static __device__ __forceinline__ unsigned bits(float p) { return __float_as_uint(p * 0x1p-112f) + 0x400u; }      // exponents 0 .. 15, eleven bits to go
+  static constexpr float LEFT = 1.0f;
+  static __device__ __forceinline__ unsigned bits(float p) { return __float_as_uint(fminf(p, 0x1.ffep14f) * 0x1p-110f) + 0x800u; }      // exponents 0 .. 31, twelve bits to go
   static __device__ __forceinline__ V pack(const f32x16& s, int half) {
     V v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = bits(s[8 * half + 2 * j]) >> 11 | (bits(s[8 * half + 2 * j + 1]) & ~0x7ffu) << 5;
+    for (int j = 0; j < 4; ++j) v[j] = bits(s[8 * half + 2 * j]) >> 12 | (bits(s[8 * half + 2 * j + 1]) & ~0xfffu) << 4;
     return v;
   }
   static __device__ __forceinline__ float get(const V& v, int j) {
-    return __uint_as_float(j & 1 ? v[j / 2] >> 5 & ~0x7ffu : (v[j / 2] & 0xffffu) << 11) * 0x1p112f;
+    return __uint_as_float(j & 1 ? v[j / 2] >> 4 & ~0xfffu : (v[j / 2] & 0xffffu) << 12) * 0x1p96f;
   }
 };
 
@@ -806,7 +811,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     constexpr int cur = decltype(place)::value % 3, next = (cur + 1) % 3;
     if (tid < BN && i < i1) {
       rs[cur][tid] = lv_.x;
-      ls[cur][tid] = lv_.y;
+      ls[cur][tid] = lv_.y - LIFT;                      // P times 2^14
       ds[cur][tid] = dl_;
     }
     tile_barrier();
@@ -885,10 +890,11 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     };
     turns<6>(i0, i1, step);
   }
+  const float unit = values ? 0x1p-14f : p.scale / Pass::LEFT;
   if (p.parts > 1) {
-    if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, values ? 1.0f : p.scale, h, p.D);
+    if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, unit, h, p.D);
   } else {
-    store_cols<T, DP>(values ? (T*)p.dv + at * p.dv_t + hk * p.dv_h : (T*)p.dk + at * p.dk_t + hk * p.dk_h, acc, values ? 1.0f : p.scale, h, p.D, there);
+    store_cols<T, DP>(values ? (T*)p.dv + at * p.dv_t + hk * p.dv_h : (T*)p.dk + at * p.dk_t + hk * p.dk_h, acc, unit, h, p.D, there);
   }
 }
 

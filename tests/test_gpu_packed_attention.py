@@ -382,3 +382,59 @@ def test_large_scores_of_equal_keys(size, dtype, D):
         want, tol = reference(q, k, v, lens, causal, 1 / math.sqrt(D), do)
         for m in got:
             check(m, got[m], want[m], tol[m], HALF[dtype])
+
+
+# ---- other sizes of scores and gradients -------------------------------------------------------------------------------------------------------
+def exact(q, k, v, causal, scale, do, eps):
+    """One sequence in fp64: results, bounds on each element's error, and what rounding one by one adds up to as a root of a sum of squares.
+
+    As above, with the fp32 scores' own errors: a score is a sum of D products, off by at most D 2^-24 of the sum A of their sizes, scale and its product with
+    the score add 4 roundings, and numerator and denominator of a probability both have it: P is off by rho = 2 (D + 4) 2^-24 max A of its value."""
+    q, k, v, do = (t.detach().double().cpu() for t in (q, k, v, do))
+    n, G, D = q.shape[0], q.shape[1] // k.shape[1], q.shape[2]
+    got = {m: torch.zeros_like(t) for m, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+    tol, sq = ({m: torch.zeros_like(t) for m, t in got.items()} for _ in range(2))
+    for h in range(q.shape[1]):
+        Q, K, V, g, j = q[:, h], k[:, h // G], v[:, h // G], do[:, h], h // G
+        s, A = scale * Q @ K.T, scale * Q.abs() @ K.abs().T
+        if causal:
+            late = torch.ones(n, n).triu(1).bool()
+            s, A = s.masked_fill(late, -math.inf), A.masked_fill(late, 0.0)
+        rho = 2 * (D + 4) * 2.0 ** -24 * A.amax(1, keepdim=True)
+        p = torch.softmax(s, 1)
+        o, dp = p @ V, g @ V.T
+        ds = p * (dp - (g * o).sum(1, keepdim=True))
+        eds = eps * (ds.abs() + p * (g * o).abs().sum(1, keepdim=True)) + rho * (ds.abs() + p * (p * dp.abs()).sum(1, keepdim=True))
+        got["o"][:, h], tol["o"][:, h] = o, eps * o.abs() + (eps + rho) * (p @ V.abs())
+        got["dq"][:, h], tol["dq"][:, h], sq["dq"][:, h] = scale * ds @ K, scale * (eds @ K.abs()), scale ** 2 * eps ** 2 * (ds ** 2 @ K ** 2)
+        got["dk"][:, j] += scale * ds.T @ Q
+        tol["dk"][:, j] += scale * (eds.T @ Q.abs())
+        sq["dk"][:, j] += scale ** 2 * eps ** 2 * (ds.T ** 2 @ Q ** 2)
+        got["dv"][:, j] += p.T @ g
+        tol["dv"][:, j] += ((eps + rho) * p).T @ g.abs()
+        sq["dv"][:, j] += eps ** 2 * (p.T ** 2 @ g ** 2)
+    for m in ("dq", "dk", "dv"):
+        tol[m] += eps * got[m].abs()
+    return got, tol, sq
+
+
+RAMPS = [(400, 2, 1, 64, True, 0.125), (400, 2, 2, 64, False, 0.125), (300, 2, 1, 128, True, 0.25), (257, 3, 3, 96, False, 0.05), (333, 2, 1, 40, True, 1.5), (2600, 1, 1, 64, True, 0.125),
+         (2600, 1, 1, 64, False, 0.125), (2100, 2, 1, 128, True, 0.125), (2100, 1, 1, 128, False, 0.125)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16], ids=["bf16"])
+@pytest.mark.parametrize("case", RAMPS, ids=[f"{c[0]}_{c[1]}x{c[2]}x{c[3]}{'c' if c[4] else ''}" for c in RAMPS])
+def test_scores_that_climb_and_fall_along_the_keys(case, dtype):
+    """Scores from -60 to 60 and beyond: every second query's climb from key to key, so that its maximum moves tile after tile (and, where the keys are dealt out, lies in
+    the last part), the others' fall, so that it lies in the first.  Scales other than the default."""
+    n, H, K, D, causal, scale = case
+    q, k, v, do = make(n, H, K, D, torch.float32, seed=n)
+    q, k = 0.3 * q, 0.3 * k
+    q[..., 0] = torch.where(torch.arange(n, device="cuda") % 2 == 0, 8.0, -8.0)[:, None]
+    k[..., 0] = torch.linspace(-60, 60, n, device="cuda")[:, None] / (8 * scale)
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+    got = run(q, k, v, do, offsets([n]), causal, scale)
+    want, tol, _ = exact(q, k, v, causal, scale, do, HALF[dtype])
+    for m in got:
+        check(m, got[m], want[m], tol[m], 1.0)
