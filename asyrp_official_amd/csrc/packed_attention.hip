@@ -325,7 +325,7 @@ __device__ __forceinline__ typename Frag<T>::V pack8(const f32x16& s, int half) 
   return v;
 }
 
-// sums += A * dS for 16 rows of a tile.  dS is rounded to the operands' type, except in the tiles that the mask cuts or the sequence ends in: there it
+// sums += A * dS for 16 rows of a tile.  dS is rounded to the operands' type (f16: under its column's power of two, below), except in the tiles that the mask cuts or the sequence ends in: there it
 // goes in as two terms (its rounded value and the rest).  Under the causal mask those tiles hold the rows with few keys, whose dS is largest, and most
 // of what dq and dk would be off; all others are many to one of them.
 template <typename T, int DP>
@@ -341,6 +341,42 @@ __device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const char* tile,
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = Frag<T>::mma(read_cols<T, DP>(tile, row0, dt, lane), hi, acc[dt]);
 }
+
+// dS on its way into f16 has a power of two for every column (query or key) that keeps what matters of it inside f16's range: gradients of a mean loss over a long
+// sequence put dS at 2^-20 and less, where f16 has few bits or none (without it 4 % of dq at do = 1e-4 and 3000 rows), others over 65504.  It is found as
+// a softmax finds its reference: the first values of a column that are not zero are taken to 2^8, and where later ones pass 2^14 it falls and the sums with it.  All steps are
+// by powers of two, exact.  What is then too small for f16 is 2^-32 of the column's largest.  bf16 has the range of fp32.
+template <typename T> struct Range {
+  static constexpr float up = 1.f, shift = 0.f;
+  template <int N> __device__ __forceinline__ void fit(f32x16&, f32x16 (&)[N]) {}
+  __device__ __forceinline__ float undo() const { return 1.f; }
+};
+template <> struct Range<_Float16> {
+  float up = 1.f, shift = 0.f, limit = 0.f;             // the power of two, its logarithm, what a value may reach under it
+  // `ds` comes times `up`
+  template <int N> __device__ __forceinline__ void fit(f32x16& ds, f32x16 (&acc)[N]) {
+    float t = fabsf(ds[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) t = fmaxf(t, fabsf(ds[r]));
+    if (__any(t > limit)) {
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+      t = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+      // 2^8 over the power of two in t, no more than 2^30 (dS under 2^-44 reaches no f16 value of dq or dk)
+      const int e = t > limit ? min(135 - (int)(__float_as_uint(t) >> 23), 30) : 0;
+      const float f = __uint_as_float((unsigned)(127 + e) << 23);
+      limit = t > limit ? 16384.f : limit;
+      up *= f;
+      shift += (float)e;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] *= f;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+    }
+  }
+  __device__ __forceinline__ float undo() const { return 1.f / up; }
+};
 
 // What a wave of the forward carries from one half tile (32 keys) to the next
 template <typename T, int DP>
@@ -549,6 +585,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+  Range<T> range;
   const float sc = p.scale * LOG2E;
   const int all = p.causal ? min(f.len, f.row0 + BM) : f.len, tiles = (all + BN - 1) / BN;
   const int kbeg = tiles * split / p.splits * BN, kend = min(all, tiles * (split + 1) / p.splits * BN);      // this part of the key tiles
@@ -583,13 +620,14 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
         g = Frag<T>::mma(read_rows<T, DP>(vt[buf], 32 * n, ks, lane), gf[ks], g);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], sc, -sum.x) - sum.y) * (g[r] - delta);
+      for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], sc, -sum.x) - (sum.y - range.shift)) * (g[r] - delta);
       if (edge) {
         stay_a_branch();
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (32 * n + 8 * (r >> 2) + (r & 3) > last) s[r] = 0.f;
       }
+      range.fit(s, acc);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         add_ds<T, DP>(acc, kt[buf], 32 * n + 16 * b, s, b, edge, lane);
@@ -598,10 +636,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
   };
   turns<2>(0, (kend - kbeg + BN - 1) / BN, step);
   if (p.splits > 1) {
-    if (there) store_cols<DP>(p.partial + ((split * p.T + at) * p.Hq + head) * p.D, acc, p.scale, h, p.D);
+    if (there) store_cols<DP>(p.partial + ((split * p.T + at) * p.Hq + head) * p.D, acc, p.scale * range.undo(), h, p.D);
     return;
   }
-  store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale, h, p.D, there);
+  store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale * range.undo(), h, p.D, there);
 }
 
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them.  A wave's 32 keys and values and both sums stay in its
@@ -636,6 +674,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[dt][r] = dv[dt][r] = 0.f;
+  Range<T> range;
   const float sc = p.scale * LOG2E;
   const int qbeg = p.causal ? f.row0 : 0;               // a multiple of BN
   const int per = (f.len - qbeg + BN - 1) / BN, total = per * G;
@@ -703,8 +742,9 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
       for (int r4 = 0; r4 < 4; ++r4) {
         const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[buf][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) g[4 * r4 + j] = s[4 * r4 + j] * (g[4 * r4 + j] - dl[j]);
+        for (int j = 0; j < 4; ++j) g[4 * r4 + j] = s[4 * r4 + j] * (g[4 * r4 + j] - dl[j]) * range.up;
       }
+      range.fit(g, dk);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const typename Frag<T>::V pf = pack8<T>(s, b);
@@ -717,10 +757,10 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
   turns<2>(i0, i1, step);
   if (p.parts > 1) {
     float* to = p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D;
-    if (there) store_cols<DP>(to, dk, p.scale, h, p.D);
+    if (there) store_cols<DP>(to, dk, p.scale * range.undo(), h, p.D);
     if (there) store_cols<DP>(to + p.D, dv, 1.0f, h, p.D);
   } else {
-    store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, p.scale, h, p.D, there);
+    store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, p.scale * range.undo(), h, p.D, there);
     store_cols<T, DP>((T*)p.dv + at * p.dv_t + hk * p.dv_h, dv, 1.0f, h, p.D, there);
   }
 }
@@ -733,9 +773,9 @@ constexpr float LIFT = 14.f;
 template <typename T> struct Handed;
 template <> struct Handed<__bf16> {
   typedef Frag<_Float16>::V V;
-  static constexpr float LEFT = 0x1p14f;                // get() returns this times P
+  static constexpr float LEFT = 0x1p14f;                // get() returns this times P (f16 operands: times `up`)
   static __device__ __forceinline__ V pack(const f32x16& s, int half) { return pack8<_Float16>(s, half); }
-  static __device__ __forceinline__ float get(const V& v, int j) { return (float)v[j]; }
+  static __device__ __forceinline__ float get(const V& v, int j, float) { return (float)v[j]; }
 };
 template <> struct Handed<_Float16> {
   typedef unsigned V __attribute__((ext_vector_type(4)));
@@ -747,8 +787,8 @@ template <> struct Handed<_Float16> {
     for (int j = 0; j < 4; ++j) v[j] = bits(s[8 * half + 2 * j]) >> 12 | (bits(s[8 * half + 2 * j + 1]) & ~0xfffu) << 4;
     return v;
   }
-  static __device__ __forceinline__ float get(const V& v, int j) {
-    return __uint_as_float(j & 1 ? v[j / 2] >> 4 & ~0xfffu : (v[j / 2] & 0xffffu) << 12) * 0x1p96f;
+  static __device__ __forceinline__ float get(const V& v, int j, float up) {     // up is at most 2^30
+    return __uint_as_float(j & 1 ? v[j / 2] >> 4 & ~0xfffu : (v[j / 2] & 0xffffu) << 12) * (0x1p96f * up);
   }
 };
 
@@ -785,6 +825,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
+  Range<T> range;
   const float sc = p.scale * LOG2E;
   const int qbeg = p.causal ? f.row0 : 0;               // a multiple of BN
   const int per = (f.len - qbeg + BN - 1) / BN, total = per * G;
@@ -882,15 +923,17 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
           for (int r4 = 2 * b; r4 < 2 * b + 2; ++r4) {
             const f32x4 dl = *reinterpret_cast<const f32x4*>(&ds[prev][32 * n + 8 * r4 + 4 * h]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) g[4 * r4 + j] = Pass::get(pr, 4 * (r4 - 2 * b) + j) * (g[4 * r4 + j] - dl[j]);
+            for (int j = 0; j < 4; ++j) g[4 * r4 + j] = Pass::get(pr, 4 * (r4 - 2 * b) + j, range.up) * (g[4 * r4 + j] - dl[j]);
           }
-          add_ds<T, DP>(acc, qt[prev], 32 * n + 16 * b, g, b, edge, lane);
         }
+        range.fit(g, acc);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) add_ds<T, DP>(acc, qt[prev], 32 * n + 16 * b, g, b, edge, lane);
       }
     };
     turns<6>(i0, i1, step);
   }
-  const float unit = values ? 0x1p-14f : p.scale / Pass::LEFT;
+  const float unit = values ? 0x1p-14f : p.scale / Pass::LEFT * range.undo();
   if (p.parts > 1) {
     if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, unit, h, p.D);
   } else {

@@ -438,3 +438,40 @@ def test_scores_that_climb_and_fall_along_the_keys(case, dtype):
     want, tol, _ = exact(q, k, v, causal, scale, do, HALF[dtype])
     for m in got:
         check(m, got[m], want[m], tol[m], 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, "mixed"])
+def test_small_gradients_of_long_sequences_in_f16(size, D, causal):
+    """Gradients of a mean loss.  Every term of a sum is rounded by itself, by at most half a step of f16 relative to it, and the stored result once more, or by half its smallest step
+    (2^-25): of independent errors the squares add up, and 1.5 times the root bounds the 2-norm of all of them (an error is uniform up to its bound, so its root mean square is 1 / sqrt(3) of it)."""
+    n, eps = 3000, 2.0 ** -11
+    q, k, v, do = make(n, 1, 1, D, torch.float16, seed=4)
+    sizes = 10.0 ** (-6 * torch.rand(n, 1, 1, generator=torch.Generator().manual_seed(0))).cuda() if size == "mixed" else size
+    do = (do.float() * sizes).half()
+    got = run(q, k, v, do, offsets([n]), causal)
+    want, _, sq = exact(q, k, v, causal, 1 / math.sqrt(D), do, eps)
+    for m in ("dq", "dk", "dv"):
+        bound = (sq[m] + (eps * want[m]) ** 2 + 2.0 ** -50).sum().sqrt()
+        err = (got[m].double().cpu() - want[m]).norm()
+        assert err <= 1.5 * bound, f"{m}: {float(err / bound):.2f} of the bound, {float(err / want[m].norm()):.2e} of the gradient"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_whose_inner_values_pass_f16(D):
+    """dS is over 65504 here, dq and dk are not; sizes grow along the rows of the first sequence, so that what went before is small beside what follows."""
+    lens = [200] + [4] * 16
+    q, k, v, do = make(sum(lens), 2, 1, D, torch.float32, seed=5)
+    grow = torch.cat([torch.logspace(-2, 1, 200), torch.full((64,), 10.0)]).cuda()[:, None, None]
+    q, k, v, do = (t.half() for t in (0.02 * q, 0.02 * k, 0.8 * v * grow, 800 * do * grow))
+    dp = do[-4:, 0].double() @ v[-4:, 0].double().T                    # of the last sequence, whose probabilities are all close to 1 / 4
+    assert ((dp - dp.mean(1, keepdim=True)) / 4).abs().max() > 70000
+    for causal in (True, False):
+        got = run(q, k, v, do, offsets(lens), causal)
+        want, tol = reference(q, k, v, lens, causal, 1 / math.sqrt(D), do)
+        assert max(float(want[m].abs().max()) for m in want) < 60000
+        for m in got:
+            check(m, got[m], want[m], tol[m], HALF[torch.float16])
