@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <utility>
 
 namespace asyrp {
@@ -642,6 +643,11 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
   store_cols<T, DP>((T*)p.dq + at * p.dq_t + head * p.dq_h, acc, p.scale * range.undo(), h, p.D, there);
 }
 
+// P on its way into f16 comes 2^14 times as large, which the exponent has for nothing: it keeps all its bits from 2^-28 on (as it is, from 2^-14: dv of keys that many queries see a little was
+// off by 280 half steps where P is about 1e-7, and by a few in sequences of 65536 rows).  bf16 needs that only where f16 hands it over.
+constexpr float LIFT = 14.f, LIFTED = 0x1p14f;
+template <typename T> constexpr bool is_f16 = std::is_same<T, _Float16>::value;
+
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them.  A wave's 32 keys and values and both sums stay in its
 // registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 28 us, bound by
 // latency (four tiles a workgroup).
@@ -700,7 +706,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
     const int at0 = q0;                                 // first query of this tile
     if (tid < BN) {
       rs[buf][tid] = lv_.x;
-      ls[buf][tid] = lv_.y;
+      ls[buf][tid] = is_f16<T> ? lv_.y - LIFT : lv_.y;
       ds[buf][tid] = dl_;
     }
     tile_barrier();
@@ -755,25 +761,25 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
     }
   };
   turns<2>(i0, i1, step);
+  const float unit_v = is_f16<T> ? 1.f / LIFTED : 1.f, unit_k = p.scale * unit_v * range.undo();
   if (p.parts > 1) {
     float* to = p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D;
-    if (there) store_cols<DP>(to, dk, p.scale * range.undo(), h, p.D);
-    if (there) store_cols<DP>(to + p.D, dv, 1.0f, h, p.D);
+    if (there) store_cols<DP>(to, dk, unit_k, h, p.D);
+    if (there) store_cols<DP>(to + p.D, dv, unit_v, h, p.D);
   } else {
-    store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, p.scale * range.undo(), h, p.D, there);
-    store_cols<T, DP>((T*)p.dv + at * p.dv_t + hk * p.dv_h, dv, 1.0f, h, p.D, there);
+    store_cols<T, DP>((T*)p.dk + at * p.dk_t + hk * p.dk_h, dk, unit_k, h, p.D, there);
+    store_cols<T, DP>((T*)p.dv + at * p.dv_t + hk * p.dv_h, dv, unit_v, h, p.D, there);
   }
 }
 
-// P in 16 bits on its way from one wave to another, finer than the operands' type, so that dS is nearly rounded once in effect.  It comes 2^14 times as large, so that what
+// P in 16 bits on its way from one wave to another, finer than the operands' type, so that dS is nearly rounded once in effect.  It comes 2^14 times as large (LIFT), so that what
 // is small has all its bits too: for bf16 operands f16 holds 11 of them from P = 2^-28 on (and under it steps of 2^-38); for f16 ones P, which is never negative, takes five bits of
 // exponent and eleven of mantissa: 12 bits from P = 2^-30 on, steps of 2^-41 under it.  (As f16 without the factor, the dk of keys that few queries see lost its bits: 26 half steps
 // of bf16 where P is 1e-7.)  The clamp is for P that does not belong to its sum: its bits would reach into the neighbour's.
-constexpr float LIFT = 14.f;
 template <typename T> struct Handed;
 template <> struct Handed<__bf16> {
   typedef Frag<_Float16>::V V;
-  static constexpr float LEFT = 0x1p14f;                // get() returns this times P (f16 operands: times `up`)
+  static constexpr float LEFT = LIFTED;                // get() returns this times P (f16 operands: times `up`)
   static __device__ __forceinline__ V pack(const f32x16& s, int half) { return pack8<_Float16>(s, half); }
   static __device__ __forceinline__ float get(const V& v, int j, float) { return (float)v[j]; }
 };
@@ -933,7 +939,7 @@ __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const Pack
     };
     turns<6>(i0, i1, step);
   }
-  const float unit = values ? 0x1p-14f : p.scale / Pass::LEFT * range.undo();
+  const float unit = values ? 1.f / LIFTED : p.scale / Pass::LEFT * range.undo();
   if (p.parts > 1) {
     if (there) store_cols<DP>(p.partial + ((part * p.T + at) * p.Hkv + hk) * 2 * p.D + (values ? p.D : 0), acc, unit, h, p.D);
   } else {

@@ -423,7 +423,7 @@ RAMPS = [(400, 2, 1, 64, True, 0.125), (400, 2, 2, 64, False, 0.125), (300, 2, 1
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", [torch.bfloat16], ids=["bf16"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("case", RAMPS, ids=[f"{c[0]}_{c[1]}x{c[2]}x{c[3]}{'c' if c[4] else ''}" for c in RAMPS])
 def test_scores_that_climb_and_fall_along_the_keys(case, dtype):
     """Scores from -60 to 60 and beyond: every second query's climb from key to key, so that its maximum moves tile after tile (and, where the keys are dealt out, lies in
