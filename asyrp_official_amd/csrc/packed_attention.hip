@@ -46,11 +46,14 @@ template <> struct Frag<__bf16> {
 constexpr int BM = 128;      // rows of a workgroup: four waves of 32
 constexpr int BN = 64;       // rows of a tile in LDS
 constexpr float LOG2E = 1.4426950408889634f;
+template <typename T> constexpr bool is_f16 = std::is_same<T, _Float16>::value;
+// What rounding took from an output is kept this many times as large: in f16 it would be nothing under outputs of 2^-14 or so.  It is never over the output's own size.
+template <typename T> constexpr float FINER = is_f16<T> ? 2048.f : 1.f;
 
 struct PackedAttnArgs {
   const void *q, *k, *v, *o, *dout;
   void *out, *dq, *dk, *dv;
-  void* rest;                // [T][Hq][D]: what rounding took from o (delta of the unrounded o halves what dq and dk are off); null: not kept
+  void* rest;                // [T][Hq][D]: what rounding took from o, times FINER (delta of the unrounded o halves what dq and dk are off); null: not kept
   // [Hq][T] reference and log2 of the sum.  Apart, since a large score less a reference close to it is exact, and their own sum is not: as one float, P was off by
   // 0.5 % at scores of 1e5 and of any size at 2e7.
   float2* sums;
@@ -285,7 +288,7 @@ __device__ __forceinline__ void store_cols(float* row, const f32x16 (&acc)[DP / 
     }
 }
 // The same in 16 bits: a row's two lanes hold four values of every eight each; they exchange them, so that each stores 16 bytes.  All lanes of the wave
-// come here, `there` says whose row is stored.  `rest`: where given, what the rounding to T took away, rounded itself.
+// come here, `there` says whose row is stored.  `rest`: where given, what the rounding to T took away times FINER, rounded itself.
 template <typename T, int DP>
 __device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float m, int h, int D, bool there, T* rest = nullptr) {
   typedef T T2 __attribute__((ext_vector_type(2)));
@@ -297,7 +300,7 @@ __device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32],
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float a = acc[dt][8 * i + 2 * j] * m, b = acc[dt][8 * i + 2 * j + 1] * m;
-        const T2 v{(T)a, (T)b}, r{(T)(a - (float)v[0]), (T)(b - (float)v[1])};
+        const T2 v{(T)a, (T)b}, r{(T)((a - (float)v[0]) * FINER<T>), (T)((b - (float)v[1]) * FINER<T>)};
         w[0][j] = __builtin_bit_cast(unsigned, v);
         w[1][j] = __builtin_bit_cast(unsigned, r);
       }
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[ks][j], (float)of[ks][j] + (float)rf[ks][j], delta);
+      for (int j = 0; j < 8; ++j) delta = __builtin_fmaf((float)gf[ks][j], __builtin_fmaf((float)rf[ks][j], 1.f / FINER<T>, (float)of[ks][j]), delta);
   }
   delta = both_halves_sum(delta);
   const float2 sum = there ? p.sums[(long long)head * p.T + at] : make_float2(0.f, 0.f);
@@ -644,9 +647,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
 }
 
 // P on its way into f16 comes 2^14 times as large, which the exponent has for nothing: it keeps all its bits from 2^-28 on (as it is, from 2^-14: dv of keys that many queries see a little was
-// off by 280 half steps where P is about 1e-7, and by a few in sequences of 65536 rows).  bf16 needs that only where f16 hands it over.
+// off by 280 half steps where P is about 1e-7).  bf16 needs that only where f16 hands it over.
 constexpr float LIFT = 14.f, LIFTED = 0x1p14f;
-template <typename T> constexpr bool is_f16 = std::is_same<T, _Float16>::value;
 
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them.  A wave's 32 keys and values and both sums stay in its
 // registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 28 us, bound by
@@ -1012,7 +1014,7 @@ __global__ __launch_bounds__(256) void packed_attn_join_fwd_kernel(const PackedA
   for (int j = 0; j < 8; ++j) {
     const float o = s[j] * inv;
     x[j] = (T)o;
-    r[j] = (T)(o - (float)x[j]);
+    r[j] = (T)((o - (float)x[j]) * FINER<T>);
   }
   *reinterpret_cast<typename Frag<T>::V*>((T*)p.out + row * p.o_t + head * p.o_h + d) = x;
   if (p.rest) *reinterpret_cast<typename Frag<T>::V*>((T*)p.rest + i) = r;

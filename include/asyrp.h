@@ -297,7 +297,7 @@ int asyrp_sampler_update(int device, const float* x, const float* model_out, int
  * ascending values from 0; values outside [0, tokens] or falling ones are held inside the tensors but give no defined result).
  * sums [heads][tokens][2] (nullable in the forward, 8-byte aligned) = a reference r of the row's scaled scores times log2 e, and log2 of the sum of 2^(score log2 e - r): their
  * sum times log 2 is the log sum exp of the scaled scores.  out_rest [tokens][heads][head_dim] contiguous (nullable in both) = what the
- * rounding of out took away, so that the backward's rowsum(d_out * out) is that of the unrounded output.  Rows behind the last sequence are set to zero in the gradients
+ * rounding of out took away (f16: times 2^11), so that the backward's rowsum(d_out * out) is that of the unrounded output.  Rows behind the last sequence are set to zero in the gradients
  * and, where fill_tail is not 0, in out.  The gradients are contiguous; workspace: asyrp_packed_attention_workspace() floats of the
  * direction (negative: an error code; 0: none, null will do), 16-byte aligned. */
 int asyrp_packed_attention_forward(int device, const asyrp_packed_attention* p, const void* q, const void* k, const void* v, const int32_t* cu_seqlens,

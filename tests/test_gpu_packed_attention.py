@@ -475,3 +475,16 @@ def test_gradients_whose_inner_values_pass_f16(D):
         assert max(float(want[m].abs().max()) for m in want) < 60000
         for m in got:
             check(m, got[m], want[m], tol[m], HALF[torch.float16])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_of_outputs_among_the_smallest_of_f16(D):
+    """Outputs of about 1e-6 (f16 has steps of 6e-8 there), keys of about 40: rowsum(do * o) is to be that of the unrounded output here too."""
+    q, k, v, do = make(400, 2, 1, D, torch.float32, seed=12)
+    q, k, v, do = (t.half() for t in (0.02 * q, 40 + k, 1e-5 * v, do))
+    for causal in (True, False):
+        got = run(q, k, v, do, offsets([400]), causal)
+        want, tol, _ = exact(q, k, v, causal, 1 / math.sqrt(D), do, HALF[torch.float16])
+        for m in got:
+            check(m, got[m], want[m], tol[m], 1.0)
