@@ -389,12 +389,19 @@ struct FwdWave {
   f32x16 acc[DP / 32];
   float m, l, mx;            // reference and sum of each column, and the maximum of the next half's scores, in the scores' own units
   float sc;
+  static constexpr float LAG = is_f16<T> ? 3.f : 8.f;
 
   __device__ __forceinline__ void scores(f32x16& s, const char* k, int row0, int lane) const {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) s = Frag<T>::mma(read_rows<T, DP>(k, row0, ks, lane), qf[ks], s);
+  }
+  // What the exponentials are taken over, in powers of two.  With f16 operands it lies 7 under the reference, so that probabilities of 2^-21 of the largest still have all
+  // their bits there (as it is, of 2^-14: where a first key takes nearly everything, outputs were off by 2.6 half steps at 2^-19).
+  __device__ __forceinline__ float base() const {
+    const float b = m > -INFINITY ? m * sc : 0.f;       // keys of minus infinity so far: their exponentials are zeros
+    return is_f16<T> ? b - 7.f : b;
   }
   __device__ __forceinline__ void maximum(const f32x16& s) {
     float a = s[0];
@@ -406,9 +413,9 @@ struct FwdWave {
   // Half a tile: the exponentials and sums of `cur` (values from row `vrow` of `v` on) together with the scores `next` of the half behind it (keys from row
   // `krow` of `k` on), so that one's products run under the other's exponentials.
   __device__ __forceinline__ void half(f32x16& cur, f32x16& next, const char* k, int krow, const char* v, int vrow, int lane) {
-    // The reference moves only where a column's maximum has outgrown it by 8 powers of two (and in the first half): the exponentials stay under
-    // 2^8, well inside f16, and most halves leave the sums as they are.
-    if (__any(!((mx - m) * sc <= 8.f))) {
+    // The reference moves only where a column's maximum has outgrown it by LAG powers of two (and in the first half): most halves leave the sums as they are.  The
+    // exponentials stay under 2^8, in f16 under 2^10.  (Both have to leave room: base() is rounded, and that reaches 2^4 at scores of 1e8.)
+    if (__any(!((mx - m) * sc <= LAG))) {
       const float mn = fmaxf(m, mx), keep = m > -INFINITY ? exp2_fast((m - mn) * sc) : 0.f;
       m = mn;
       l *= keep;
@@ -417,7 +424,7 @@ struct FwdWave {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] *= keep;
     }
-    const float ms = m > -INFINITY ? m * sc : 0.f;      // keys of minus infinity so far: their exponentials are zeros
+    const float ms = base();
     scores(next, k, krow, lane);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -533,12 +540,12 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   if (p.splits > 1) {
     const long long at = f.start + row;
     if (there) store_cols<DP>(p.partial + ((split * p.T + at) * p.Hq + head) * p.D, w.acc, 1.0f, h, p.D);
-    if (there && h == 0) p.stats[((long long)split * p.Hq + head) * p.T + at] = make_float2(w.m * w.sc, l);
+    if (there && h == 0) p.stats[((long long)split * p.Hq + head) * p.T + at] = make_float2(w.m > -INFINITY ? w.base() : -INFINITY, l);
     return;
   }
   store_cols<T, DP>((T*)p.out + (f.start + row) * p.o_t + head * p.o_h, w.acc, 1.0f / l, h, p.D, there,
                     p.rest ? (T*)p.rest + ((f.start + row) * p.Hq + head) * p.D : nullptr);
-  if (there && p.sums && h == 0) p.sums[(long long)head * p.T + f.start + row] = make_float2(w.m > -INFINITY ? w.m * w.sc : 0.f, log2f(l));
+  if (there && p.sums && h == 0) p.sums[(long long)head * p.T + f.start + row] = make_float2(w.base(), log2f(l));
 }
 
 // dq, and delta = rowsum(do * o) for the other kernel.  As the forward, with dP beside S; three products a tile and no running maximum.  172 us for the

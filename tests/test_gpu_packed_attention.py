@@ -366,7 +366,7 @@ def test_tangents_and_traces_are_refused():
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
-@pytest.mark.parametrize("size", [1e4, 1e5, 1e6, 2e7])
+@pytest.mark.parametrize("size", [1e4, 1e5, 1e6, 2e7, 1e8])
 def test_large_scores_of_equal_keys(size, dtype, D):
     """Rows that see one key, or several equal ones: probabilities are 1 / n whatever the scores, in the backward pass too.  (Score sums of the same numbers in the same order are equal to the bit.)"""
     lens = [1] * 20 + [2, 4] * 6 + [130]
@@ -488,3 +488,20 @@ def test_gradients_of_outputs_among_the_smallest_of_f16(D):
         want, tol, _ = exact(q, k, v, causal, 1 / math.sqrt(D), do, HALF[torch.float16])
         for m in got:
             check(m, got[m], want[m], tol[m], 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [500, 3000])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+def test_a_heavy_key_whose_value_is_nothing(n, causal):
+    """The first key takes all but 1.3e-6 per key of every query and has a value of zero: outputs are sums of what the others get, all of one size, so that roundings do not average out."""
+    q, k, v, do = make(n, 1, 1, 64, torch.float16, seed=11)
+    q.zero_()
+    k.zero_()
+    q[..., 0], k[0, 0, 0] = 8.0, 13.55
+    v = v.abs()
+    v[0] = 0
+    got = run(q, k, v, do, offsets([n]), causal)
+    want, tol, _ = exact(q, k, v, causal, 0.125, do, HALF[torch.float16])
+    for m in got:
+        check(m, got[m], want[m], tol[m], 1.0)
