@@ -1098,8 +1098,12 @@ int check(PackedAttnArgs& a, int dtype, const long long* strides, int n, bool ba
   a.tiles = (int)std::min<long long>(a.T / BM + a.nseq + 1, 0x7fffffff);
   a.splits = parts_of(a.T, a.nseq, a.Hq, 1, wanted(a, backward));
   a.parts = parts_of(a.T, a.nseq, a.Hkv, a.Hq / a.Hkv, a.D > 64 ? 257 : wanted(a, backward));
-  const long long tiles = a.T / BM + a.nseq + 1, threads = std::max(tiles * a.Hq * a.splits * 256, tiles * a.Hkv * a.parts * 512);
-  if (threads > 0xffffffffLL) return refuse("packed attention: (rows / 128 + sequences) x heads are too many for one launch (2^24 / heads at most, half that for the gradients)");
+  // a launch has fewer than 2^32 threads: 256 a workgroup of the forward, of dq and of dk / dv of narrow heads, 512 of those of wide ones
+  const long long tiles = a.T / BM + a.nseq + 1, most = 0xffffffffLL;
+  if (a.Hq > most / 256 / a.splits / tiles)
+    return refuse("packed attention: (rows / 128 + sequences) x query heads are too many for one launch (2^24 at most, parts of long sequences counted)");
+  if (backward && a.Hkv > most / (a.D > 64 ? 512 : 256) / a.parts / tiles)
+    return refuse("packed attention: (rows / 128 + sequences) x key / value heads are too many for one launch (2^24 at most, heads wider than 64 twice and parts of long sequences counted)");
   return 0;
 }
 bool unaligned(std::initializer_list<const void*> ps) {

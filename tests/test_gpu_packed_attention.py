@@ -505,3 +505,21 @@ def test_a_heavy_key_whose_value_is_nothing(n, causal):
     want, tol, _ = exact(q, k, v, causal, 0.125, do, HALF[torch.float16])
     for m in got:
         check(m, got[m], want[m], tol[m], 1.0)
+
+
+def test_launch_limits_are_those_of_each_direction():
+    """The workspace query launches nothing.  2^32 - 1 threads are one launch's most: 256 a workgroup of 128 rows and query head (forward, dq), or of a key / value head (dk and dv of heads up to 64),
+    512 of one of wider heads; every sequence may need a workgroup of its own."""
+    from asyrp_official_amd import _lib
+    lib = _lib.load()
+    most = 2 ** 24 - 1                                                  # workgroups of 256 threads, one of which the launch keeps for itself
+
+    def words(n, H, K, D, backward):
+        return lib.asyrp_packed_attention_workspace(_lib.PACKED_ATTENTION.pack(0, n, H, K, D, 0, _lib.F16, 1.0, *([H * D, D] * 5)), backward)
+
+    for D, H, K, backward, n in ((64, 1, 1, 0, most - 1), (128, 1, 1, 0, most - 1), (64, 1, 1, 1, most - 1), (128, 1, 1, 1, 2 ** 23 - 2), (64, 4, 4, 0, 2 ** 22 - 2), (128, 4, 1, 1, 2 ** 22 - 2),
+                                 (128, 4, 4, 1, 2 ** 21 - 2), (128, 2, 1, 1, 2 ** 23 - 2)):
+        assert words(n, H, K, D, backward) >= 0, (D, H, K, backward)
+        assert words(n + 1, H, K, D, backward) == -1, (D, H, K, backward)
+        assert b"too many for one launch" in lib.asyrp_last_error()
+    assert words(2 ** 31 - 1, 2 ** 31 - 1, 1, 8, 0) == -1
