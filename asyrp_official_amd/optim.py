@@ -164,37 +164,50 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Takes what state_dict() of an optimiser with the same state_bits gave.  Moments, step counts and a learning rate on the device that are there
-        already take their values in place, so that a captured step goes on with what was loaded."""
-        saved, groups = state_dict["state"], state_dict["param_groups"]
+        already take their values in place, so that a captured step goes on with what was loaded.  What does not fit is refused before anything has changed."""
+        taken = {}
+        # the state does not go through the base class, which would convert it to the parameters' type: it is taken out behind all hooks in front, and
+        # put in place in front of all hooks behind
+        front = self.register_load_state_dict_pre_hook(lambda _, sd: taken.update(self._take_state(sd)) or {**sd, "state": {}})
+        behind = self.register_load_state_dict_post_hook(lambda _: self._put_state(**taken), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            front.remove()
+            behind.remove()
+
+    def _take_state(self, sd):
+        """What _put_state needs of a state dict and of what is there, or ValueError."""
+        saved, groups = sd["state"], sd["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("loaded state dict has other parameter groups")
         want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
-        pairs = [(i, p) for g, mine in zip(groups, self.param_groups) for i, p in zip(g["params"], mine["params"])]
-        for i, p in pairs:
+        for i, p in [(i, p) for g, mine in zip(groups, self.param_groups) for i, p in zip(g["params"], mine["params"])]:
             st = saved.get(i)
             if not st:
                 continue
             if set(st) != want or tuple(st["exp_avg"].shape) != tuple(p.shape) or tuple(st["exp_avg_sq"].shape) != tuple(p.shape) \
                     or (st["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
                 raise ValueError(f"loaded state of parameter {i} is not one of AdamW with {self.state_bits}-bit moments and shape {tuple(p.shape)}")
-        moments, norm, rates = self._moments, self.grad_norm, [g["lr"] for g in self.param_groups]
-        super().load_state_dict({"state": {}, "param_groups": groups})
+        return dict(saved=saved, ids=[g["params"] for g in groups], moments=self._moments, norm=self.grad_norm, rates=[g["lr"] for g in self.param_groups])
+
+    @torch.no_grad()
+    def _put_state(self, saved, ids, moments, norm, rates):
         self._moments, self.grad_norm = moments, norm
-        with torch.no_grad():
-            for g, lr in zip(self.param_groups, rates):
-                if isinstance(lr, torch.Tensor) and lr.is_cuda:
-                    lr.fill_(float(g["lr"]))
-                    g["lr"] = lr
-            for k, mo in list(moments.items()):
-                if not mo.of(self.param_groups[k]["params"]):
-                    del moments[k]
-                    continue
-                for i, p in enumerate(mo.params):
-                    views, st = mo.views(i), saved.get(groups[k]["params"][i]) or {}
-                    for key, view in views.items():
-                        view.copy_(torch.as_tensor(st[key]).reshape(view.shape)) if key in st else view.zero_()
-                    self.state[p] = views
-        for i, p in pairs:
+        for g, lr in zip(self.param_groups, rates):
+            if isinstance(lr, torch.Tensor) and lr.is_cuda:
+                lr.fill_(float(g["lr"]))
+                g["lr"] = lr
+        for k, mo in list(moments.items()):
+            if not mo.of(self.param_groups[k]["params"]):
+                del moments[k]
+                continue
+            for i, p in enumerate(mo.params):
+                views, st = mo.views(i), saved.get(ids[k][i]) or {}
+                for key, view in views.items():
+                    view.copy_(torch.as_tensor(st[key]).reshape(view.shape)) if key in st else view.zero_()
+                self.state[p] = views
+        for i, p in [(i, p) for mine, g in zip(ids, self.param_groups) for i, p in zip(mine, g["params"])]:
             if saved.get(i) and p not in self.state:
                 self.state[p] = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in saved[i].items()}
 

@@ -516,3 +516,30 @@ def test_library_refuses_what_its_kernels_do_not_take():
     assert lib.asyrp_adamw_moments(0, 4096, 4096, 4096, 4096, 100, 4096, 4096, None) == -1
     assert lib.asyrp_adamw_moments(0, None, 4096, 4096, 4096, 256, 4096, 4096, None) == -1
     assert lib.asyrp_adamw_moments(0, None, None, None, None, 0, None, None, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("stepped", [False, True], ids=["fresh", "stepped"])
+def test_hooks_of_a_load_see_the_state(bits, stepped):
+    """A hook in front may edit or replace what is loaded, one behind sees what was; both come off again."""
+    src, _ = trained(bits)
+    dst, ps = trained(bits, steps=5) if stepped else trained(bits, steps=0)
+    seen = []
+
+    def front(opt, sd):
+        assert opt is dst and set(sd["state"]) == {0, 1, 2}
+        return {**sd, "state": {i: {**st, "step": torch.full_like(st["step"], 7)} for i, st in sd["state"].items() if i != 1}}
+
+    front_handle = dst.register_load_state_dict_pre_hook(front)
+    behind = dst.register_load_state_dict_post_hook(lambda opt: seen.append([int(opt.state[p]["step"]) if opt.state.get(p) else 0 for p in ps]))
+    dst.load_state_dict(src.state_dict())
+    assert seen == [[7, 0, 7]]
+    for (a, b), (c, d) in zip(dst.moments(), src.moments()):
+        keep = torch.ones_like(a, dtype=torch.bool)
+        keep[512:768] = False                                          # the second of three parameters of 300, 35 and 256 values: its moments were left out
+        assert torch.equal(a[keep], c[keep]) and torch.equal(b[keep], d[keep]) and not a[~keep].any() and not b[~keep].any()
+    front_handle.remove()
+    behind.remove()
+    dst.load_state_dict(src.state_dict())
+    assert len(seen) == 1 and [int(dst.state[p]["step"]) for p in ps] == [3, 3, 3]
