@@ -181,13 +181,16 @@ class AdamW(torch.optim.Optimizer):
         saved, groups = sd["state"], sd["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("loaded state dict has other parameter groups")
-        want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
         for i, p in [(i, p) for g, mine in zip(groups, self.param_groups) for i, p in zip(g["params"], mine["params"])]:
             st = saved.get(i)
             if not st:
                 continue
-            if set(st) != want or tuple(st["exp_avg"].shape) != tuple(p.shape) or tuple(st["exp_avg_sq"].shape) != tuple(p.shape) \
-                    or (st["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
+            want = {"exp_avg": tuple(p.shape), "exp_avg_sq": tuple(p.shape)}
+            if self.state_bits == 8:
+                want["exp_avg_scale"] = want["exp_avg_sq_scale"] = (-(-p.numel() // BLOCK),)
+            codes = [k for k in st if k != "step" and isinstance(st[k], torch.Tensor) and st[k].dtype == torch.uint8]
+            if set(st) != {"step", *want} or torch.as_tensor(st["step"]).numel() != 1 or any(tuple(torch.as_tensor(st[k]).shape) != shape for k, shape in want.items()) \
+                    or len(codes) != (4 if self.state_bits == 8 else 0):
                 raise ValueError(f"loaded state of parameter {i} is not one of AdamW with {self.state_bits}-bit moments and shape {tuple(p.shape)}")
         return dict(saved=saved, ids=[g["params"] for g in groups], moments=self._moments, norm=self.grad_norm, rates=[g["lr"] for g in self.param_groups])
 

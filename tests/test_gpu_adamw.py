@@ -543,3 +543,19 @@ def test_hooks_of_a_load_see_the_state(bits, stepped):
     behind.remove()
     dst.load_state_dict(src.state_dict())
     assert len(seen) == 1 and [int(dst.state[p]["step"]) for p in ps] == [3, 3, 3]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_load_that_is_refused_changes_nothing(bits):
+    src, _ = trained(bits)
+    opt, ps = trained(bits, steps=5)
+    opt.param_groups[0]["lr"] = 0.25
+    want = [t.clone() for pair in opt.moments() for t in pair]
+    good = src.state_dict()
+    for key in ("exp_avg", "exp_avg_sq", "step") + (("exp_avg_scale", "exp_avg_sq_scale") if bits == 8 else ()):
+        bad = {**good, "state": {i: {**st, key: torch.zeros(3, device="cuda", dtype=st[key].dtype)} if i == 2 else st for i, st in good["state"].items()}}
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        assert all(torch.equal(a, b) for a, b in zip(want, [t for pair in opt.moments() for t in pair])), key
+        assert opt.param_groups[0]["lr"] == 0.25 and [int(opt.state[p]["step"]) for p in ps] == [5, 5, 5]
