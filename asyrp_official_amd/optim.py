@@ -4,6 +4,7 @@ The reference steps its DeltaBlock with a torch optimiser (diffusion_latent.py:2
     opt = AdamW(model.layer_0.parameters(), lr=1e-4, state_bits=8, max_norm=1.0)
     opt.zero_grad(); loss.backward(); opt.step()
 """
+import math
 import operator
 import struct
 
@@ -215,6 +216,22 @@ class AdamW(torch.optim.Optimizer):
                 self.state[p] = {k: t.detach().clone() if isinstance(t, torch.Tensor) else t for k, t in saved[i].items()}
 
     # ---- the step --------------------------------------------------------------------------------------
+    @staticmethod
+    def _hyper(g, device):
+        """((lr, address of lr on the device), (beta1, beta2, eps, weight decay)) of a group as it is now, or ValueError: before anything is launched for any group."""
+        lr, at = g["lr"], 0
+        if isinstance(lr, torch.Tensor) and lr.is_cuda:
+            if lr.dtype != torch.float32 or lr.device != device or lr.numel() != 1:
+                raise ValueError(f"lr as a device tensor must be one float32 value on {device}")
+            lr, at = 0.0, lr.data_ptr()
+        (b1, b2), eps, decay = g["betas"], float(g["eps"]), float(g["weight_decay"])
+        lr, b1, b2 = float(lr), float(b1), float(b2)
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"betas must lie in [0, 1), got {g['betas']}")
+        if not (math.isfinite(lr) and 0.0 <= eps < math.inf and math.isfinite(decay)):
+            raise ValueError(f"lr, eps and weight_decay must be finite and eps not negative, got {lr}, {eps}, {decay}")
+        return (lr, at), (b1, b2, eps, decay)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -242,27 +259,24 @@ class AdamW(torch.optim.Optimizer):
                 flat, params = by_type.setdefault(p.dtype, ([], []))
                 flat += (p.data_ptr(), grad.data_ptr(), n, at, i)
                 params.append(p)
-            todo += [(g, mo, _lib.DTYPES[dtype], len(params), struct.pack(f"{len(flat)}q", *flat), params) for dtype, (flat, params) in by_type.items()]
+            if by_type:
+                lr, hyper = self._hyper(g, device)
+                todo += [(lr, hyper, mo, _lib.DTYPES[dtype], len(params), struct.pack(f"{len(flat)}q", *flat), params) for dtype, (flat, params) in by_type.items()]
         if not todo:
             return loss
         sumsq, clip = None, (0, 0.0, 0, 0)
         if self.max_norm is not None:
-            counts = [-(-n // _lib.ADAMW_TABLE) * _lib.ADAMW_PARTIALS for _, _, _, n, _, _ in todo]
+            counts = [-(-n // _lib.ADAMW_TABLE) * _lib.ADAMW_PARTIALS for _, _, _, _, n, _, _ in todo]
             sumsq = torch.empty(sum(counts), device=device, dtype=torch.float64)
             if self.grad_norm is None or self.grad_norm.device != device:
                 self.grad_norm = torch.zeros((), device=device, dtype=torch.float32)
             at = sumsq.data_ptr()
             clip = (at, self.max_norm, self.grad_norm.data_ptr(), sum(counts))
-            for (_, _, dtype, n, table, _), c in zip(todo, counts):
+            for (_, _, _, dtype, n, table, _), c in zip(todo, counts):
                 _lib.check(lib.asyrp_grad_sumsq(device.index, table, n, dtype, at, stream))
                 at += 8 * c
-        for g, mo, dtype, n, table, params in todo:
-            lr, lr_device = g["lr"], 0
-            if isinstance(lr, torch.Tensor) and lr.is_cuda:
-                if lr.dtype != torch.float32 or lr.device != device:
-                    raise ValueError(f"lr as a device tensor must be float32 on {device}")
-                lr, lr_device = 0.0, lr.data_ptr()
-            spec = _lib.ADAMW.pack(float(lr), *g["betas"], g["eps"], g["weight_decay"], lr_device, mo.steps.data_ptr(), *clip[:3], mo.m.data_ptr(), mo.v.data_ptr(),
+        for (lr, lr_device), hyper, mo, dtype, n, table, params in todo:
+            spec = _lib.ADAMW.pack(lr, *hyper, lr_device, mo.steps.data_ptr(), *clip[:3], mo.m.data_ptr(), mo.v.data_ptr(),
                                    *((mo.me.data_ptr(), mo.ve.data_ptr()) if mo.bits == 8 else (0, 0)), clip[3], mo.bits, self.seed)
             scratch = torch.empty(4 * (n + 1) + n, device=device, dtype=torch.float32)
             _lib.check(lib.asyrp_adamw_step(device.index, spec, table, n, dtype, scratch.data_ptr(), stream))

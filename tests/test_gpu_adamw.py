@@ -559,3 +559,22 @@ def test_a_load_that_is_refused_changes_nothing(bits):
             opt.load_state_dict(bad)
         assert all(torch.equal(a, b) for a, b in zip(want, [t for pair in opt.moments() for t in pair])), key
         assert opt.param_groups[0]["lr"] == 0.25 and [int(opt.state[p]["step"]) for p in ps] == [5, 5, 5]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_that_is_refused_changes_nothing(bits):
+    """A value of the second group that the step does not take is found before the first group has moved."""
+    for key, bad in (("lr", math.nan), ("lr", torch.tensor(1e-3, device="cuda", dtype=torch.float64)), ("lr", torch.tensor(math.inf)), ("betas", (0.9, 1.0)), ("betas", (math.nan, 0.9)), ("eps", -1.0),
+                     ("weight_decay", math.inf)):
+        ps = params_of(tensors([(40,), (50,)]))
+        opt = AdamW([{"params": ps[:1]}, {"params": ps[1:]}], state_bits=bits, max_norm=1.0)
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        want = [p.detach().clone() for p in ps] + [t.clone() for pair in opt.moments() for t in pair]
+        opt.param_groups[1][key] = bad
+        with pytest.raises(ValueError):
+            opt.step()
+        assert all(torch.equal(a, b) for a, b in zip(want, [p.detach() for p in ps] + [t for pair in opt.moments() for t in pair])), (key, bad)
+        assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
