@@ -370,7 +370,9 @@ int asyrp_adamw_step(int device, const asyrp_adamw* c, const asyrp_adamw_tensor*
   if (int rc = check(tensors, n, dtype)) return rc;
   if (!c || (n > 0 && (!scratch || !c->steps))) return refuse("AdamW: null argument");
   if (c->state_bits != 32 && c->state_bits != 8) return refuse("AdamW: states are kept in 32 or 8 bits");
-  if (n > 0 && (!c->exp_avg || !c->exp_avg_sq || (c->state_bits == 8 && (!c->exp_avg_scale || !c->exp_avg_sq_scale)))) return refuse("AdamW: null state");
+  // (tensors without values have a step count and no moments)
+  const bool any = std::any_of(tensors, tensors + n, [](const asyrp_adamw_tensor& t) { return t.numel > 0; });
+  if (any && (!c->exp_avg || !c->exp_avg_sq || (c->state_bits == 8 && (!c->exp_avg_scale || !c->exp_avg_sq_scale)))) return refuse("AdamW: null state");
   if (((uintptr_t)c->exp_avg | (uintptr_t)c->exp_avg_sq | (uintptr_t)scratch) & 15) return refuse("AdamW: states must be 16-byte aligned");
   if (!(c->beta1 >= 0 && c->beta1 < 1 && c->beta2 >= 0 && c->beta2 < 1) || !(c->eps >= 0) || !std::isfinite(c->eps) || !std::isfinite(c->weight_decay) || !std::isfinite(c->lr))
     return refuse("AdamW: betas must lie in [0, 1), eps, lr and weight decay must be finite");

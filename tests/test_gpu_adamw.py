@@ -578,3 +578,17 @@ def test_a_step_that_is_refused_changes_nothing(bits):
             opt.step()
         assert all(torch.equal(a, b) for a, b in zip(want, [p.detach() for p in ps] + [t for pair in opt.moments() for t in pair])), (key, bad)
         assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_group_of_nothing_but_empty_parameters_steps(bits):
+    e = torch.zeros(0, 3, device="cuda", requires_grad=True)
+    p = torch.ones(5, device="cuda", requires_grad=True)
+    opt = AdamW([{"params": [e]}, {"params": [p]}], state_bits=bits, max_norm=1.0)
+    e.grad, p.grad = torch.zeros_like(e), torch.ones_like(p)
+    opt.step()
+    assert int(opt.state[e]["step"]) == 1 and int(opt.state[p]["step"]) == 1 and not torch.equal(p.detach(), torch.ones_like(p))
+    alone = AdamW([e], state_bits=bits)
+    alone.step()
+    assert int(alone.state[e]["step"]) == 1 and [t.numel() for t in alone.moments()[0]] == [0, 0]
