@@ -592,3 +592,91 @@ def test_a_group_of_nothing_but_empty_parameters_steps(bits):
     alone = AdamW([e], state_bits=bits)
     alone.step()
     assert int(alone.state[e]["step"]) == 1 and [t.numel() for t in alone.moments()[0]] == [0, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,half", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)], ids=["bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 255, 700, 4500])
+def test_8_bit_moments_of_16_bit_parameters(n, dtype, half):
+    """The moments are those of the gradients' values, code for code; a parameter is off by half a step of its type from the fp64 step that starts at what it held."""
+    import numpy as np
+    f, lr = np.float32, 1e-2
+    (p,) = params_of(tensors([(n,)], dtype))
+    opt = AdamW([p], lr=lr, state_bits=8, seed=77)
+    m, v = np.zeros(n, f), np.zeros(n, f)
+    for k in range(1, 4):
+        g = (tensors([(n,)], seed=k)[0] * 10.0 ** torch.linspace(-3, 1, n)).to(dtype)
+        if k == 2:
+            g[::3] = 0
+        p.grad, before = g.cuda(), p.detach().double().cpu().numpy()
+        opt.step()
+        g = g.float().numpy()
+        m = m * f(0.9) + g * f(1 - 0.9)
+        v = v * f(0.999) + (g * g) * f(1 - 0.999)
+        up = (m.astype(np.float64) / (1 - 0.9 ** k)) / (np.sqrt(v.astype(np.float64) / (1 - 0.999 ** k)) + 1e-8)
+        want = before * (1 - lr * 1e-2) - lr * up
+        # half a step of the stored value (where it is under the type's normal range: of 2^-24 or less), and fp32 arithmetic as in the test above
+        assert np.all(np.abs(p.detach().double().cpu().numpy() - want) <= half * np.abs(want) + 2.0 ** -25 + 4 * U * (np.abs(want) + 1) + lr * 200 * U * np.abs(up))
+        for b in range(0, n, 256):
+            c = [coins(i, 77, k) for i in range(b, min(n, b + 256))]
+            km, _ = keep8(np.abs(m[b:b + 256]), [x[0] for x in c], 16)
+            kv, unit = keep8(v[b:b + 256], [x[1] for x in c], 32)
+            m[b:b + 256] = np.where(m[b:b + 256] < 0, -np.array(km), km).astype(f)
+            v[b:b + 256] = np.maximum(kv, unit).astype(f)
+        gm, gv = (t[:n].cpu().numpy() for t in opt.moments()[0])
+        assert np.array_equal(gm, m) and np.array_equal(gv, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_addresses_that_no_wide_load_may_take(dtype, bits):
+    """A parameter, its gradient or both one value behind a wide address: equal to the bit to the aligned run, and nothing beside them moves."""
+    n = 2 * 4096 + 809
+    init, grads = tensors([(n,)], dtype)[0], [tensors([(n,)], dtype, seed=60 + k)[0] for k in range(3)]
+
+    def go(shift_p, shift_g):
+        pads = [torch.full((n + 9,), 3.0, device="cuda", dtype=dtype) for _ in range(2)]
+        p, g = (t[s:s + n] for t, s in zip(pads, (shift_p, shift_g)))
+        p = p.copy_(init).requires_grad_()
+        opt = AdamW([p], lr=1e-2, state_bits=bits, seed=5, max_norm=20.0)
+        for src in grads:
+            g.copy_(src)
+            p.grad = g
+            opt.step()
+        for t, s in zip(pads, (shift_p, shift_g)):
+            assert (t[:s] == 3.0).all() and (t[s + n:] == 3.0).all()
+        assert torch.equal(g.cpu(), grads[-1])
+        return [p.detach().clone(), opt.grad_norm.clone(), *opt.moments()[0]]
+
+    want = go(0, 0)
+    assert not torch.equal(want[0].cpu(), init)
+    for shifts in ((1, 0), (0, 1), (1, 1), (3, 2)):
+        assert all(torch.equal(a, b) for a, b in zip(go(*shifts), want)), shifts
+
+
+@pytest.mark.gpu
+def test_every_parameter_of_two_groups_and_three_types_follows_fp64():
+    shapes, types = [(6, 4, 3, 3), (300,), (129,), (64, 2)], [torch.float32, torch.bfloat16, torch.float16, torch.float32]
+    hyper = [dict(lr=1e-2, betas=(0.9, 0.999), weight_decay=1e-2)] * 2 + [dict(lr=1e-3, betas=(0.5, 0.9), weight_decay=0.5)] * 2
+    ps = params_of([t.to(d) for t, d in zip(tensors(shapes), types)])
+    flat = torch.zeros(129 + 3, device="cuda", dtype=torch.float16)
+    ps[2] = flat[3:].copy_(ps[2].detach()).requires_grad_()
+    opt = AdamW([{"params": ps[:2], **hyper[0]}, {"params": ps[2:], **hyper[2]}], max_norm=0.1)
+    m, v = [0.0] * 4, [0.0] * 4
+    for k in range(1, 4):
+        gs, before = [t.to(d) for t, d in zip(tensors(shapes, seed=k), types)], [p.detach().double().cpu() for p in ps]
+        for p, g in zip(ps, gs):
+            p.grad = g.cuda()
+        opt.step()
+        f = min(1.0, 0.1 / (math.sqrt(sum(float((g.double() ** 2).sum()) for g in gs)) + 1e-6))
+        for i, (p, g, h) in enumerate(zip(ps, gs, hyper)):
+            (b1, b2), g = h["betas"], g.double() * f
+            m[i], v[i] = b1 * m[i] + (1 - b1) * g, b2 * v[i] + (1 - b2) * g * g
+            up = (m[i] / (1 - b1 ** k)) / ((v[i] / (1 - b2 ** k)).sqrt() + 1e-8)
+            want = before[i] * (1 - h["lr"] * h["weight_decay"]) - h["lr"] * up
+            half = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[p.dtype]
+            # half a step of its type; three roundings of p; the update's ten, and what the moments are off: 4 u of terms that reach 6 f (the largest gradient) over sqrt(v)
+            noise = 4 * k * U * 6 * f / (v[i] / (1 - b2 ** k)).sqrt().clamp(min=1e-12)
+            off = (p.detach().double().cpu() - want).abs()
+            assert (off <= half * want.abs() + (2.0 ** -25 if half else 0.0) + 3 * U * (before[i].abs() + 0.1) + h["lr"] * (10 * U * (1 + up.abs()) + noise)).all(), (k, i)
