@@ -523,3 +523,32 @@ def test_launch_limits_are_those_of_each_direction():
         assert words(n + 1, H, K, D, backward) == -1, (D, H, K, backward)
         assert b"too many for one launch" in lib.asyrp_last_error()
     assert words(2 ** 31 - 1, 2 ** 31 - 1, 1, 8, 0) == -1
+
+
+@pytest.mark.gpu
+def test_bad_offsets_touch_nothing_around_the_gradients_and_the_workspace():
+    """The C entries with every output in the middle of a larger buffer."""
+    from asyrp_official_amd import _lib
+    lib, T, H, K, pad = _lib.load(), 1500, 2, 1, 4096
+    for D, nseq in ((64, 1), (128, 1), (64, 70), (128, 2)):
+        q, k, v, do = make(T, H, K, D, torch.float16, seed=9)
+        spec = _lib.PACKED_ATTENTION.pack(T, nseq, H, K, D, 1, _lib.F16, 0.125, *(H * D, D), *(K * D, D), *(K * D, D), *(H * D, D), *(H * D, D))
+        words = [lib.asyrp_packed_attention_workspace(spec, b) for b in (0, 1)]
+        assert min(words) >= 0
+
+        def room(numel, dtype):
+            t = torch.full((numel + 2 * pad,), 5.0, device="cuda", dtype=dtype)
+            return t, t[pad:pad + numel].data_ptr()
+
+        outs = {m: room(T * h * D, torch.float16) for m, h in (("out", H), ("rest", H), ("dq", H), ("dk", K), ("dv", K))}
+        stats, ws = room(2 * H * T, torch.float32), [room(max(4, w), torch.float32) for w in words]
+        for cu in ([0] * nseq + [2000], [-5] + [1500] * nseq, [900, 100] + [1400] * nseq, [0, 2 ** 31 - 1] + [-2 ** 31] * nseq, [1450] + [10] * nseq, [-2 ** 31] * (nseq + 1)):
+            cu = torch.tensor(cu[:nseq + 1], dtype=torch.int32, device="cuda")
+            stream = torch.cuda.current_stream().cuda_stream
+            for fill in (0, 1):
+                assert lib.asyrp_packed_attention_forward(0, spec, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(), outs["out"][1], stats[1], outs["rest"][1], ws[0][1], fill, stream) == 0
+            assert lib.asyrp_packed_attention_backward(0, spec, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu.data_ptr(), outs["out"][1], stats[1], outs["rest"][1], do.data_ptr(), ws[1][1],
+                                                       outs["dq"][1], outs["dk"][1], outs["dv"][1], stream) == 0
+            torch.cuda.synchronize()
+            for t in [t for t, _ in outs.values()] + [stats[0]] + [t for t, _ in ws]:
+                assert (t[:pad] == 5.0).all() and (t[-pad:] == 5.0).all()
