@@ -96,3 +96,64 @@ def test_a_training_step_of_an_encoder(bits):
         ((encoder(xo, own, cu) - target.cuda()) ** 2).mean().backward()
         opt.step()
     assert all(torch.isfinite(t).all() for t in flat)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_deltablock_step_encoder_loss_and_adamw_in_one_chain(bits):
+    """The training loop's shape: one denoising step through the frozen UNet, its x0 as patches through the encoder, a loss against an embedding, back into the DeltaBlock, and AdamW on it."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+    from oracle import sampler as osamp
+    from oracle.weights import SMALL, hash_normal
+    from util_models import hip_model, synthetic
+    from asyrp_official_amd import denoising_step
+    B, side, patch = 2, SMALL.resolution, 4
+    model = hip_model(SMALL, synthetic(SMALL, 1, seed=11), 1, max_batch=B)
+    for p in model.parameters():
+        p.requires_grad_(False)
+    delta = list(model.layer_0.parameters())
+    for p in delta:
+        p.requires_grad_(True)
+    b, one = osamp.beta_schedule().cuda(), torch.ones(B, device="cuda")
+    x = hash_normal("chain.x", (B, 3, side, side)).cuda()
+    kw = dict(models=model, logvars=None, b=b, sampling_type="ddim", eta=0.0, index=0, t_edit=500, hs_coeff=(1.0, 1.0))
+    lens = [(side // patch) ** 2] * B
+    blocks, g = weights(2, seed=3), torch.Generator().manual_seed(4)
+    embed, target = torch.randn(WIDTH, 3 * patch * patch, generator=g) * (3 * patch * patch) ** -0.5, torch.randn(B, WIDTH, generator=g)
+    own, cu = [{k: t.cuda() for k, t in blk.items()} for blk in blocks], torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+
+    def loss_of(x0, embed, blocks, target, run):
+        rows = torch.nn.functional.unfold(x0, patch, stride=patch).transpose(1, 2).reshape(-1, 3 * patch * patch)
+        h = run(torch.nn.functional.linear(rows, embed), blocks)
+        return ((h.view(B, -1, WIDTH).mean(1) - target) ** 2).mean()
+
+    opt = AdamW(delta, lr=1e-2, state_bits=bits, max_norm=1.0)
+    for k in range(3):
+        opt.zero_grad()
+        x0 = denoising_step(x, t=one * 768.0, t_next=one * 743.0, **kw)[1]
+        leaf = x0.detach().clone().requires_grad_()
+        loss = loss_of(leaf, embed.cuda(), own, target.cuda(), lambda t, w: encoder(t, w, cu))
+        (up,) = torch.autograd.grad(loss, leaf)
+        ref = x0.detach().double().cpu().requires_grad_()
+        want = loss_of(ref, embed.double(), [{n: t.double() for n, t in blk.items()} for blk in blocks], target.double(), lambda t, w: plain(t, w, lens))
+        (exact,) = torch.autograd.grad(want, ref)
+        assert abs(float(loss.detach()) / float(want.detach()) - 1) <= 0.023
+        assert float((up.double().cpu() - exact).norm() / exact.norm()) <= 0.023
+        # the chain in one piece gives the DeltaBlock what its pieces give
+        pieces = torch.autograd.grad(x0, delta, up)
+        x0 = denoising_step(x, t=one * 768.0, t_next=one * 743.0, **kw)[1]
+        loss_of(x0, embed.cuda(), own, target.cuda(), lambda t, w: encoder(t, w, cu)).backward()
+        assert all(torch.equal(p.grad, q) for p, q in zip(delta, pieces)) and any(q.any() for q in pieces)
+        before = [p.detach().clone() for p in delta]
+        opt.step()
+        norm = math.sqrt(sum(float((q.double() ** 2).sum()) for q in pieces))
+        assert abs(float(opt.grad_norm) / norm - 1) <= 2.0 ** -22
+        if k == 0:
+            f = min(1.0, 1.0 / (norm + 1e-6))
+            for p, p0, q in zip(delta, before, pieces):
+                p0, q = p0.double(), f * q.double()
+                step = p0 * (1 - 1e-2 * 1e-2) - 1e-2 * q / (q.abs() + 1e-8)
+                assert ((p.detach().double() - step).abs() <= 2.0 ** -24 * (3 * step.abs() + 1e-2 * 10 * 2)).all()
+        assert all(torch.isfinite(p).all() for p in delta)
