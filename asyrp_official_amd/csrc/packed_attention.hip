@@ -11,8 +11,8 @@
 // the first operand is simply read in the order in which the registers hold the second (rows {4h .. 4h+3, 8+4h .. 8+4h+3} of 16, h = lane / 32),
 // by the transposing 16-bit LDS read, which hands a lane four rows of one column.
 //
-// The probabilities are rounded to the operands' type before P v, P^T do and dS k, dS^T q (half a step per term, relative to it); every
-// sum, the row maximum, the row sum and delta are fp32.  There is no atomic: dq and dk/dv are two kernels that each form S
+// P is rounded to the operands' type before P v and P^T do, dS before dS k and dS^T q (half a step per term, relative to it; f16 under powers of two, so that small ones keep their
+// bits; dS as two terms where the mask cuts); every sum, the row maximum, the row sum and delta are fp32.  There is no atomic: dq and dk/dv are two kernels that each form S
 // again (7 products instead of 5), and the result does not depend on the order in which workgroups run.
 #include "kernels.h"
 #include "../../include/asyrp.h"
@@ -55,7 +55,7 @@ struct PackedAttnArgs {
   void *out, *dq, *dk, *dv;
   void* rest;                // [T][Hq][D]: what rounding took from o, times FINER (delta of the unrounded o halves what dq and dk are off); null: not kept
   // [Hq][T] reference and log2 of the sum.  Apart, since a large score less a reference close to it is exact, and their own sum is not: as one float, P was off by
-  // 0.5 % at scores of 1e5 and of any size at 2e7.
+  // 0.5 % at scores of 1e5 and of any size at 2e7.  (A subtraction an element: 2 % of the backward.)
   float2* sums;
   float* delta;              // [Hq][T]
   const int* cu;
@@ -349,7 +349,8 @@ __device__ __forceinline__ void add_ds(f32x16 (&acc)[DP / 32], const char* tile,
 // dS on its way into f16 has a power of two for every column (query or key) that keeps what matters of it inside f16's range: gradients of a mean loss over a long
 // sequence put dS at 2^-20 and less, where f16 has few bits or none (without it 4 % of dq at do = 1e-4 and 3000 rows), others over 65504.  It is found as
 // a softmax finds its reference: the first values of a column that are not zero are taken to 2^8, and where later ones pass 2^14 it falls and the sums with it.  All steps are
-// by powers of two, exact.  What is then too small for f16 is 2^-32 of the column's largest.  bf16 has the range of fp32.
+// by powers of two, exact.  What is then too small for f16 is 2^-32 of the column's largest.  bf16 has the range of fp32.  (8192 rows, 8 heads, both directions: of 64 447 us without and 454 with it, of 128
+// 746 and 755; with a multiplication for every value of dS, instead of in P's exponent or factor, 472 and 771.)
 template <typename T> struct Range {
   static constexpr float up = 1.f, shift = 0.f;
   template <int N> __device__ __forceinline__ void fit(f32x16&, f32x16 (&)[N]) {}
@@ -414,7 +415,7 @@ struct FwdWave {
   // `krow` of `k` on), so that one's products run under the other's exponentials.
   __device__ __forceinline__ void half(f32x16& cur, f32x16& next, const char* k, int krow, const char* v, int vrow, int lane) {
     // The reference moves only where a column's maximum has outgrown it by LAG powers of two (and in the first half): most halves leave the sums as they are.  The
-    // exponentials stay under 2^8, in f16 under 2^10.  (Both have to leave room: base() is rounded, and that reaches 2^4 at scores of 1e8.)
+    // exponentials stay under 2^8, in f16 under 2^10.  (There has to be room: a base is rounded, and that is worth up to 2^4 at scores of 1e8.)
     if (__any(!((mx - m) * sc <= LAG))) {
       const float mn = fmaxf(m, mx), keep = m > -INFINITY ? exp2_fast((m - mn) * sc) : 0.f;
       m = mn;
@@ -548,8 +549,8 @@ __global__ __launch_bounds__(256, 2) void packed_attn_fwd_kernel(const PackedAtt
   if (there && p.sums && h == 0) p.sums[(long long)head * p.T + f.start + row] = make_float2(w.base(), log2f(l));
 }
 
-// dq, and delta = rowsum(do * o) for the other kernel.  As the forward, with dP beside S; three products a tile and no running maximum.  172 us for the
-// packed sequences above: 0.84 PFLOP/s.
+// dq, and delta = rowsum(do * o) for the other kernel.  As the forward, with dP beside S; three products a tile and no running maximum.  178 us for the
+// packed sequences above: 0.81 PFLOP/s.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char kt[2][BN * DP * 2], vt[2][BN * DP * 2];
@@ -658,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dq_kernel(const PackedAttn
 constexpr float LIFT = 14.f, LIFTED = 0x1p14f;
 
 // dk and dv of 128 keys: over the query heads that share them and the query tiles that see them.  A wave's 32 keys and values and both sums stay in its
-// registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 28 us, bound by
+// registers, which heads of up to 64 columns leave room for two waves a SIMD for.  32 f16 images of 197 rows, 12 heads of 64: 29 us, bound by
 // latency (four tiles a workgroup).
 template <typename T, int DP>
 __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAttnArgs p) {
@@ -810,8 +811,8 @@ template <> struct Handed<_Float16> {
 // The same for heads wider than 64, where one wave cannot hold both sums, its keys' and values' fragments and the scores in half a SIMD's registers, and a
 // wave alone on its SIMD waits out every exponential: eight waves, two on each SIMD, share the four products of 128 keys.  The first of a pair forms S and P
 // and sums dv; it hands P over through LDS, and the second forms dP and dS and sums dk one tile behind, so that the only wait is the barrier that there is for the
-// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, 277 us so (0.69 PFLOP/s), and
-// 3 % less with constant places of its tiles.
+// tiles.  Three tiles are held.  16 query heads on 4, 128 wide, 8192 rows, causal: 435 us with one wave per SIMD, 310 us with pairs that both form S, 277 us so, and
+// 257 us (0.74 PFLOP/s) with constant places of its tiles.
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void packed_attn_dkv_pair_kernel(const PackedAttnArgs p) {
   __shared__ __attribute__((aligned(16))) char qt[3][BN * DP * 2], gt[3][BN * DP * 2];

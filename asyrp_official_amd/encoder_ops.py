@@ -142,7 +142,8 @@ def packed_attention(q, k, v, cu_seqlens, *, causal=False, scale=None, out=None)
 
     Returns [tokens, heads, head_dim].  Rows behind the last sequence are zero there and in the gradients.  `out` (without gradients only;
     the result's type and shape, laid out as q may be, beside q, k and v and not over them) takes the result and keeps what it holds in those rows.  Sums and softmax statistics are float32;
-    probabilities are rounded to the inputs' type before they multiply v.  A value that is not finite may reach every row of its own sequence, the
+    probabilities, and in the backward pass those and the scores' gradients, are rounded to the inputs' type before they multiply (float16: under powers of two that keep small
+    ones' bits).  A call with gradients keeps the result, as much again for its roundings, and two float32 per token and head until its backward pass.  A value that is not finite may reach every row of its own sequence, the
     rows before it included, and no other sequence.  Results do not depend on the order in which the card works."""
     device = _tensor(q, "q", None, _HALF)
     same = (q.dtype,)
