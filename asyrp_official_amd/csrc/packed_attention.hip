@@ -179,8 +179,9 @@ __device__ __forceinline__ int wave_sum(int v) {
   return __builtin_amdgcn_readlane(v, 63);
 }
 
-// The sequence and the row tile that tile number `t` of the launch stands for.  Tiles are numbered sequence by sequence; the numbers
-// behind the last one share the rows behind the last sequence.  Every wave finds it by itself: 64 lengths at a time, summed over the wave.
+// The sequence and the row tile that tile number `t` of the launch stands for.  Up to 64 sequences: tiles are numbered sequence by sequence, and the numbers
+// behind the last one share the rows behind the last sequence; every wave finds its own from the 64 lengths, summed over the wave.  More: sequence b's tiles are numbered from
+// offset[b] / BM + b on, which leaves room for all of them and is found by looking at 64 offsets at a time (100000 sequences of one row: the forward 50 ms when the lengths in front were summed).
 // Offsets are held inside [0, T] and never fall, so that no value of `cu` leads outside the tensors.
 struct TileAt { long long start; int len, row0; int idle; int idles; int low, end; };
 // lane `src`'s value as one that the compiler knows to be the same in all lanes (all lanes active, src < 64)
@@ -192,7 +193,6 @@ __device__ __forceinline__ int uniform(int v, int src) { return __builtin_amdgcn
 enum { IN_ORDER, BY_WEIGHT, BY_WEIGHT_FROM_END };
 __device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T, int t, int tiles, int lane, int order) {
   TileAt f{0, 0, 0, 0, 1, 0, 0};
-  int before = 0;
   if (order != IN_ORDER && nseq <= 64) {
     long long s = 0, e = 0;
     if (lane < nseq) { s = cu[lane]; e = cu[lane + 1]; }
@@ -221,40 +221,62 @@ __device__ __forceinline__ TileAt find_tile(const int* cu, int nseq, long long T
     f.end = uniform((int)e, nseq - 1);
     return f;
   }
-  bool found = false;
-  int high = 0, low = 0;
-  for (int b0 = 0; b0 < nseq; b0 += 64) {
-    const int b = b0 + lane;
-    long long s = 0, e = 0;
-    if (b < nseq) { s = cu[b]; e = cu[b + 1]; }
+  if (nseq > 64) {
+    const auto first = [&](int b) { const long long s = cu[b]; return (int)((s < 0 ? 0 : s > T ? T : s) / BM) + b; };      // b's first tile
+    const int behind = first(nseq);
+    if (t >= behind) {
+      const long long s = cu[0], e = cu[nseq];
+      f.idle = 1 + (t - behind);
+      f.idles = tiles - behind;
+      f.low = (int)(s < 0 ? 0 : s > T ? T : s);
+      f.end = (int)(e < f.low ? f.low : e > T ? T : e);
+      return f;
+    }
+    f.idle = 1;                                           // a number that stands for nothing, unless the search ends at a sequence with so many tiles
+    f.end = (int)T;
+    int lo = 0, hi = nseq;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, b = lo + lane * step;
+      const int at_or_before = __popcll(__ballot(b < hi && first(b < hi ? b : lo) <= t));
+      if (!at_or_before) return f;
+      lo += (at_or_before - 1) * step;
+      hi = min(lo + step, hi);
+    }
+    long long s = cu[lo], e = cu[lo + 1];
     s = s < 0 ? 0 : s > T ? T : s;
-    e = e < s ? s : e > T ? T : e;                        // T < 2^31
-    const int n = (int)((e - s + BM - 1) / BM);
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(sum, o);
-      if (lane >= o) sum += up;
+    e = e < s ? s : e > T ? T : e;
+    const long long row0 = (long long)(t - first(lo)) * BM;
+    if (row0 >= 0 && row0 < e - s) {
+      f.start = __builtin_amdgcn_readfirstlane((int)s);
+      f.len = __builtin_amdgcn_readfirstlane((int)(e - s));
+      f.row0 = __builtin_amdgcn_readfirstlane((int)row0);
+      f.idle = 0;
     }
-    const int first = before + sum - n;
-    const unsigned long long hit = __ballot(n > 0 && t >= first && t < first + n);
-    if (hit) {
-      const int src = __ffsll(hit) - 1;
-      f.start = uniform((int)s, src);
-      f.len = uniform((int)e, src) - (int)f.start;
-      f.row0 = (t - uniform(first, src)) * BM;
-      found = true;
-      break;
-    }
-    before = min(before + uniform(sum, 63), (1 << 30) - 1);     // (more tiles than any launch has: only offsets that fall lead there)
-    high = uniform((int)e, nseq - 1 - b0 < 63 ? nseq - 1 - b0 : 63);
-    if (b0 == 0) low = uniform((int)s, 0);
+    return f;
   }
-  if (!found) {
-    f.idle = 1 + (t - before);
-    f.idles = tiles - before;
-    f.low = low;
-    f.end = high;
+  long long s = 0, e = 0;
+  if (lane < nseq) { s = cu[lane]; e = cu[lane + 1]; }
+  s = s < 0 ? 0 : s > T ? T : s;
+  e = e < s ? s : e > T ? T : e;                          // T < 2^31
+  const int n = (int)((e - s + BM - 1) / BM);
+  int sum = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(sum, o);
+    if (lane >= o) sum += up;
+  }
+  const unsigned long long hit = __ballot(n > 0 && t >= sum - n && t < sum);
+  if (hit) {
+    const int src = __ffsll(hit) - 1;
+    f.start = uniform((int)s, src);
+    f.len = uniform((int)e, src) - (int)f.start;
+    f.row0 = (t - uniform(sum - n, src)) * BM;
+  } else {
+    const int total = uniform(sum, 63);
+    f.idle = 1 + (t - total);
+    f.idles = tiles - total;
+    f.low = uniform((int)s, 0);
+    f.end = uniform((int)e, nseq - 1);
   }
   return f;
 }

@@ -552,3 +552,42 @@ def test_bad_offsets_touch_nothing_around_the_gradients_and_the_workspace():
             torch.cuda.synchronize()
             for t in [t for t, _ in outs.values()] + [stats[0]] + [t for t, _ in ws]:
                 assert (t[:pad] == 5.0).all() and (t[-pad:] == 5.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
+@pytest.mark.parametrize("D", [32, 128])
+def test_thousands_of_sequences_read_as_in_small_batches(D, causal):
+    """Every sequence by itself gives the same bits: in calls of up to 50 sequences and in one of 5000, empty ones, rows in front of the first and behind the last among them."""
+    g = torch.Generator().manual_seed(0)
+    lens = torch.tensor([0, 1, 1, 2, 3, 7, 64, 127, 128, 129, 200])[torch.randint(0, 11, (5000,), generator=g)].tolist()
+    lens[:3], lens[70:140], lens[-2:] = [0, 130, 0], [0] * 70, [1, 0]
+    ahead, T = 300, sum(lens)
+    q, k, v, do = make(ahead + T + 500, 2, 1, D, torch.float16, seed=1)
+    got = run(q, k, v, do, offsets(lens) + ahead, causal)
+    at = 0
+    for i in range(0, len(lens), 50):
+        part = lens[i:i + 50]
+        r = slice(ahead + at, ahead + at + sum(part))
+        at += sum(part)
+        want = run(q[r], k[r], v[r], do[r], offsets(part), causal)
+        for m in got:
+            assert torch.equal(got[m][r], want[m]), (m, i)
+    for m in got:
+        assert not got[m][:ahead].any() and not got[m][ahead + T:].any()
+
+
+@pytest.mark.gpu
+def test_the_time_of_many_sequences_goes_with_their_number():
+    """200000 sequences of one row, both directions: some milliseconds, where every workgroup reading all offsets up to its own took 200 in the forward alone."""
+    n = 200_000
+    q, k, v, do = make(n, 1, 1, 64, torch.float16)
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    got = run(q, k, v, do, cu, True)
+    assert torch.equal(got["o"], v) and torch.equal(got["dv"], do)
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    run(q, k, v, do, cu, True)
+    end.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(end) < 50
