@@ -807,7 +807,7 @@ __global__ __launch_bounds__(256, 2) void packed_attn_dkv_kernel(const PackedAtt
 // P in 16 bits on its way from one wave to another, finer than the operands' type, so that dS is nearly rounded once in effect.  It comes 2^14 times as large (LIFT), so that what
 // is small has all its bits too: for bf16 operands f16 holds 11 of them from P = 2^-28 on (and under it steps of 2^-38); for f16 ones P, which is never negative, takes five bits of
 // exponent and eleven of mantissa: 12 bits from P = 2^-30 on, steps of 2^-41 under it.  (As f16 without the factor, the dk of keys that few queries see lost its bits: 26 half steps
-// of bf16 where P is 1e-7.)  The clamp is for P that does not belong to its sum: its bits would reach into the neighbour's.
+// of bf16 where P is 1e-7.)  bf16's dk is summed under the factor: over 2^113 it becomes infinite.  The clamp is for P that does not belong to its sum: its bits would reach into the neighbour's.
 template <typename T> struct Handed;
 template <> struct Handed<__bf16> {
   typedef Frag<_Float16>::V V;
